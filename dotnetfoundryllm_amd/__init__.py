@@ -142,6 +142,16 @@ class DeviceBuffer:
         _check(N.dev.fllm_buf_create(ctx.h, nbytes, C.byref(h)))
         self.h, self.n, self.ctx = h, nbytes, ctx
 
+    @classmethod
+    def wrap(cls, ctx, device_ptr, nbytes):
+        """A buffer over the caller's device memory, which has to outlive it. Another library's tensor is
+        such memory when both run on one HIP runtime: torch brings its own, so import torch first."""
+        h = C.c_void_p()
+        _check(N.dev.fllm_buf_wrap(ctx.h, device_ptr, nbytes, C.byref(h)))
+        b = cls.__new__(cls)
+        b.h, b.n, b.ctx = h, nbytes, ctx
+        return b
+
     def write(self, arr, offset=0):
         arr = np.ascontiguousarray(arr)
         _check(N.dev.fllm_buf_write(self.h, offset, arr.ctypes.data_as(C.c_void_p), arr.nbytes))
@@ -187,6 +197,109 @@ def gemv_time(ctx, tensor_type, w_bufs, rows, cols, x_buf, y_buf, iters, layout=
         _check(N.dev.fllm_gemv_time_ex(ctx.h, tensor_type, C.cast(arr, C.POINTER(C.c_void_p)), len(w_bufs), rows,
                                        cols, x_buf.h, y_buf.h, iters, layout, C.byref(out)))
     return out.value
+
+
+# ----------------------------------------------------------------------------------------
+NO_WINDOW = 0x7FFFFFFF
+
+
+class Rows:
+    """Rows of a matrix in a DeviceBuffer (fllm_rows): ld elements apart, `offset` bytes into it."""
+
+    def __init__(self, buf, ld, tensor_type=F32, offset=0):
+        self.buf = buf  # kept alive
+        self.d = N.RowsDesc(buf.h, offset, ld, tensor_type, 0)
+        self.ref = C.byref(self.d)
+
+
+class PagedKvCache:
+    """The keys and values of several sequences in pages, F16 / Q8_0 / Q4_0, for all layers (fllm_pages);
+    in `memory` (a DeviceBuffer) at `offset`, or in memory of its own."""
+
+    def __init__(self, ctx, tensor_type, n_layers, n_kv_heads, head_dim, page_size, n_pages, memory=None, offset=0):
+        self.ctx, self.memory = ctx, memory
+        self.desc = N.PagesDesc(tensor_type, n_layers, n_kv_heads, head_dim, page_size, n_pages)
+        h = C.c_void_p()
+        _check(N.dev.fllm_pages_create(ctx.h, C.byref(self.desc), memory.h if memory else None, offset, C.byref(h)))
+        self.h = h
+
+    @staticmethod
+    def bytes_for(tensor_type, n_layers, n_kv_heads, head_dim, page_size, n_pages):
+        d, n = N.PagesDesc(tensor_type, n_layers, n_kv_heads, head_dim, page_size, n_pages), C.c_uint64()
+        _check(N.dev.fllm_pages_bytes(C.byref(d), C.byref(n)))
+        return n.value
+
+    def batch(self, n_heads, window=NO_WINDOW):
+        if not self.h:
+            raise ObjectDisposedException("PagedKvCache")
+        return PagedBatch(self, n_heads, window)
+
+    def close(self):
+        if self.h:
+            N.dev.fllm_pages_destroy(self.h)
+            self.h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+
+class PagedBatch:
+    """The sequences that a step works on (fllm_batch), and the calls of its layers."""
+
+    def __init__(self, pages, n_heads, window):
+        h = C.c_void_p()
+        _check(N.dev.fllm_batch_create(pages.h, n_heads, window, C.byref(h)))
+        self.h, self.pages = h, pages
+
+    def _handle(self):
+        if not self.h:
+            raise ObjectDisposedException("PagedBatch")
+        return self.h
+
+    def set(self, new_tokens, lengths, tables):
+        """Per sequence: new tokens, positions with them, and its pages (a row of the 2-d `tables`)."""
+        n, k = (np.ascontiguousarray(a, dtype=np.int32).reshape(-1) for a in (new_tokens, lengths))
+        t = np.ascontiguousarray(tables, dtype=np.int32)
+        if n.size != k.size or t.ndim != 2 or t.shape[0] != n.size:
+            raise ArgumentException("new_tokens, lengths and the rows of tables must be as many")
+        _check(N.dev.fllm_batch_set(self._handle(), n.size, _iptr(n), _iptr(k), _iptr(t), t.shape[1]))
+
+    def append(self, layer, k, v):
+        """The new tokens' key and value rows into their pages."""
+        _check(N.dev.fllm_pages_append(self._handle(), layer, k.ref, v.ref))
+
+    def read(self, layer, k=None, v=None, new_only=False):
+        """Rows of every position (or of the new tokens) out of the pages."""
+        _check(N.dev.fllm_pages_read(self._handle(), layer, 1 if new_only else 0, k.ref if k else None,
+                                     v.ref if v else None))
+
+    def attention(self, layer, q, out, scale, softcap=0.0):
+        """Attention of the new tokens over their sequences' pages."""
+        _check(N.dev.fllm_pages_attention(self._handle(), layer, q.ref, out.ref, scale, softcap))
+
+    def close(self):
+        if self.h:
+            N.dev.fllm_batch_destroy(self.h)
+            self.h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *a):
+        self.close()
+
+
+def draft_verify(ctx, n_seqs, n_draft, vocab, target, tokens, u_accept, u_sample, out_tokens, out_counts, draft=None,
+                 counts=None):
+    """Drafted tokens against the target's probabilities (fllm_draft_verify): kept tokens, then the drawn
+    one, then -1 in out_tokens, their number in out_counts. target, draft: Rows; the others DeviceBuffers."""
+    hd = lambda b: b.h if b is not None else None  # noqa: E731
+    d = N.DraftDesc(n_seqs, n_draft, vocab, 0, target.d, draft.d if draft is not None else N.RowsDesc(), hd(tokens),
+                    hd(counts), hd(u_accept), hd(u_sample), hd(out_tokens), hd(out_counts))
+    _check(N.dev.fllm_draft_verify(ctx.h, C.byref(d)))
 
 
 # ----------------------------------------------------------------------------------------

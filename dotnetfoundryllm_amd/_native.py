@@ -73,6 +73,23 @@ class GenerateStats(C.Structure):
                 ("decode_ms", C.c_double), ("tokens_per_second", C.c_double), ("finish_reason", C.c_int32)]
 
 
+class PagesDesc(C.Structure):
+    _fields_ = [("type", C.c_int32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("page_size", C.c_int32), ("n_pages", C.c_int32)]
+
+
+class RowsDesc(C.Structure):
+    _fields_ = [("buf", C.c_void_p), ("offset", C.c_uint64), ("ld", C.c_int64), ("type", C.c_int32),
+                ("reserved", C.c_int32)]
+
+
+class DraftDesc(C.Structure):
+    _fields_ = [("n_seqs", C.c_int32), ("n_draft", C.c_int32), ("vocab", C.c_int32), ("reserved", C.c_int32),
+                ("target", RowsDesc), ("draft", RowsDesc), ("tokens", C.c_void_p), ("counts", C.c_void_p),
+                ("u_accept", C.c_void_p), ("u_sample", C.c_void_p), ("out_tokens", C.c_void_p),
+                ("out_counts", C.c_void_p)]
+
+
 P = C.c_void_p
 I32, I64, U64, F32_, F64 = C.c_int32, C.c_int64, C.c_uint64, C.c_float, C.c_double
 PI32, PI64, PU64, PF32, PF64 = (C.POINTER(C.c_int32), C.POINTER(C.c_int64), C.POINTER(C.c_uint64),
@@ -122,6 +139,7 @@ DEVICE_SIGS = {
     "fllm_dequantize_noalloc": (I32, [P, I32, P, U64, PF32, I64]),
     "fllm_element_count": (I32, [I32, I64, PI64]),
     "fllm_buf_create": (I32, [P, U64, PP]),
+    "fllm_buf_wrap": (I32, [P, P, U64, PP]),
     "fllm_buf_destroy": (I32, [P]),
     "fllm_buf_write": (I32, [P, U64, P, U64]),
     "fllm_buf_read": (I32, [P, U64, P, U64]),
@@ -130,6 +148,16 @@ DEVICE_SIGS = {
     "fllm_gemv_pack": (I32, [P, I32, P, U64, I64, I64, P]),
     "fllm_gemv_ex": (I32, [P, I32, P, U64, I64, I64, P, P, I32]),
     "fllm_gemv_time_ex": (I32, [P, I32, PP, I32, I64, I64, P, P, I32, I32, PF64]),
+    "fllm_pages_bytes": (I32, [C.POINTER(PagesDesc), PU64]),
+    "fllm_pages_create": (I32, [P, C.POINTER(PagesDesc), P, U64, PP]),
+    "fllm_pages_destroy": (I32, [P]),
+    "fllm_batch_create": (I32, [P, I32, I32, PP]),
+    "fllm_batch_set": (I32, [P, I32, PI32, PI32, PI32, I64]),
+    "fllm_batch_destroy": (I32, [P]),
+    "fllm_pages_append": (I32, [P, I32, C.POINTER(RowsDesc), C.POINTER(RowsDesc)]),
+    "fllm_pages_read": (I32, [P, I32, I32, C.POINTER(RowsDesc), C.POINTER(RowsDesc)]),
+    "fllm_pages_attention": (I32, [P, I32, C.POINTER(RowsDesc), C.POINTER(RowsDesc), F32_, F32_]),
+    "fllm_draft_verify": (I32, [P, C.POINTER(DraftDesc)]),
     "fllm_seq_set_profile": (I32, [P, I32]),
     "fllm_seq_profile_count": (I32, [P, PI32]),
     "fllm_seq_profile_entry": (I32, [P, I32, C.c_char_p, I32, PI64, PF64, PF64]),

@@ -42,7 +42,8 @@ def _run(cmd, cwd):
     return out
 
 
-DEVICE_SRCS = ["csrc/kernels.hip", "csrc/gemv.hip", "csrc/attention.hip", "csrc/prefill.hip", "csrc/pf_gemm8.hip", "csrc/api.hip"]
+DEVICE_SRCS = ["csrc/kernels.hip", "csrc/gemv.hip", "csrc/attention.hip", "csrc/prefill.hip", "csrc/pf_gemm8.hip", "csrc/pages.hip",
+               "csrc/pages_attention.hip", "csrc/draft.hip", "csrc/api.hip", "csrc/api_pages.hip"]
 
 
 def build_device_lib(verbose=False):

@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <new>
 #include <string>
 #include <thread>
 #include <vector>
@@ -18,8 +19,8 @@
 #include "attention.hpp"
 #include "gemv.hpp"
 #include "kernels.hpp"
+#include "objects.hpp"
 #include "prefill.hpp"
-#include "staging.hpp"
 
 using namespace fllm;
 
@@ -28,7 +29,7 @@ using namespace fllm;
 // =====================================================================================
 static thread_local std::string g_err;
 
-static int32_t fail(int32_t code, const char* fmt, ...) {
+int32_t fllm::fail(int32_t code, const char* fmt, ...) {
     char buf[512];
     va_list ap;
     va_start(ap, fmt);
@@ -38,33 +39,12 @@ static int32_t fail(int32_t code, const char* fmt, ...) {
     return code;
 }
 
-#define HIP_TRY(expr)                                                                          \
-    do {                                                                                       \
-        hipError_t _e = (expr);                                                                \
-        if (_e != hipSuccess) return fail(FLLM_E_DEVICE, "%s: %s", #expr, hipGetErrorString(_e)); \
-    } while (0)
-
-#define NOT_NULL(p)                                                  \
-    do {                                                             \
-        if (!(p)) return fail(FLLM_E_NULL, "%s must not be null", #p); \
-    } while (0)
-
 extern "C" const char* fllm_last_error(void) { return g_err.c_str(); }
 extern "C" int32_t fllm_version(void) { return 100; }
 
 // =====================================================================================
 // objects
 // =====================================================================================
-struct fllm_ctx {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    int n_cu = 0;
-    int64_t hbm = 0;
-    Staging stage;
-    uint8_t* scratch = nullptr;  // this device's address of the no-allocation scratch array
-    hipError_t scratch_err = hipSuccess;  // why it could not be resolved, if so
-};
-
 // Scratch of fllm_dequantize_noalloc: the staged source blocks (kNoallocSrcBytes plus the slack the
 // dequant kernel may read past them) and the dequantized floats (kNoallocElems). Each device holds
 // its own copy for the life of the process. On the host the array's name is no device address: its
@@ -93,14 +73,6 @@ static hipError_t scratch_init(int device, uint8_t** out) {
     *out = g_scratch_dev[device];
     return hipSuccess;
 }
-
-struct fllm_buf {
-    fllm_ctx* ctx = nullptr;
-    uint8_t* ptr = nullptr;
-    uint64_t n = 0;
-};
-
-static const uint64_t kPad = 256;  // slack after every weight allocation for aligned over-reads
 
 struct Tensor {
     uint8_t* ptr = nullptr;
@@ -255,6 +227,7 @@ extern "C" int32_t fllm_ctx_destroy(fllm_ctx* ctx) {
     hipSetDevice(ctx->device);
     hipStreamSynchronize(ctx->stream);
     staging_free(ctx->stage);
+    if (ctx->ws.ptr) hipFree(ctx->ws.ptr);
     hipStreamDestroy(ctx->stream);
     delete ctx;
     return FLLM_OK;
@@ -370,11 +343,29 @@ extern "C" int32_t fllm_buf_create(fllm_ctx* ctx, uint64_t nbytes, fllm_buf** ou
     return FLLM_OK;
 }
 
+extern "C" int32_t fllm_buf_wrap(fllm_ctx* ctx, void* device_ptr, uint64_t nbytes, fllm_buf** out) {
+    NOT_NULL(ctx);
+    NOT_NULL(out);
+    *out = nullptr;
+    NOT_NULL(device_ptr);
+    if ((uintptr_t)device_ptr % 16 != 0) return fail(FLLM_E_ARG, "device_ptr must be 16-byte aligned");
+    fllm_buf* b = new (std::nothrow) fllm_buf();
+    if (!b) return fail(FLLM_E_OOM, "out of host memory");
+    b->ctx = ctx;
+    b->ptr = (uint8_t*)device_ptr;
+    b->n = nbytes;
+    b->owned = false;
+    *out = b;
+    return FLLM_OK;
+}
+
 extern "C" int32_t fllm_buf_destroy(fllm_buf* b) {
     if (!b) return FLLM_OK;
-    hipSetDevice(b->ctx->device);
-    hipStreamSynchronize(b->ctx->stream);
-    hipFree(b->ptr);
+    if (b->owned) {
+        hipSetDevice(b->ctx->device);
+        hipStreamSynchronize(b->ctx->stream);
+        hipFree(b->ptr);
+    }
     delete b;
     return FLLM_OK;
 }
@@ -415,7 +406,10 @@ static int32_t check_gemv_args(int32_t type, fllm_buf* w, uint64_t w_offset, int
     if (w_offset % 16 != 0) return fail(FLLM_E_ARG, "weight offset must be 16-byte aligned");
     uint64_t wb = type_bytes(type, rows * cols);
     if (w_offset > w->n || wb > w->n - w_offset) return fail(FLLM_E_ARG, "weight buffer too small");
+    // the kernels may read up to kPad bytes past a matrix, which every allocated buffer has behind it
+    if (!w->owned && kPad > w->n - w_offset - wb) return fail(FLLM_E_ARG, "a wrapped buffer ends %d bytes or more behind the weights", (int)kPad);
     if ((uint64_t)cols * 4 > x->n) return fail(FLLM_E_ARG, "x buffer too small");
+    if (!x->owned && kPad > x->n - (uint64_t)cols * 4) return fail(FLLM_E_ARG, "a wrapped buffer ends %d bytes or more behind x", (int)kPad);
     if ((uint64_t)rows * 4 > y->n) return fail(FLLM_E_ARG, "y buffer too small");
     return FLLM_OK;
 }
@@ -443,6 +437,7 @@ extern "C" int32_t fllm_gemv_pack(fllm_ctx* ctx, int32_t type, fllm_buf* src, ui
     if (src_offset % 16 != 0) return fail(FLLM_E_ARG, "source offset must be 16-byte aligned");
     const uint64_t nb = type_bytes(type, rows * cols);
     if (src_offset > src->n || nb > src->n - src_offset) return fail(FLLM_E_ARG, "source buffer too small");
+    if (!src->owned && kPad > src->n - src_offset - nb) return fail(FLLM_E_ARG, "a wrapped buffer ends %d bytes or more behind the weights", (int)kPad);
     if (nb > dst->n) return fail(FLLM_E_ARG, "destination buffer too small");
     if (dst == src) return fail(FLLM_E_ARG, "the regrouping is not in place");
     HIP_TRY(hipSetDevice(ctx->device));

@@ -1,0 +1,382 @@
+// api_pages.hip — the paged K/V cache and the draft check in the C ABI (include/fllm.h): descriptions,
+// batches and argument checks; the kernels are in pages.hip, pages_attention.hip and draft.hip.
+#include <math.h>
+#include <string.h>
+
+#include <mutex>
+#include <new>
+#include <vector>
+
+#include "objects.hpp"
+#include "pages.hpp"
+#include "pages_plan.hpp"
+
+using namespace fllm;
+
+struct fllm_pages {
+    fllm_ctx* ctx = nullptr;
+    fllm_pages_desc d{};
+    uint8_t* ptr = nullptr;
+    bool owned = false;
+    uint64_t cell = 0;
+    int n_batches = 0;
+    bool disposed = false;
+};
+
+struct fllm_batch {
+    fllm_pages* p = nullptr;
+    int n_heads = 0, window = 0;
+    BatchPlan plan;
+    // the plan's arrays on the device and the pinned block that they are copied from; `sent` says when
+    // the last copy has read it
+    uint8_t *dev = nullptr, *pin = nullptr;
+    uint64_t cap = 0;
+    hipEvent_t sent = nullptr;
+    bool in_flight = false;
+    BatchView view{};
+};
+
+// Runs a body that may allocate on the host: no exception crosses the ABI.
+template <typename F>
+static int32_t guarded(F body) {
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        return fail(FLLM_E_OOM, "out of host memory");
+    } catch (...) {
+        return fail(FLLM_E_INVALID_OP, "unexpected exception");
+    }
+}
+
+// =====================================================================================
+// pages
+// =====================================================================================
+extern "C" int32_t fllm_pages_bytes(const fllm_pages_desc* desc, uint64_t* out) {
+    NOT_NULL(desc);
+    NOT_NULL(out);
+    BatchError e;
+    if (pages_desc_check(*desc, out, &e)) return fail(e.code, "%s", e.text);
+    return FLLM_OK;
+}
+
+extern "C" int32_t fllm_pages_create(fllm_ctx* ctx, const fllm_pages_desc* desc, fllm_buf* mem, uint64_t offset,
+                                     fllm_pages** out) {
+    NOT_NULL(ctx);
+    NOT_NULL(desc);
+    NOT_NULL(out);
+    *out = nullptr;
+    uint64_t bytes = 0;
+    BatchError err;
+    if (pages_desc_check(*desc, &bytes, &err)) return fail(err.code, "%s", err.text);
+    if (mem) {
+        if (mem->ctx != ctx) return fail(FLLM_E_ARG, "the buffer belongs to another context");
+        if (offset % 16 != 0) return fail(FLLM_E_ARG, "offset must be a multiple of 16");
+        if (offset > mem->n || bytes > mem->n - offset)
+            return fail(FLLM_E_ARG, "the pages take %llu bytes at %llu of a buffer of %llu", (unsigned long long)bytes,
+                        (unsigned long long)offset, (unsigned long long)mem->n);
+    }
+    fllm_pages* p = new (std::nothrow) fllm_pages();
+    if (!p) return fail(FLLM_E_OOM, "out of host memory");
+    p->ctx = ctx;
+    p->d = *desc;
+    p->cell = pages_cell_bytes(*desc);
+    if (mem) {
+        p->ptr = mem->ptr + offset;
+    } else {
+        hipError_t e = hipSetDevice(ctx->device);
+        if (e == hipSuccess) e = hipMalloc(&p->ptr, bytes);
+        if (e != hipSuccess) {
+            delete p;
+            return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "hipMalloc(%llu): %s", (unsigned long long)bytes,
+                        hipGetErrorString(e));
+        }
+        p->owned = true;
+        e = hipMemsetAsync(p->ptr, 0, bytes, ctx->stream);
+        if (e != hipSuccess) {
+            hipFree(p->ptr);
+            delete p;
+            return fail(FLLM_E_DEVICE, "hipMemsetAsync: %s", hipGetErrorString(e));
+        }
+    }
+    *out = p;
+    return FLLM_OK;
+}
+
+static void pages_free(fllm_pages* p) {
+    hipSetDevice(p->ctx->device);
+    hipStreamSynchronize(p->ctx->stream);
+    if (p->owned) hipFree(p->ptr);
+    delete p;
+}
+
+extern "C" int32_t fllm_pages_destroy(fllm_pages* p) {
+    if (!p) return FLLM_OK;
+    p->disposed = true;
+    if (p->n_batches == 0) pages_free(p);
+    return FLLM_OK;
+}
+
+// =====================================================================================
+// batches
+// =====================================================================================
+extern "C" int32_t fllm_batch_create(fllm_pages* p, int32_t n_heads, int32_t window, fllm_batch** out) {
+    NOT_NULL(p);
+    NOT_NULL(out);
+    *out = nullptr;
+    if (p->disposed) return fail(FLLM_E_DISPOSED, "the pages were destroyed");
+    if (n_heads < 1 || n_heads > 65535 || n_heads % p->d.n_kv_heads != 0)
+        return fail(FLLM_E_ARG, "%d query heads over %d kv heads", n_heads, p->d.n_kv_heads);
+    if (window < 1) return fail(FLLM_E_ARG_RANGE, "window must be positive");
+    HIP_TRY(hipSetDevice(p->ctx->device));
+    return guarded([&]() -> int32_t {
+        fllm_batch* b = new fllm_batch();
+        hipError_t e = hipEventCreateWithFlags(&b->sent, hipEventDisableTiming);
+        if (e != hipSuccess) {
+            delete b;
+            return fail(FLLM_E_DEVICE, "hipEventCreate: %s", hipGetErrorString(e));
+        }
+        b->p = p;
+        b->n_heads = n_heads;
+        b->window = window;
+        p->n_batches++;
+        *out = b;
+        return FLLM_OK;
+    });
+}
+
+// Room for n bytes on the device and in the pinned block. The old memory may still be read by enqueued
+// calls: they are waited for first.
+static hipError_t batch_room(fllm_batch* b, uint64_t n) {
+    hipError_t e = hipSuccess;
+    if (b->in_flight) e = hipEventSynchronize(b->sent);
+    b->in_flight = false;
+    if (e != hipSuccess || n <= b->cap) return e;
+    e = hipStreamSynchronize(b->p->ctx->stream);
+    if (e != hipSuccess) return e;
+    if (b->dev) hipFree(b->dev);
+    if (b->pin) hipHostFree(b->pin);
+    b->dev = b->pin = nullptr;
+    b->cap = 0;
+    const uint64_t want = n + n / 2 + 4096;
+    e = hipMalloc(&b->dev, want);
+    if (e == hipSuccess) e = hipHostMalloc((void**)&b->pin, want, hipHostMallocDefault);
+    if (e == hipSuccess) b->cap = want;
+    return e;
+}
+
+extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* new_tokens, const int32_t* lengths,
+                                  const int32_t* tables, int64_t ld) {
+    NOT_NULL(b);
+    fllm_pages* p = b->p;
+    b->view = BatchView{};
+    if (p->disposed) return fail(FLLM_E_DISPOSED, "the pages were destroyed");
+    if (n_seqs < 0) return fail(FLLM_E_ARG_RANGE, "n_seqs must not be negative");
+    if (n_seqs == 0) {
+        b->plan = BatchPlan{};
+        return FLLM_OK;
+    }
+    NOT_NULL(new_tokens);
+    NOT_NULL(lengths);
+    NOT_NULL(tables);
+    if (ld < 0) return fail(FLLM_E_ARG_RANGE, "ld must not be negative");
+    HIP_TRY(hipSetDevice(p->ctx->device));
+    return guarded([&]() -> int32_t {
+        BatchError err;
+        if (batch_plan(p->d, b->window, n_seqs, new_tokens, lengths, tables, ld, &b->plan, &err)) {
+            b->plan.n_seqs = b->plan.n_rows = b->plan.n_pos = 0;
+            return fail(err.code, "%s", err.text);
+        }
+        const BatchPlan& pl = b->plan;
+        const uint64_t n_seq_bytes = pl.seqs.size() * sizeof(SeqPlan), n_tab = pl.tables.size() * sizeof(int32_t);
+        const int n_plan_seqs = pl.n_seqs;
+        b->plan.n_seqs = 0;  // empty until everything is on its way
+        hipError_t e = batch_room(b, n_seq_bytes + n_tab);
+        if (e != hipSuccess)
+            return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "batch memory: %s", hipGetErrorString(e));
+        memcpy(b->pin, pl.seqs.data(), n_seq_bytes);
+        if (n_tab) memcpy(b->pin + n_seq_bytes, pl.tables.data(), n_tab);
+        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, n_seq_bytes + n_tab, hipMemcpyHostToDevice, p->ctx->stream));
+        HIP_TRY(hipEventRecord(b->sent, p->ctx->stream));
+        b->in_flight = true;
+        b->plan.n_seqs = n_plan_seqs;
+        b->view.seqs = (const int4*)b->dev;
+        b->view.tables = (const int*)(b->dev + n_seq_bytes);
+        b->view.tab_w = pl.tab_w;
+        b->view.n_seqs = n_plan_seqs;
+        b->view.new_blocks = pl.new_blocks;
+        b->view.all_blocks = pl.all_blocks;
+        b->view.n_rows = pl.n_rows;
+        b->view.n_heads = b->n_heads;
+        b->view.window = b->window;
+        return FLLM_OK;
+    });
+}
+
+extern "C" int32_t fllm_batch_destroy(fllm_batch* b) {
+    if (!b) return FLLM_OK;
+    fllm_pages* p = b->p;
+    hipSetDevice(p->ctx->device);
+    hipStreamSynchronize(p->ctx->stream);
+    if (b->dev) hipFree(b->dev);
+    if (b->pin) hipHostFree(b->pin);
+    if (b->sent) hipEventDestroy(b->sent);
+    delete b;
+    p->n_batches--;
+    if (p->disposed && p->n_batches == 0) pages_free(p);
+    return FLLM_OK;
+}
+
+// =====================================================================================
+// calls
+// =====================================================================================
+// Rows that a call reads or writes: `n` of them, `width` elements wide, each aligned to `align` bytes.
+static int32_t check_rows(fllm_ctx* ctx, const fllm_rows* r, const char* name, int64_t n, int64_t width, RowsView* out,
+                          uint64_t align = 16) {
+    if (!r || !r->buf) return fail(FLLM_E_NULL, "%s must not be null", name);
+    if (r->buf->ctx != ctx) return fail(FLLM_E_ARG, "%s: the buffer belongs to another context", name);
+    if (r->type != FLLM_TYPE_F32 && r->type != FLLM_TYPE_F16 && r->type != FLLM_TYPE_BF16)
+        return fail(FLLM_E_NOT_SUPPORTED, "%s: rows of type %d are not supported", name, r->type);
+    const uint64_t esz = r->type == FLLM_TYPE_F32 ? 4 : 2;
+    if (r->ld < width || r->ld > INT64_MAX / 8 || (uint64_t)r->ld * esz % align != 0 || r->offset % align != 0)
+        return fail(FLLM_E_ARG, "%s: offset %llu, ld %lld for rows of %lld elements (both multiples of %llu bytes)", name,
+                    (unsigned long long)r->offset, (long long)r->ld, (long long)width, (unsigned long long)align);
+    if (n > 0) {
+        const unsigned __int128 end = (unsigned __int128)r->offset + ((unsigned __int128)(n - 1) * (uint64_t)r->ld + (uint64_t)width) * esz;
+        if (end > r->buf->n)
+            return fail(FLLM_E_ARG, "%s: %lld rows do not fit a buffer of %llu bytes", name, (long long)n, (unsigned long long)r->buf->n);
+    }
+    out->p = r->buf->ptr + r->offset;
+    out->ld = r->ld;
+    out->type = r->type;
+    return FLLM_OK;
+}
+
+static bool overlap(const RowsView& a, const RowsView& b, int64_t n, int64_t width) {
+    if (n <= 0) return false;
+    const auto end = [&](const RowsView& r) { return r.p + ((n - 1) * r.ld + width) * (r.type == FLLM_TYPE_F32 ? 4 : 2); };
+    return a.p < end(b) && b.p < end(a);
+}
+
+static int32_t check_call(fllm_batch* b, int32_t layer) {
+    NOT_NULL(b);
+    if (b->p->disposed) return fail(FLLM_E_DISPOSED, "the pages were destroyed");
+    if (layer < 0 || layer >= b->p->d.n_layers)
+        return fail(FLLM_E_ARG_RANGE, "Layer index must be in [0, %d].", b->p->d.n_layers - 1);
+    return FLLM_OK;
+}
+
+static PagesView pages_view(const fllm_pages* p, int layer) {
+    const uint64_t half = p->cell * (uint64_t)p->d.n_kv_heads * (uint64_t)p->d.n_pages;
+    PagesView v{};
+    v.k = p->ptr + 2 * half * (uint64_t)layer;
+    v.v = v.k + half;
+    v.type = p->d.type;
+    v.nkv = p->d.n_kv_heads;
+    v.hd = p->d.head_dim;
+    v.page_log2 = p->d.page_size == 16 ? 4 : p->d.page_size == 32 ? 5 : p->d.page_size == 64 ? 6 : 7;
+    v.cell = p->cell;
+    v.scale_off = (uint32_t)pages_code_bytes(p->d);
+    return v;
+}
+
+extern "C" int32_t fllm_pages_append(fllm_batch* b, int32_t layer, const fllm_rows* k, const fllm_rows* v) {
+    int32_t rc = check_call(b, layer);
+    if (rc) return rc;
+    fllm_pages* p = b->p;
+    const int64_t width = (int64_t)p->d.n_kv_heads * p->d.head_dim;
+    RowsView rk{}, rv{};
+    if ((rc = check_rows(p->ctx, k, "k", b->view.n_rows, width, &rk))) return rc;
+    if ((rc = check_rows(p->ctx, v, "v", b->view.n_rows, width, &rv))) return rc;
+    if (b->view.n_rows == 0) return FLLM_OK;
+    HIP_TRY(hipSetDevice(p->ctx->device));
+    HIP_TRY(launch_pages_append(pages_view(p, layer), b->view, rk, rv, p->ctx->stream));
+    return FLLM_OK;
+}
+
+extern "C" int32_t fllm_pages_read(fllm_batch* b, int32_t layer, int32_t new_only, const fllm_rows* k, const fllm_rows* v) {
+    int32_t rc = check_call(b, layer);
+    if (rc) return rc;
+    if (new_only != 0 && new_only != 1) return fail(FLLM_E_ARG_RANGE, "new_only must be 0 or 1");
+    fllm_pages* p = b->p;
+    const int64_t width = (int64_t)p->d.n_kv_heads * p->d.head_dim;
+    const int64_t n = b->view.n_seqs == 0 ? 0 : new_only ? b->view.n_rows : b->plan.n_pos;
+    RowsView rk{}, rv{};
+    if (!k && !v) return fail(FLLM_E_NULL, "k and v must not both be null");
+    if (k && (rc = check_rows(p->ctx, k, "k", n, width, &rk))) return rc;
+    if (v && (rc = check_rows(p->ctx, v, "v", n, width, &rv))) return rc;
+    if (k && v && overlap(rk, rv, n, width)) return fail(FLLM_E_ARG, "k and v overlap");
+    if (!new_only && b->view.n_seqs && b->plan.holes) return fail(FLLM_E_INVALID_OP, "pages before the window were given back");
+    if (n == 0) return FLLM_OK;
+    HIP_TRY(hipSetDevice(p->ctx->device));
+    HIP_TRY(launch_pages_read(pages_view(p, layer), b->view, new_only != 0, rk, rv, p->ctx->stream));
+    return FLLM_OK;
+}
+
+extern "C" int32_t fllm_pages_attention(fllm_batch* b, int32_t layer, const fllm_rows* q, const fllm_rows* out, float scale,
+                                        float softcap) {
+    int32_t rc = check_call(b, layer);
+    if (rc) return rc;
+    fllm_pages* p = b->p;
+    const int64_t width = (int64_t)b->n_heads * p->d.head_dim;
+    RowsView rq{}, ro{};
+    if ((rc = check_rows(p->ctx, q, "q", b->view.n_rows, width, &rq))) return rc;
+    if ((rc = check_rows(p->ctx, out, "out", b->view.n_rows, width, &ro))) return rc;
+    if (overlap(rq, ro, b->view.n_rows, width)) return fail(FLLM_E_ARG, "q and out overlap");
+    if (!isfinite(scale)) return fail(FLLM_E_ARG_RANGE, "scale must be finite");
+    if (!isfinite(softcap) || softcap < 0.0f) return fail(FLLM_E_ARG_RANGE, "softcap must be finite and not negative");
+    if (b->view.n_rows == 0) return FLLM_OK;
+    HIP_TRY(hipSetDevice(p->ctx->device));
+    HIP_TRY(launch_pages_attention(pages_view(p, layer), b->view, rq, ro, scale, softcap, p->ctx->stream));
+    return FLLM_OK;
+}
+
+// =====================================================================================
+// drafted tokens
+// =====================================================================================
+// n 4-byte values in a buffer of the context.
+static int32_t check_values(fllm_ctx* ctx, const fllm_buf* b, const char* name, int64_t n) {
+    if (!b) return fail(FLLM_E_NULL, "%s must not be null", name);
+    if (b->ctx != ctx) return fail(FLLM_E_ARG, "%s: the buffer belongs to another context", name);
+    if ((uint64_t)n > b->n / 4) return fail(FLLM_E_ARG, "%s: %lld values do not fit a buffer of %llu bytes", name, (long long)n, (unsigned long long)b->n);
+    return FLLM_OK;
+}
+
+extern "C" int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d) {
+    NOT_NULL(ctx);
+    NOT_NULL(d);
+    if (d->n_seqs < 0 || d->n_draft < 0 || d->vocab < 1)
+        return fail(FLLM_E_ARG_RANGE, "%d sequences, %d drafted tokens, vocabulary %d", d->n_seqs, d->n_draft, d->vocab);
+    const int64_t n = d->n_seqs, nd = n * d->n_draft, nt = n * ((int64_t)d->n_draft + 1);
+    RowsView target{}, draft{};
+    int32_t rc;
+    if ((rc = check_rows(ctx, &d->target, "target", nt, d->vocab, &target, 4))) return rc;
+    if (d->draft.buf && (rc = check_rows(ctx, &d->draft, "draft", nd, d->vocab, &draft, 4))) return rc;
+    if (target.type != FLLM_TYPE_F32 || (d->draft.buf && draft.type != FLLM_TYPE_F32))
+        return fail(FLLM_E_NOT_SUPPORTED, "probabilities are F32");
+    if (d->n_draft) {
+        if ((rc = check_values(ctx, d->tokens, "tokens", nd))) return rc;
+        if ((rc = check_values(ctx, d->u_accept, "u_accept", nd))) return rc;
+    }
+    if (d->counts && (rc = check_values(ctx, d->counts, "counts", n))) return rc;
+    if ((rc = check_values(ctx, d->u_sample, "u_sample", n))) return rc;
+    if ((rc = check_values(ctx, d->out_tokens, "out_tokens", nt))) return rc;
+    if ((rc = check_values(ctx, d->out_counts, "out_counts", n))) return rc;
+    if (n == 0) return FLLM_OK;
+    HIP_TRY(hipSetDevice(ctx->device));
+    DraftView v{};
+    v.n_seqs = d->n_seqs;
+    v.n_draft = d->n_draft;
+    v.vocab = d->vocab;
+    v.target = (const float*)target.p;
+    v.target_ld = target.ld;
+    v.draft = (const float*)draft.p;
+    v.draft_ld = draft.ld;
+    v.tokens = d->n_draft ? (const int*)d->tokens->ptr : nullptr;
+    v.counts = d->counts ? (const int*)d->counts->ptr : nullptr;
+    v.u_accept = d->n_draft ? (const float*)d->u_accept->ptr : nullptr;
+    v.u_sample = (const float*)d->u_sample->ptr;
+    v.out_tokens = (int*)d->out_tokens->ptr;
+    v.out_counts = (int*)d->out_counts->ptr;
+    HIP_TRY(launch_draft_verify(v, ctx->stream));
+    return FLLM_OK;
+}

@@ -1,0 +1,51 @@
+// objects.hpp — the ABI's device context and buffers and its error reporting, shared by the files
+// that define entry points of include/fllm.h.
+#pragma once
+
+#include "common.hpp"
+#include "staging.hpp"
+
+namespace fllm {
+
+// Records the message that fllm_last_error returns and gives `code` back (api.hip).
+int32_t fail(int32_t code, const char* fmt, ...);
+
+#define HIP_TRY(expr)                                                                          \
+    do {                                                                                       \
+        hipError_t _e = (expr);                                                                \
+        if (_e != hipSuccess) return fail(FLLM_E_DEVICE, "%s: %s", #expr, hipGetErrorString(_e)); \
+    } while (0)
+
+#define NOT_NULL(p)                                                  \
+    do {                                                             \
+        if (!(p)) return fail(FLLM_E_NULL, "%s must not be null", #p); \
+    } while (0)
+
+static const uint64_t kPad = 256;  // slack after every weight allocation for aligned over-reads
+
+// Device memory that the calls on one context's stream share: it grows, never shrinks, and a call's
+// contents are dead once the call's last kernel has run, so calls in stream order need no more.
+struct Workspace {
+    uint8_t* ptr = nullptr;
+    uint64_t n = 0;
+};
+
+}  // namespace fllm
+
+struct fllm_ctx {
+    int device = 0;
+    hipStream_t stream = nullptr;
+    int n_cu = 0;
+    int64_t hbm = 0;
+    fllm::Staging stage;
+    uint8_t* scratch = nullptr;  // this device's address of the no-allocation scratch array
+    hipError_t scratch_err = hipSuccess;  // why it could not be resolved, if so
+    fllm::Workspace ws;          // partial results of the paged attention and of the draft check
+};
+
+struct fllm_buf {
+    fllm_ctx* ctx = nullptr;
+    uint8_t* ptr = nullptr;
+    uint64_t n = 0;
+    bool owned = true;  // false: the caller's memory (fllm_buf_wrap)
+};

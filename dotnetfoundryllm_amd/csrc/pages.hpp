@@ -1,0 +1,70 @@
+// pages.hpp — launch interface of the paged K/V cache kernels: rows into and out of the pages
+// (pages.hip), attention over them (pages_attention.hip), and the check of drafted tokens (draft.hip).
+#pragma once
+
+#include "common.hpp"
+
+namespace fllm {
+
+// One layer's pages: cell (page, kv head) of K at k + (page * nkv + head) * cell, its codes, then at
+// scale_off its scales (layouts in fllm.h).
+struct PagesView {
+    uint8_t *k, *v;
+    int type, nkv, hd, page_log2;
+    uint64_t cell;
+    uint32_t scale_off;
+};
+// A batch on the device: the pages of sequence s at tables + s * tab_w, and per sequence
+// {first row of its new tokens, their number, its length, first row of its positions}.
+struct BatchView {
+    const int* tables;
+    const int4* seqs;
+    int tab_w, n_seqs;
+    int new_blocks, all_blocks;  // most pages of a sequence that hold new tokens, that hold any
+    int n_rows;                  // new tokens of all sequences
+    int n_heads, window;
+};
+struct RowsView {
+    uint8_t* p;
+    int64_t ld;
+    int type;
+};
+
+// the new rows into their pages / rows out of the pages (k.p or v.p null: not read)
+hipError_t launch_pages_append(const PagesView& pg, const BatchView& b, const RowsView& k, const RowsView& v, hipStream_t st);
+hipError_t launch_pages_read(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v,
+                             hipStream_t st);
+hipError_t launch_pages_attention(const PagesView& pg, const BatchView& b, const RowsView& q, const RowsView& out,
+                                  float scale, float softcap, hipStream_t st);
+
+struct DraftView {
+    int n_seqs, n_draft, vocab;
+    const float* target;
+    int64_t target_ld;
+    const float* draft;  // null: one-point distributions
+    int64_t draft_ld;
+    const int *tokens, *counts;  // counts null: n_draft
+    const float *u_accept, *u_sample;
+    int *out_tokens, *out_counts;
+};
+hipError_t launch_draft_verify(const DraftView& d, hipStream_t st);
+
+// ---- elements ---------------------------------------------------------------------------
+__device__ __forceinline__ float row_elem(const RowsView& r, int64_t i) {
+    if (r.type == FLLM_TYPE_F32) return ((const float*)r.p)[i];
+    if (r.type == FLLM_TYPE_F16) return (float)((const _Float16*)r.p)[i];
+    return bf16_exact(((const uint16_t*)r.p)[i]);
+}
+// round to nearest even; a NaN stays one
+__device__ __forceinline__ uint16_t bf16_round(float f) {
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40u);
+    return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+__device__ __forceinline__ void row_store(const RowsView& r, int64_t i, float f) {
+    if (r.type == FLLM_TYPE_F32) ((float*)r.p)[i] = f;
+    else if (r.type == FLLM_TYPE_F16) ((_Float16*)r.p)[i] = (_Float16)f;
+    else ((uint16_t*)r.p)[i] = bf16_round(f);
+}
+
+}  // namespace fllm

@@ -1,0 +1,165 @@
+// pages_plan.hpp — what the host works out for a batch over the paged K/V cache: the checks of its
+// lengths and page tables. Plain C++ without the HIP API, so the CPU tests compile it by itself.
+#pragma once
+
+#include <climits>
+#include <cstdint>
+#include <cstdio>
+#include <vector>
+
+#include "../../include/fllm.h"
+
+namespace fllm {
+
+constexpr int kPagesMaxLength = 1 << 30;  // positions of a sequence
+
+// Bytes of one cell (a page of one kv head, K or V); 0 where the description is not a valid one.
+inline uint64_t pages_cell_bytes(const fllm_pages_desc& d) {
+    const uint64_t n = (uint64_t)d.page_size * (uint64_t)d.head_dim;
+    switch (d.type) {
+        case FLLM_TYPE_F16: return 2 * n;
+        case FLLM_TYPE_Q8_0: return n / 32 * 34;
+        case FLLM_TYPE_Q4_0: return n / 32 * 18;
+    }
+    return 0;
+}
+
+// Bytes of a cell's codes: its scales start there.
+inline uint64_t pages_code_bytes(const fllm_pages_desc& d) {
+    const uint64_t n = (uint64_t)d.page_size * (uint64_t)d.head_dim;
+    return d.type == FLLM_TYPE_F16 ? 2 * n : d.type == FLLM_TYPE_Q8_0 ? n : n / 2;
+}
+
+struct BatchError {
+    int32_t code = FLLM_OK;
+    char text[200] = "";
+};
+
+inline int32_t pages_desc_check(const fllm_pages_desc& d, uint64_t* bytes, BatchError* e) {
+    e->code = FLLM_E_ARG;
+    if (d.type != FLLM_TYPE_F16 && d.type != FLLM_TYPE_Q8_0 && d.type != FLLM_TYPE_Q4_0) {
+        snprintf(e->text, sizeof(e->text), "pages of type %d are not supported", d.type);
+        return e->code = FLLM_E_NOT_SUPPORTED;
+    }
+    if (d.head_dim < 32 || d.head_dim > 256 || d.head_dim % 32 != 0) {
+        snprintf(e->text, sizeof(e->text), "head_dim %d is not a multiple of 32 in [32, 256]", d.head_dim);
+        return e->code;
+    }
+    if (d.page_size != 16 && d.page_size != 32 && d.page_size != 64 && d.page_size != 128) {
+        snprintf(e->text, sizeof(e->text), "page_size %d is not 16, 32, 64 or 128", d.page_size);
+        return e->code;
+    }
+    if (d.n_layers < 1 || d.n_kv_heads < 1 || d.n_kv_heads > 1024 || d.n_pages < 1) {
+        snprintf(e->text, sizeof(e->text), "%d layers, %d kv heads, %d pages", d.n_layers, d.n_kv_heads, d.n_pages);
+        return e->code;
+    }
+    const unsigned __int128 all = (unsigned __int128)pages_cell_bytes(d) * (unsigned)d.n_kv_heads * 2 * (unsigned)d.n_pages *
+                                  (unsigned)d.n_layers;
+    if (all > (uint64_t)INT64_MAX) {
+        snprintf(e->text, sizeof(e->text), "the pages exceed 2^63 bytes");
+        return e->code;
+    }
+    *bytes = (uint64_t)all;
+    return e->code = FLLM_OK;
+}
+
+struct SeqPlan {
+    int row0, n_new, len, pos0;  // first new row, new tokens, positions, first row of the positions
+};
+
+struct BatchPlan {
+    int n_seqs = 0, n_rows = 0, n_pos = 0;
+    int tab_w = 0;                       // pages of the longest sequence
+    int new_blocks = 0, all_blocks = 0;  // most pages of a sequence that hold new tokens, that hold any
+    int max_new = 0;                     // most new tokens of a sequence
+    bool holes = false;                  // some page before the windows was given back
+    std::vector<SeqPlan> seqs;
+    std::vector<int32_t> tables;         // [n_seqs][tab_w], 0 where there is no page
+    std::vector<uint8_t> uses;           // scratch: places that name a page (up to 2)
+};
+
+// Fills `p` from the arrays of fllm_batch_set, or says what is wrong with them.
+inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, const int32_t* n_new, const int32_t* lengths,
+                          const int32_t* tables, int64_t ld, BatchPlan* p, BatchError* e) {
+    p->n_seqs = p->n_rows = p->n_pos = p->tab_w = p->new_blocks = p->all_blocks = p->max_new = 0;
+    p->holes = false;
+    p->seqs.clear();
+    p->tables.clear();
+    e->code = FLLM_E_ARG_RANGE;
+    const int P = d.page_size;
+    int64_t rows = 0, pos = 0;
+    int wide = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        const int n = n_new[i], len = lengths[i];
+        if (n < 0 || len < 0 || n > len || len > kPagesMaxLength) {
+            snprintf(e->text, sizeof(e->text), "sequence %d: %d new tokens, length %d (at most %d)", i, n, len, kPagesMaxLength);
+            return e->code;
+        }
+        const int blocks = (len + P - 1) / P, held = n ? blocks - (len - n) / P : 0;
+        wide = blocks > wide ? blocks : wide;
+        p->new_blocks = held > p->new_blocks ? held : p->new_blocks;
+        p->max_new = n > p->max_new ? n : p->max_new;
+        rows += n;
+        pos += len;
+    }
+    if (rows > INT32_MAX || pos > INT32_MAX) {
+        e->code = FLLM_E_ARG;
+        snprintf(e->text, sizeof(e->text), "%lld new rows, %lld positions: at most %d of each", (long long)rows, (long long)pos, INT32_MAX);
+        return e->code;
+    }
+    if (ld < wide) {
+        e->code = FLLM_E_ARG;
+        snprintf(e->text, sizeof(e->text), "tables of %lld pages a sequence, %d are needed", (long long)ld, wide);
+        return e->code;
+    }
+    if ((int64_t)n_seqs * wide > INT32_MAX) {
+        e->code = FLLM_E_ARG;
+        snprintf(e->text, sizeof(e->text), "tables of %d sequences and %d pages", n_seqs, wide);
+        return e->code;
+    }
+    p->uses.assign((size_t)d.n_pages, 0);
+    p->tables.assign((size_t)n_seqs * (size_t)wide, 0);
+    p->seqs.reserve((size_t)n_seqs);
+    int r = 0, q = 0;
+    for (int i = 0; i < n_seqs; i++) {
+        const int n = n_new[i], len = lengths[i], blocks = (len + P - 1) / P;
+        // the first position that any new token sees; without new tokens nothing is read
+        const int64_t low = n ? (int64_t)(len - n) - window + 1 : len;
+        const int first = low > 0 ? (int)(low / P) : 0;
+        for (int k = 0; k < blocks; k++) {
+            const int32_t page = tables[(int64_t)i * ld + k];
+            if (page == -1 && k < first) {
+                p->holes = true;
+                continue;
+            }
+            if (page < 0 || page >= d.n_pages) {
+                e->code = FLLM_E_ARG_RANGE;
+                snprintf(e->text, sizeof(e->text), "sequence %d, block %d: page %d outside [0, %d)", i, k, page, d.n_pages);
+                return e->code;
+            }
+            p->tables[(size_t)i * (size_t)wide + (size_t)k] = page;
+            if (p->uses[(size_t)page] < 2) p->uses[(size_t)page]++;
+        }
+        p->seqs.push_back({r, n, len, q});
+        r += n;
+        q += len;
+    }
+    for (int i = 0; i < n_seqs; i++) {
+        const SeqPlan& s = p->seqs[(size_t)i];
+        for (int k = s.n_new ? (s.len - s.n_new) / P : 0; s.n_new && k < (s.len + P - 1) / P; k++) {
+            const int32_t page = p->tables[(size_t)i * (size_t)wide + (size_t)k];
+            if (p->uses[(size_t)page] > 1) {
+                e->code = FLLM_E_ARG;
+                snprintf(e->text, sizeof(e->text), "sequence %d writes page %d, which the tables name twice", i, page);
+                return e->code;
+            }
+        }
+    }
+    p->n_seqs = n_seqs;
+    p->n_rows = r;
+    p->n_pos = q;
+    p->tab_w = p->all_blocks = wide;
+    return e->code = FLLM_OK;
+}
+
+}  // namespace fllm

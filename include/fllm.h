@@ -315,6 +315,12 @@ FLLM_API int32_t fllm_element_count(int32_t type, int64_t nbytes, int64_t* out);
 
 /* Device buffers. */
 FLLM_API int32_t fllm_buf_create(fllm_ctx* ctx, uint64_t nbytes, fllm_buf** out);
+/* A buffer over device memory that the caller allocated and keeps: another library's tensor, a part of
+ * a larger allocation. device_ptr is a 16-byte aligned address on the context's device; the caller frees
+ * the memory after fllm_buf_destroy and after the calls that use it have run (fllm_ctx_sync). Calls on
+ * the buffer run on the context's stream and know no other: work on other streams is ordered by the
+ * caller. No counterpart in the reference. */
+FLLM_API int32_t fllm_buf_wrap(fllm_ctx* ctx, void* device_ptr, uint64_t nbytes, fllm_buf** out);
 FLLM_API int32_t fllm_buf_destroy(fllm_buf* b);
 FLLM_API int32_t fllm_buf_write(fllm_buf* b, uint64_t offset, const void* src, uint64_t n);
 FLLM_API int32_t fllm_buf_read(fllm_buf* b, uint64_t offset, void* dst, uint64_t n);
@@ -354,6 +360,120 @@ FLLM_API int32_t fllm_gemv_ex(fllm_ctx* ctx, int32_t type, fllm_buf* w, uint64_t
 FLLM_API int32_t fllm_gemv_time_ex(fllm_ctx* ctx, int32_t type, fllm_buf* const* w, int32_t n_w,
                                    int64_t rows, int64_t cols, fllm_buf* x, fllm_buf* y,
                                    int32_t iters, int32_t layout, double* avg_us);
+
+/* ---- paged K/V cache of several sequences ------------------------------------
+ * The operators of a layer whose keys and values lie in pages, for a caller that runs several
+ * sequences together: write a batch's new rows, attend from them, read rows back. They stand beside
+ * fllm_kv_append / fllm_kv_read (one sequence, F32, contiguous) and have no counterpart in the
+ * reference, whose KvCache.cs holds one sequence.
+ *
+ * A page holds page_size positions of one sequence; position p of a sequence lies in the page
+ * that its table names at p / page_size, at p % page_size, in every layer. The pages are one array
+ * [n_layers][2: K, V][n_pages][n_kv_heads] of cells. A cell is its codes, then (Q8_0, Q4_0) its scales
+ * in half precision, and takes as many bytes as page_size * head_dim elements of the type:
+ *   K codes  [head_dim / 32][page_size][32]      Q4_0: 16 bytes in place of 32 codes, byte j holding
+ *   V codes  [head_dim / 32][32][page_size]      element j in its low half, j + 16 in its high half
+ *   scales   [head_dim / 32][page_size]
+ * so that a key's block and a value's run of positions are each contiguous. Of every 32 elements x of
+ * a row, m being the one of largest magnitude (the first of equals):
+ *   F16   x rounded to half precision
+ *   Q8_0  d = |m| / 127, code = x / d rounded, in [-127, 127]; the value is code * d
+ *   Q4_0  d = m / -8, code = x / d rounded, in [-8, 7], stored plus 8; the value is code * d
+ * with d rounded to half precision first (at most 65504) and every rounding to nearest even. d == 0 gives zeros;
+ * a NaN or an infinity among the 32 gives 32 NaNs (Q8_0, Q4_0). */
+typedef struct fllm_pages_desc {
+    int32_t type;        /* FLLM_TYPE_F16, FLLM_TYPE_Q8_0 or FLLM_TYPE_Q4_0 */
+    int32_t n_layers;
+    int32_t n_kv_heads;
+    int32_t head_dim;    /* a multiple of 32, 32 to 256 */
+    int32_t page_size;   /* positions: 16, 32, 64 or 128 */
+    int32_t n_pages;
+} fllm_pages_desc;
+
+/* Rows of a matrix in a buffer: row r starts ld * r elements of `type` after `offset` bytes.
+ * offset and ld * element size are multiples of 16; ld is at least the row's width. */
+typedef struct fllm_rows {
+    fllm_buf* buf;
+    uint64_t  offset;    /* bytes */
+    int64_t   ld;        /* elements */
+    int32_t   type;      /* FLLM_TYPE_F32, FLLM_TYPE_F16 or FLLM_TYPE_BF16 */
+    int32_t   reserved;  /* 0 */
+} fllm_rows;
+
+typedef struct fllm_pages fllm_pages;  /* the pages of all layers */
+typedef struct fllm_batch fllm_batch;  /* which positions of which sequences a call works on */
+
+/* Bytes of the page array. FLLM_E_NOT_SUPPORTED for other types, FLLM_E_ARG for other sizes. */
+FLLM_API int32_t fllm_pages_bytes(const fllm_pages_desc* desc, uint64_t* out);
+/* The page array in mem at `offset` (a multiple of 16), or with mem NULL in memory of its own, which
+ * starts as zeros. mem's contents are taken as they are. */
+FLLM_API int32_t fllm_pages_create(fllm_ctx* ctx, const fllm_pages_desc* desc, fllm_buf* mem, uint64_t offset,
+                                   fllm_pages** out);
+/* Calls on the batches of destroyed pages return FLLM_E_DISPOSED; the memory is released when the last
+ * batch is destroyed (as fllm_model_destroy does for its sequences). */
+FLLM_API int32_t fllm_pages_destroy(fllm_pages* p);
+
+/* A batch for n_heads query heads (a multiple of n_kv_heads; query head h reads kv head
+ * h / (n_heads / n_kv_heads)) and a sliding window: a query at position p attends to the positions
+ * in (p - window, p] (INT32_MAX: all). One batch serves every layer of a step; models with two kinds of
+ * layers keep one for each. */
+FLLM_API int32_t fllm_batch_create(fllm_pages* p, int32_t n_heads, int32_t window, fllm_batch** out);
+/* The sequences of the following calls, replacing earlier ones: sequence i has lengths[i] positions,
+ * the last new_tokens[i] of them new (0 is allowed), in the pages tables[i * ld + 0 .. ceil(lengths[i] /
+ * page_size)). The new tokens' rows of k, v, q and out follow each other, sequence by sequence. All
+ * arrays are host memory, copied before the call returns. Entries of pages that lie before every new
+ * token's window may be -1 (a page given back); fllm_pages_read of all positions then fails.
+ * Refused, with the batch left empty: negative counts, new_tokens > lengths, a page outside
+ * [0, n_pages) -> FLLM_E_ARG_RANGE; ld too small, a page that one sequence writes and another
+ * place of the tables names too, more than INT32_MAX rows -> FLLM_E_ARG. */
+FLLM_API int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* new_tokens, const int32_t* lengths,
+                                const int32_t* tables, int64_t ld);
+FLLM_API int32_t fllm_batch_destroy(fllm_batch* b);
+
+/* The calls below are enqueued on the context's stream. Their rows lie in buffers of the same context;
+ * rows behind the batch's last one are neither read nor written. layer outside [0, n_layers) ->
+ * FLLM_E_ARG_RANGE; rows that do not fit their buffer, misaligned offsets or strides -> FLLM_E_ARG; other
+ * element types -> FLLM_E_NOT_SUPPORTED. */
+
+/* Writes the new tokens' keys and values (rows of n_kv_heads * head_dim) into their pages. */
+FLLM_API int32_t fllm_pages_append(fllm_batch* b, int32_t layer, const fllm_rows* k, const fllm_rows* v);
+/* Reads keys and values back as dense rows (either may be NULL): of every position of every sequence,
+ * one sequence after the other (new_only 0), or of the new tokens (new_only 1). k and v must not overlap. */
+FLLM_API int32_t fllm_pages_read(fllm_batch* b, int32_t layer, int32_t new_only, const fllm_rows* k, const fllm_rows* v);
+/* Attention of the new tokens over their sequences' pages: out = softmax(s) V with
+ * s = scale * q K^T, softcap * tanh(s / softcap) where softcap > 0, over the positions a query sees (its
+ * own among them: append first). q and out are rows of n_heads * head_dim and must not overlap. F32
+ * queries are multiplied with 22 significant bits of each factor and give F32-accurate results;
+ * F16 and BF16 ones with 11, as their outputs hold. A value row that is not finite makes results of queries before it
+ * in the same sequence NaN too; positions behind the sequences' lengths may hold anything.
+ * scale not finite, softcap negative or not finite -> FLLM_E_ARG_RANGE. */
+FLLM_API int32_t fllm_pages_attention(fllm_batch* b, int32_t layer, const fllm_rows* q, const fllm_rows* out, float scale,
+                                      float softcap);
+
+/* ---- verification of drafted tokens --------------------------------------------
+ * Speculative sampling over probabilities (fllm_probs_copy's kind: after temperature and nucleus): of
+ * n_seqs sequences with up to n_draft drafted tokens each, drafted token i is kept while
+ *   u_accept[i] * draft_i[token_i] < target_i[token_i];
+ * the first refused i gives a token drawn from max(target_i - draft_i, 0) (from target_i where that is
+ * zero everywhere), a draft kept whole one from target_n. Drawing takes the first id whose running
+ * sum exceeds u_sample times the whole sum, as the samplers above (TemperatureSampler.cs:53-70); sums are in 64 bits.
+ * A drafted id outside [0, vocab) is refused; weights that are not positive numbers count as zero; a row without any
+ * positive weight gives vocab - 1. Random numbers lie in [0, 1). */
+typedef struct fllm_draft_desc {
+    int32_t n_seqs, n_draft, vocab;  /* n_draft may be 0: every sequence draws from its one target row */
+    int32_t reserved;                /* 0 */
+    fllm_rows target;        /* F32, n_seqs * (n_draft + 1) rows of vocab (offset a multiple of 4, any ld) */
+    fllm_rows draft;         /* F32, n_seqs * n_draft rows of vocab; buf NULL: the draft was certain of its tokens */
+    fllm_buf* tokens;        /* int32 [n_seqs][n_draft] */
+    fllm_buf* counts;        /* int32 [n_seqs], drafted tokens of each sequence (clamped to [0, n_draft]); NULL: n_draft */
+    fllm_buf* u_accept;      /* float [n_seqs][n_draft] */
+    fllm_buf* u_sample;      /* float [n_seqs] */
+    fllm_buf* out_tokens;    /* int32 [n_seqs][n_draft + 1]: the kept tokens, the drawn one, then -1 */
+    fllm_buf* out_counts;    /* int32 [n_seqs]: kept tokens */
+} fllm_draft_desc;
+/* Enqueued on the context's stream. Negative sizes, vocab < 1 -> FLLM_E_ARG_RANGE; buffers too small,
+ * misaligned rows -> FLLM_E_ARG; other types than F32 -> FLLM_E_NOT_SUPPORTED. */
+FLLM_API int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d);
 
 /* ---- per-kernel timing of the decode step ----------------------------------- */
 /* When enabled, fllm_forward launches kernels one by one (no graph) with a HIP event pair
