@@ -227,7 +227,8 @@ extern "C" int32_t fllm_ctx_destroy(fllm_ctx* ctx) {
     hipSetDevice(ctx->device);
     hipStreamSynchronize(ctx->stream);
     staging_free(ctx->stage);
-    if (ctx->ws.ptr) hipFree(ctx->ws.ptr);
+    if (ctx->ws.part) hipFree(ctx->ws.part);
+    if (ctx->ws.cnt) hipFree(ctx->ws.cnt);
     hipStreamDestroy(ctx->stream);
     delete ctx;
     return FLLM_OK;

@@ -27,6 +27,7 @@ struct fllm_batch {
     fllm_pages* p = nullptr;
     int n_heads = 0, window = 0;
     BatchPlan plan;
+    AttnPlan attn;
     // the plan's arrays on the device and the pinned block that they are copied from; `sent` says when
     // the last copy has read it
     uint8_t *dev = nullptr, *pin = nullptr;
@@ -34,6 +35,7 @@ struct fllm_batch {
     hipEvent_t sent = nullptr;
     bool in_flight = false;
     BatchView view{};
+    AttnWork work{};
 };
 
 // Runs a body that may allocate on the host: no exception crosses the ABI.
@@ -169,6 +171,7 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
     NOT_NULL(b);
     fllm_pages* p = b->p;
     b->view = BatchView{};
+    b->work = AttnWork{};
     if (p->disposed) return fail(FLLM_E_DISPOSED, "the pages were destroyed");
     if (n_seqs < 0) return fail(FLLM_E_ARG_RANGE, "n_seqs must not be negative");
     if (n_seqs == 0) {
@@ -187,20 +190,29 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
             return fail(err.code, "%s", err.text);
         }
         const BatchPlan& pl = b->plan;
-        const uint64_t n_seq_bytes = pl.seqs.size() * sizeof(SeqPlan), n_tab = pl.tables.size() * sizeof(int32_t);
         const int n_plan_seqs = pl.n_seqs;
+        if (!attn_plan(pl, b->n_heads, p->d.n_kv_heads, b->window, p->ctx->n_cu, &b->attn)) {
+            b->plan.n_seqs = b->plan.n_rows = b->plan.n_pos = 0;
+            return fail(FLLM_E_ARG, "the batch is too large");
+        }
         b->plan.n_seqs = 0;  // empty until everything is on its way
-        hipError_t e = batch_room(b, n_seq_bytes + n_tab);
+        // sequences, items, tables: parts of 16, 32 and 4 bytes
+        const void* from[4] = {pl.seqs.data(), b->attn.items[0].data(), b->attn.items[1].data(), pl.tables.data()};
+        const uint64_t size[4] = {(pl.seqs.size() * sizeof(SeqPlan) + 31) / 32 * 32, b->attn.items[0].size() * sizeof(AttnItem),
+                                  b->attn.items[1].size() * sizeof(AttnItem), pl.tables.size() * sizeof(int32_t)};
+        uint64_t at[5] = {0};
+        for (int i = 0; i < 4; i++) at[i + 1] = at[i] + size[i];
+        hipError_t e = batch_room(b, at[4]);
         if (e != hipSuccess)
             return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "batch memory: %s", hipGetErrorString(e));
-        memcpy(b->pin, pl.seqs.data(), n_seq_bytes);
-        if (n_tab) memcpy(b->pin + n_seq_bytes, pl.tables.data(), n_tab);
-        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, n_seq_bytes + n_tab, hipMemcpyHostToDevice, p->ctx->stream));
+        for (int i = 0; i < 4; i++)
+            if (size[i]) memcpy(b->pin + at[i], from[i], i ? size[i] : pl.seqs.size() * sizeof(SeqPlan));
+        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, at[4], hipMemcpyHostToDevice, p->ctx->stream));
         HIP_TRY(hipEventRecord(b->sent, p->ctx->stream));
         b->in_flight = true;
         b->plan.n_seqs = n_plan_seqs;
         b->view.seqs = (const int4*)b->dev;
-        b->view.tables = (const int*)(b->dev + n_seq_bytes);
+        b->view.tables = (const int*)(b->dev + at[3]);
         b->view.tab_w = pl.tab_w;
         b->view.n_seqs = n_plan_seqs;
         b->view.new_blocks = pl.new_blocks;
@@ -208,6 +220,11 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         b->view.n_rows = pl.n_rows;
         b->view.n_heads = b->n_heads;
         b->view.window = b->window;
+        for (int i = 0; i < 2; i++) {
+            b->work.items[i] = (const AttnItem*)(b->dev + at[1 + i]);
+            b->work.n[i] = (int)b->attn.items[i].size();
+        }
+        b->work.part_rows = b->attn.part_rows;
         return FLLM_OK;
     });
 }
@@ -229,6 +246,31 @@ extern "C" int32_t fllm_batch_destroy(fllm_batch* b) {
 // =====================================================================================
 // calls
 // =====================================================================================
+// Room in the context's workspace (its mutex is held). Memory that earlier calls use is waited for
+// before it is replaced.
+static hipError_t workspace_room(fllm_ctx* ctx, uint64_t part_bytes, uint64_t n_cnt) {
+    Workspace& w = ctx->ws;
+    if (part_bytes <= w.part_bytes && n_cnt <= w.n_cnt) return hipSuccess;
+    hipError_t e = hipStreamSynchronize(ctx->stream);
+    if (e == hipSuccess && part_bytes > w.part_bytes) {
+        if (w.part) hipFree(w.part);
+        w.part = nullptr;
+        w.part_bytes = 0;
+        e = hipMalloc(&w.part, part_bytes + part_bytes / 2);
+        if (e == hipSuccess) w.part_bytes = part_bytes + part_bytes / 2;
+    }
+    if (e == hipSuccess && n_cnt > w.n_cnt) {
+        if (w.cnt) hipFree(w.cnt);
+        w.cnt = nullptr;
+        w.n_cnt = 0;
+        const uint64_t n = n_cnt + n_cnt / 2;
+        e = hipMalloc(&w.cnt, n * sizeof(unsigned));
+        if (e == hipSuccess) e = hipMemsetAsync(w.cnt, 0, n * sizeof(unsigned), ctx->stream);
+        if (e == hipSuccess) w.n_cnt = n;
+    }
+    return e;
+}
+
 // Rows that a call reads or writes: `n` of them, `width` elements wide, each aligned to `align` bytes.
 static int32_t check_rows(fllm_ctx* ctx, const fllm_rows* r, const char* name, int64_t n, int64_t width, RowsView* out,
                           uint64_t align = 16) {
@@ -326,7 +368,15 @@ extern "C" int32_t fllm_pages_attention(fllm_batch* b, int32_t layer, const fllm
     if (!isfinite(softcap) || softcap < 0.0f) return fail(FLLM_E_ARG_RANGE, "softcap must be finite and not negative");
     if (b->view.n_rows == 0) return FLLM_OK;
     HIP_TRY(hipSetDevice(p->ctx->device));
-    HIP_TRY(launch_pages_attention(pages_view(p, layer), b->view, rq, ro, scale, softcap, p->ctx->stream));
+    std::lock_guard<std::mutex> lock(p->ctx->ws.mu);
+    AttnWork w = b->work;
+    const uint64_t rows = (uint64_t)w.part_rows * (uint64_t)p->d.n_kv_heads;
+    hipError_t e = workspace_room(p->ctx, rows * (uint64_t)(p->d.head_dim + 2) * sizeof(float), rows);
+    if (e != hipSuccess)
+        return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "attention workspace: %s", hipGetErrorString(e));
+    w.part = (float*)p->ctx->ws.part;
+    w.cnt = p->ctx->ws.cnt;
+    HIP_TRY(launch_pages_attention(pages_view(p, layer), b->view, w, rq, ro, scale, softcap, p->ctx->stream));
     return FLLM_OK;
 }
 

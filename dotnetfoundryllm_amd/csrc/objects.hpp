@@ -23,11 +23,15 @@ int32_t fail(int32_t code, const char* fmt, ...);
 
 static const uint64_t kPad = 256;  // slack after every weight allocation for aligned over-reads
 
-// Device memory that the calls on one context's stream share: it grows, never shrinks, and a call's
-// contents are dead once the call's last kernel has run, so calls in stream order need no more.
+// Device memory that the calls on one context's stream share: `part` holds a call's partial results, dead
+// once the call's last kernel has run; `cnt` counters that are zero between calls. Both grow and never
+// shrink. A call holds `mu` while it enqueues, so that two threads' calls follow each other on the stream.
 struct Workspace {
-    uint8_t* ptr = nullptr;
-    uint64_t n = 0;
+    std::mutex mu;
+    uint8_t* part = nullptr;
+    uint64_t part_bytes = 0;
+    unsigned* cnt = nullptr;
+    uint64_t n_cnt = 0;
 };
 
 }  // namespace fllm

@@ -1,79 +1,489 @@
 // pages_attention.hip — attention of new tokens over the pages of their sequences.
+//
+// Mathematics. o = sum_j w_j v_j / sum_j w_j, w_j = exp(s_j - m), in one pass over the keys with the
+// running maximum m: whatever has been summed is multiplied by exp(m_old - m_new) when m grows. The
+// products run on the fp16 matrix cores, transposed: S^T = K Q^T and O^T = V^T P^T, so that a lane
+// holds one query's scores (column l & 15 of the tile) and the weights are, as they lie in the score
+// registers, the second product's operand. All sums are f32.
+//
+// Factors. Every row of q is scaled by a power of two (largest magnitude into [2^14, 2^15)) and rounded
+// to fp16, for F32 rows as a high and a low half that together keep 22 bits (NP = 2: two products in place of
+// one). K and V enter exactly: the halves of an F16 cache, the codes of a quantised one as
+// integers, whose scales are applied in f32: to the scores block by block, and to the weights before they are
+// rounded (as one or two halves), so that a V block's product is weights-times-scales by codes.
+//
+// k_attend_few: up to 16 TM rows (decoding, drafted tokens), bound by the bytes of K and V. A wave
+// takes steps of 64 keys (32 of an F16 cache) for all rows straight from the pages into registers: the page
+// layouts (fllm.h) are such that 8 consecutive elements of an operand are contiguous in memory, so
+// there is no LDS stage and no barrier in the loop. The four waves of a workgroup take turns at the
+// steps of an item; their results meet in LDS, and those of a tile's items in memory, joined by
+// the item that finishes last (write-through stores and a counter, as the decode attention of
+// attn_body.hpp, so no second launch).
+#include "attn_body.hpp"
 #include "pages.hpp"
+#include "pages_plan.hpp"
 
 namespace fllm {
 
 namespace {
 
-template <int TYPE>
-__device__ __forceinline__ float cell_value(const PagesView& pg, const uint8_t* cell, int kind, int d, int pos) {
-    const int P = 1 << pg.page_log2, blk = d >> 5, e = d & 31;
-    if (TYPE == FLLM_TYPE_F16) return half_exact(((const uint16_t*)cell)[kind ? d * P + pos : (blk * P + pos) * 32 + e]);
-    const float s = half_exact(*(const uint16_t*)(cell + pg.scale_off + 2 * (blk * P + pos)));
-    if (TYPE == FLLM_TYPE_Q8_0) return (float)(int8_t)cell[kind ? d * P + pos : (blk * P + pos) * 32 + e] * s;
-    const int c = cell[kind ? (blk * 16 + (e & 15)) * P + pos : (blk * P + pos) * 16 + (e & 15)];
-    return (float)((e < 16 ? c & 15 : c >> 4) - 8) * s;
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoScore = -1e30f;  // the running maximum before any key
+
+union H8 {
+    h8 v;
+    h2 p[4];
+    uint32_t u[4];
+};
+
+// 4 bytes, each code + 128 or nibble, as fp16 integers: 0x6400 | byte is 1024 + byte exactly
+template <int OFF>
+__device__ __forceinline__ void bytes_to_half(uint32_t w, uint32_t* out) {
+    const h2 off = {(_Float16)OFF, (_Float16)OFF};
+    union { uint32_t u; h2 h; } a, b;
+    a.u = __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u);
+    b.u = __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u);
+    a.h = a.h - off;
+    b.h = b.h - off;
+    out[0] = a.u;
+    out[1] = b.u;
 }
 
-// One workgroup per new token and query head; a wave per key, lane l holding the elements l + 64 i.
-template <int TYPE>
-__global__ __launch_bounds__(256) void k_pages_attention(PagesView pg, BatchView b, RowsView q, RowsView out, float scale,
-                                                         float softcap) {
-    __shared__ float s_o[4][256], s_m[4], s_l[4];
-    const int row = blockIdx.x, h = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int lo = 0, hi = b.n_seqs - 1;
-    while (lo < hi) {  // the last sequence that starts at or before this row and has one
-        const int mid = (lo + hi + 1) >> 1;
-        if (b.seqs[mid].x <= row) lo = mid;
-        else hi = mid - 1;
+// A lane's 8 operand elements out of what it loads of a cell: 16, 8 or 4 bytes.
+template <int TYPE> struct Frag;
+template <> struct Frag<FLLM_TYPE_F16> {
+    u4 w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *(const u4*)p; }
+    __device__ __forceinline__ h8 half() const {
+        H8 r;
+        for (int i = 0; i < 4; i++) r.u[i] = w[i];
+        return r.v;
     }
-    const int4 sq = b.seqs[lo];
-    const int pos = sq.z - sq.y + (row - sq.x), kvh = h / (b.n_heads / pg.nkv);
-    const int64_t first = (int64_t)pos - b.window + 1;
-    const int* table = b.tables + (int64_t)lo * b.tab_w;
-    float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-    for (int i = 0; i < 4; i++) qv[i] = lane + 64 * i < pg.hd ? row_elem(q, row * q.ld + h * pg.hd + lane + 64 * i) : 0.f;
-    for (int j = (int)(first > 0 ? first : 0) + wave; j <= pos; j += 4) {
-        const uint64_t cell = ((uint64_t)table[j >> pg.page_log2] * pg.nkv + kvh) * pg.cell;
-        const int p = j & ((1 << pg.page_log2) - 1);
-        float s = 0.f;
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < pg.hd) s = fmaf(qv[i], cell_value<TYPE>(pg, pg.k + cell, 0, lane + 64 * i, p), s);
-        for (int x = 32; x; x >>= 1) s += __shfl_xor(s, x);
-        s *= scale;
-        if (softcap > 0.f) s = softcap * tanhf(s / softcap);
-        const float nm = fmaxf(m, s), a = expf(m - nm), w = expf(s - nm);
-        m = nm;
-        l = l * a + w;
-        for (int i = 0; i < 4; i++)
-            if (lane + 64 * i < pg.hd) o[i] = o[i] * a + w * cell_value<TYPE>(pg, pg.v + cell, 1, lane + 64 * i, p);
+};
+template <> struct Frag<FLLM_TYPE_Q8_0> {
+    u2 w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *(const u2*)p; }
+    __device__ __forceinline__ h8 half() const {
+        H8 r;
+        bytes_to_half<1152>(w.x ^ 0x80808080u, r.u);
+        bytes_to_half<1152>(w.y ^ 0x80808080u, r.u + 2);
+        return r.v;
     }
-    for (int i = 0; i < 4; i++) s_o[wave][lane + 64 * i] = o[i];
-    if (lane == 0) s_m[wave] = m, s_l[wave] = l;
+};
+template <> struct Frag<FLLM_TYPE_Q4_0> {  // elements 4 g .. + 3 in the low halves, 16 + 4 g .. in the high ones
+    uint32_t w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *(const uint32_t*)p; }
+    __device__ __forceinline__ h8 half() const {
+        H8 r;
+        bytes_to_half<1032>(w & 0x0F0F0F0Fu, r.u);
+        bytes_to_half<1032>(w >> 4 & 0x0F0F0F0Fu, r.u + 2);
+        return r.v;
+    }
+};
+
+// x as fp16 halves: one rounded to nearest, or a high and a low one (both cut, together 21 to 22 bits)
+template <int NP>
+__device__ __forceinline__ void split8(const float x[8], h8 out[NP]) {
+    H8 hi, lo;
+    for (int i = 0; i < 4; i++) {
+        if (NP == 1) {
+            hi.p[i] = h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+        } else {
+            union { __fp16 __attribute__((ext_vector_type(2))) c; h2 h; } a, b;
+            a.c = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
+            hi.p[i] = a.h;
+            b.c = __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)a.h.x, x[2 * i + 1] - (float)a.h.y);
+            lo.p[i] = b.h;
+        }
+    }
+    out[0] = hi.v;
+    if (NP == 2) out[NP - 1] = lo.v;
+}
+
+// tanh to 1e-7: a series near zero, where the quotient would cancel
+__device__ __forceinline__ float tanh_of(float x) {
+    const float y = x * x;
+    const float p = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
+    const float q = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+    return fabsf(x) < 0.25f ? p : q;
+}
+
+struct FewArgs {
+    PagesView pg;
+    const int* tables;
+    const int4* seqs;
+    const AttnItem* items;
+    int tab_w, group, window;
+    RowsView q, out;
+    float scale, softcap;
+    float *part_o, *part_ml;
+    unsigned* cnt;
+};
+
+template <int TYPE, int HDP, int NP, int TM>
+__global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
+    constexpr int NB = HDP / 32, ND = HDP / 16;      // blocks of 32 elements, tiles of 16
+    constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
+    constexpr int JN = QUANT ? 2 : 1;                // runs of 32 keys a step
+    constexpr int STEP = 32 * JN, RUN = 8 * JN;      // keys a step, consecutive keys a lane holds
+    constexpr int NV = TYPE == FLLM_TYPE_Q4_0 ? NB : ND;  // loads of V a step (one byte row holds two elements in Q4_0)
+    __shared__ float s_o[4][16][HDP + 4], s_m[4][16], s_l[4][16];
+    __shared__ int s_last;
+
+    const int kvh = blockIdx.x % a.pg.nkv;
+    const AttnItem it = a.items[blockIdx.x / a.pg.nkv];
+    const int4 sq = a.seqs[it.seq];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
+    const int pos0 = sq.z - sq.y;
+    const int* table = a.tables + (int64_t)it.seq * a.tab_w;
+    const int last_block = (sq.z - 1) >> lp;
+
+    // this lane's query of each row tile: its position (-1 where there is no row), its operand halves
+    int pos[TM];
+    float unscale[TM];
+    h8 qf[TM][NB][NP];
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+        const int r = 16 * m + col;
+        const bool live = r < it.nrows;
+        const int row = it.row0 + (live ? r : 0), tok = row / a.group, head = kvh * a.group + row % a.group;
+        pos[m] = live ? pos0 + tok : -1;
+        const int64_t at = (int64_t)(sq.x + tok) * a.q.ld + (int64_t)head * hd;
+        float x[NB][8], top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NB; c++)
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                // the elements that Frag's 8 stand for
+                const int d = TYPE == FLLM_TYPE_Q4_0 ? 32 * c + 16 * half + 4 * g : 32 * c + 8 * g + 4 * half;
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+                if (live && c < nb) {
+                    if (a.q.type == FLLM_TYPE_F32) {
+                        const f4 f = *(const f4*)(a.q.p + 4 * (at + d));
+                        for (int i = 0; i < 4; i++) v[i] = f[i];
+                    } else {
+                        const u2 u = *(const u2*)(a.q.p + 2 * (at + d));
+                        for (int i = 0; i < 4; i++) {
+                            const uint32_t h = (i < 2 ? u.x : u.y) >> (16 * (i & 1)) & 0xFFFFu;
+                            v[i] = a.q.type == FLLM_TYPE_F16 ? half_exact(h) : bf16_exact(h);
+                        }
+                    }
+                }
+                for (int i = 0; i < 4; i++) {
+                    x[c][4 * half + i] = v[i];
+                    top = fmaxf(top, fabsf(v[i]));
+                }
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        int e = 0;
+        (void)frexpf(top, &e);  // top = f 2^e, f in [1/2, 1)
+        e = top > 0.0f && top < INFINITY ? 15 - e : 0;
+        e = e > 120 ? 120 : e;
+        for (int c = 0; c < NB; c++) {
+            for (int i = 0; i < 8; i++) x[c][i] = ldexpf(x[c][i], e);
+            split8<NP>(x[c], qf[m][c]);
+        }
+        unscale[m] = ldexpf(a.scale, -e) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+    }
+    const float cap = a.softcap * kLog2e;
+
+    f4 o[TM][ND];
+    float mx[TM], sum[TM];
+    int vexp = -1000;  // quantised: o is in units of 2^vexp
+    for (int m = 0; m < TM; m++) {
+        mx[m] = kNoScore;
+        sum[m] = 0.0f;
+        for (int d = 0; d < ND; d++) o[m][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // keys that every row sees need no mask: [all_lo, all_hi)
+    const int last_pos = pos0 + (it.row0 + it.nrows - 1) / a.group;
+    const int64_t all_lo = (int64_t)last_pos - a.window + 1, all_hi = pos0 + it.row0 / a.group + 1;
+    const int64_t any_lo = all_hi - a.window;  // the first key that any row sees
+
+    const int ksub = QUANT ? 16 : 8;  // keys of a lane group
+    for (int k0 = it.k0 + wave * STEP; k0 < it.k1; k0 += 4 * STEP) {
+        // K: row col of tile (j, t) is key ksub (col >> 2) + 8 j + 4 t + (col & 3); V: this lane holds the
+        // keys ksub g .. + RUN. Both lie in one page each; past the table's end the last page stands in.
+        const int kk = k0 + ksub * (col >> 2), kv = k0 + ksub * g;
+        const int bk = min(kk >> lp, last_block), bv = min(kv >> lp, last_block);
+        const uint64_t ck = ((uint64_t)(uint32_t)table[bk] * a.pg.nkv + kvh) * a.pg.cell;
+        const uint64_t cv = ((uint64_t)(uint32_t)table[bv] * a.pg.nkv + kvh) * a.pg.cell;
+        const int pk = (kk & (P - 1)) + (col & 3), pv = kv & (P - 1);
+        constexpr int KB = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;  // bytes of a block's codes
+        const uint8_t* kp = a.pg.k + ck + (uint32_t)(pk * KB + g * (KB / 4));
+        Frag<TYPE> kf[2 * JN][NB];
+#pragma unroll
+        for (int t = 0; t < 2 * JN; t++)
+#pragma unroll
+            for (int c = 0; c < NB; c++)
+                if (c < nb) kf[t][c].load(kp + (uint32_t)((c * P + 4 * t) * KB));
+        // scales of this lane's keys, 16 to a block
+        u4 ks[QUANT ? NB : 1][2], vs[QUANT ? NB : 1][2];
+        if (QUANT) {
+#pragma unroll
+            for (int c = 0; c < NB; c++)
+                if (c < nb)
+                    for (int i = 0; i < 2; i++) {
+                        ks[c][i] = *(const u4*)(a.pg.k + cv + a.pg.scale_off + (uint32_t)(2 * (c * P + pv)) + 16 * i);
+                        vs[c][i] = *(const u4*)(a.pg.v + cv + a.pg.scale_off + (uint32_t)(2 * (c * P + pv)) + 16 * i);
+                    }
+        }
+        u4 vf[NV];  // 16 bytes: 8 halves or 16 codes of this lane's keys
+        constexpr int VE = TYPE == FLLM_TYPE_F16 ? 2 : 1;
+        const uint8_t* vp = a.pg.v + cv + (uint32_t)((col * P + pv) * VE);
+#pragma unroll
+        for (int d = 0; d < NV; d++)
+            if (d * (TYPE == FLLM_TYPE_Q4_0 ? 32 : 16) < hd) vf[d] = *(const u4*)(vp + (uint32_t)(d * 16 * P * VE));
+
+        const bool edge = k0 < all_lo || k0 + STEP > all_hi;
+        if (edge) {
+            // what lies outside the sequence may be anything: no scale and no half of it may be a NaN
+            for (int i = 0; i < RUN; i++) {
+                const bool in = kv + i >= any_lo && kv + i < sq.z;
+                if (QUANT) {
+                    const uint32_t keep = in ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+                    for (int c = 0; c < NB; c++) vs[c][i >> 3][(i & 7) >> 1] &= keep;
+                } else {
+                    const uint32_t keep = in ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+                    for (int d = 0; d < NV; d++) vf[d][i >> 1] &= keep;
+                }
+            }
+        }
+        if (QUANT) {  // the units of o: the largest scale so far
+            h2 top = {(_Float16)0, (_Float16)0};
+            for (int c = 0; c < NB; c++)
+                if (c < nb)
+                    for (int i = 0; i < 8; i++) {
+                        union { uint32_t u; h2 h; } s;
+                        s.u = vs[c][i >> 2][i & 3] & 0x7FFF7FFFu;
+                        top = __builtin_elementwise_max(top, s.h);
+                    }
+            float f = fmaxf((float)top.x, (float)top.y);
+            f = fmaxf(f, __shfl_xor(f, 16));
+            f = fmaxf(f, __shfl_xor(f, 32));
+            const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(f) >> 23) - 126);  // f < 2^e
+            if (e > vexp) {
+                const float down = ldexpf(1.0f, vexp - e > -140 ? vexp - e : -140);
+                for (int m = 0; m < TM; m++)
+                    for (int d = 0; d < ND; d++) o[m][d] *= down;
+                vexp = e;
+            }
+        }
+        const float vunit = ldexpf(1.0f, QUANT ? 14 - vexp : 14);
+
+#pragma unroll
+        for (int m = 0; m < TM; m++) {
+            float s[RUN];
+#pragma unroll
+            for (int t = 0; t < 2 * JN; t++) {
+                f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NB; c++) {
+                    if (c >= nb) continue;
+                    const h8 kh = kf[t][c].half();
+                    if (QUANT) {
+                        f4 b = {0.f, 0.f, 0.f, 0.f};
+                        for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[m][c][n], b, 0, 0, 0);
+                        for (int e = 0; e < 4; e++) {
+                            union { uint32_t u; h2 h; } d;
+                            d.u = ks[c][t >> 1][2 * (t & 1) + (e >> 1)];
+                            acc[e] = fmaf(b[e], (float)(e & 1 ? d.h.y : d.h.x), acc[e]);
+                        }
+                    } else {
+                        for (int n = NP - 1; n >= 0; n--) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[m][c][n], acc, 0, 0, 0);
+                    }
+                }
+                for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e] * unscale[m];
+            }
+            if (a.softcap > 0.0f)
+                for (int i = 0; i < RUN; i++) s[i] = cap * tanh_of(s[i]);
+            if (edge)
+                for (int i = 0; i < RUN; i++)
+                    if (kv + i > pos[m] || (int64_t)kv + i <= (int64_t)pos[m] - a.window) s[i] = -INFINITY;
+            float top = s[0];
+            for (int i = 1; i < RUN; i++) top = fmaxf(top, s[i]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float nm = fmaxf(mx[m], top);
+            const float down = __builtin_amdgcn_exp2f(mx[m] - nm);
+            mx[m] = nm;
+            float l = 0.0f;
+            for (int i = 0; i < RUN; i++) {
+                s[i] = __builtin_amdgcn_exp2f(s[i] - nm);
+                l += s[i];
+            }
+            sum[m] = sum[m] * down + l;
+            for (int d = 0; d < ND; d++) o[m][d] *= down;
+
+            if (!QUANT) {
+                float w[8];
+                for (int i = 0; i < 8; i++) w[i] = s[i] * vunit;
+                h8 wf[NP];
+                split8<NP>(w, wf);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    if (d * 16 >= hd) continue;
+                    H8 v;
+                    for (int i = 0; i < 4; i++) v.u[i] = vf[d][i];
+                    for (int n = NP - 1; n >= 0; n--) o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[n], o[m][d], 0, 0, 0);
+                }
+            } else {
+                for (int i = 0; i < RUN; i++) s[i] *= vunit;
+#pragma unroll
+                for (int c = 0; c < NB; c++) {
+                    if (c >= nb) continue;
+                    h8 wf[JN][NP];
+                    for (int j = 0; j < JN; j++) {
+                        float w[8];
+                        for (int i = 0; i < 8; i++) {
+                            union { uint32_t u; h2 h; } d;
+                            d.u = vs[c][j][i >> 1];
+                            w[i] = s[8 * j + i] * (float)(i & 1 ? d.h.y : d.h.x);
+                        }
+                        split8<NP>(w, wf[j]);
+                    }
+                    for (int h = 0; h < 2; h++)
+                        for (int j = 0; j < JN; j++) {
+                            H8 v;
+                            if (TYPE == FLLM_TYPE_Q8_0) {
+                                bytes_to_half<1152>(vf[TYPE == FLLM_TYPE_Q4_0 ? 0 : 2 * c + h][2 * j] ^ 0x80808080u, v.u);
+                                bytes_to_half<1152>(vf[TYPE == FLLM_TYPE_Q4_0 ? 0 : 2 * c + h][2 * j + 1] ^ 0x80808080u, v.u + 2);
+                            } else {
+                                bytes_to_half<1032>(vf[c][2 * j] >> 4 * h & 0x0F0F0F0Fu, v.u);
+                                bytes_to_half<1032>(vf[c][2 * j + 1] >> 4 * h & 0x0F0F0F0Fu, v.u + 2);
+                            }
+                            for (int n = NP - 1; n >= 0; n--)
+                                o[m][2 * c + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[j][n], o[m][2 * c + h], 0, 0, 0);
+                        }
+                }
+            }
+        }
+    }
+
+    // the four waves' results, a row tile at a time
+    const float unit = ldexpf(1.0f, QUANT ? (vexp > -1000 ? vexp - 14 : 0) : -14);
+    const int64_t part0 = ((int64_t)it.part + (int64_t)it.split * it.nrows) * a.pg.nkv + kvh;
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+        sum[m] += __shfl_xor(sum[m], 16);
+        sum[m] += __shfl_xor(sum[m], 32);
+        if (m) __syncthreads();
+        if (g == 0) {
+            s_m[wave][col] = mx[m];
+            s_l[wave][col] = sum[m];
+        }
+        for (int d = 0; d < ND; d++) *(f4*)&s_o[wave][col][16 * d + 4 * g] = o[m][d] * unit;
+        __syncthreads();
+        for (int u = threadIdx.x; u < 16 * (HDP / 4); u += 256) {
+            const int r = u / (HDP / 4), d = u % (HDP / 4) * 4, row = 16 * m + r;
+            if (row >= it.nrows || d >= hd) continue;
+            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+            f4 acc = {0.f, 0.f, 0.f, 0.f};
+            float l = 0.0f;
+            for (int w = 0; w < 4; w++) {
+                const float f = __builtin_amdgcn_exp2f(s_m[w][r] - top);
+                l += f * s_l[w][r];
+                acc += f * *(const f4*)&s_o[w][r][d];
+            }
+            if (it.nsplit == 1) {
+                const int tr = it.row0 + row, tok = tr / a.group, head = kvh * a.group + tr % a.group;
+                const int64_t at = (int64_t)(sq.x + tok) * a.out.ld + (int64_t)head * hd + d;
+                const float inv = 1.0f / l;
+                for (int i = 0; i < 4; i++) row_store(a.out, at + i, acc[i] * inv);
+            } else {
+                const int64_t pr = part0 + (int64_t)row * a.pg.nkv;
+                for (int i = 0; i < 4; i++) st_wt(a.part_o + pr * hd + d + i, acc[i]);
+                if (d == 0) {
+                    st_wt(a.part_ml + 2 * pr, top);
+                    st_wt(a.part_ml + 2 * pr + 1, l);
+                }
+            }
+        }
+    }
+    if (it.nsplit == 1) return;
+
+    // the tile's last item joins the partial rows
+    wt_complete();
     __syncthreads();
-    const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float sum = 0.f, acc = 0.f;
-    for (int w = 0; w < 4; w++) {
-        const float f = s_l[w] > 0.f ? expf(s_m[w] - top) : 0.f;
-        sum += f * s_l[w];
-        if (threadIdx.x < pg.hd) acc += f * s_o[w][threadIdx.x];
+    unsigned* cnt = a.cnt + (int64_t)it.part * a.pg.nkv + kvh;
+    if (threadIdx.x == 0)
+        s_last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(it.nsplit - 1);
+    __syncthreads();
+    if (!s_last) return;
+    if (threadIdx.x == 0) st_wt_u(cnt, 0u);
+    for (int u = threadIdx.x; u < it.nrows * (hd / 4); u += 256) {
+        const int row = u / (hd / 4), d = u % (hd / 4) * 4;
+        float top = kNoScore, l = 0.0f;
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int k = 0; k < it.nsplit; k++) {
+            const int64_t pr = ((int64_t)it.part + (int64_t)k * it.nrows + row) * a.pg.nkv + kvh;
+            const float m1 = __hip_atomic_load(a.part_ml + 2 * pr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float l1 = __hip_atomic_load(a.part_ml + 2 * pr + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            f4 p;
+            for (int i = 0; i < 4; i++) p[i] = __hip_atomic_load(a.part_o + pr * hd + d + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const float nm = fmaxf(top, m1), f0 = __builtin_amdgcn_exp2f(top - nm), f1 = __builtin_amdgcn_exp2f(m1 - nm);
+            acc = acc * f0 + p * f1;
+            l = l * f0 + l1 * f1;
+            top = nm;
+        }
+        const int tr = it.row0 + row, tok = tr / a.group, head = kvh * a.group + tr % a.group;
+        const int64_t at = (int64_t)(sq.x + tok) * a.out.ld + (int64_t)head * hd + d;
+        const float inv = 1.0f / l;
+        for (int i = 0; i < 4; i++) row_store(a.out, at + i, acc[i] * inv);
     }
-    if (threadIdx.x < pg.hd) row_store(out, row * out.ld + h * pg.hd + threadIdx.x, acc / sum);
+}
+
+template <int TYPE, int HDP, int NP>
+hipError_t launch_few(FewArgs a, const AttnWork& w, hipStream_t st) {
+    for (int c = 0; c < 2; c++) {
+        if (w.n[c] == 0) continue;
+        a.items = w.items[c];
+        const dim3 grid((unsigned)w.n[c] * (unsigned)a.pg.nkv);
+        if (c == 0) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2>), grid, dim3(256), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <int TYPE, int NP>
+hipError_t launch_few_hd(const FewArgs& a, const AttnWork& w, hipStream_t st) {
+    if (a.pg.hd <= 64) return launch_few<TYPE, 64, NP>(a, w, st);
+    if (a.pg.hd <= 128) return launch_few<TYPE, 128, NP>(a, w, st);
+    return launch_few<TYPE, 256, NP>(a, w, st);
+}
+
+template <int TYPE>
+hipError_t launch_few_np(const FewArgs& a, const AttnWork& w, hipStream_t st) {
+    // 16-bit rows: 11-bit factors lose less than their outputs' rounding
+    return a.q.type == FLLM_TYPE_F32 || a.out.type == FLLM_TYPE_F32 ? launch_few_hd<TYPE, 2>(a, w, st)
+                                                                    : launch_few_hd<TYPE, 1>(a, w, st);
 }
 
 }  // namespace
 
-hipError_t launch_pages_attention(const PagesView& pg, const BatchView& b, const RowsView& q, const RowsView& out,
-                                  float scale, float softcap, hipStream_t st) {
-    if (b.n_rows == 0) return hipSuccess;
-    const dim3 grid(b.n_rows, b.n_heads);
+hipError_t launch_pages_attention(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q,
+                                  const RowsView& out, float scale, float softcap, hipStream_t st) {
+    const FewArgs a{pg, b.tables, b.seqs, nullptr, b.tab_w, b.n_heads / pg.nkv, b.window, q, out, scale, softcap,
+                    w.part, w.part + w.part_rows * pg.nkv * pg.hd, w.cnt};
     switch (pg.type) {
-        case FLLM_TYPE_F16: hipLaunchKernelGGL(k_pages_attention<FLLM_TYPE_F16>, grid, dim3(256), 0, st, pg, b, q, out, scale, softcap); break;
-        case FLLM_TYPE_Q8_0: hipLaunchKernelGGL(k_pages_attention<FLLM_TYPE_Q8_0>, grid, dim3(256), 0, st, pg, b, q, out, scale, softcap); break;
-        case FLLM_TYPE_Q4_0: hipLaunchKernelGGL(k_pages_attention<FLLM_TYPE_Q4_0>, grid, dim3(256), 0, st, pg, b, q, out, scale, softcap); break;
-        default: return hipErrorNotSupported;
+        case FLLM_TYPE_F16: return launch_few_np<FLLM_TYPE_F16>(a, w, st);
+        case FLLM_TYPE_Q8_0: return launch_few_np<FLLM_TYPE_Q8_0>(a, w, st);
+        case FLLM_TYPE_Q4_0: return launch_few_np<FLLM_TYPE_Q4_0>(a, w, st);
     }
-    return hipGetLastError();
+    return hipErrorNotSupported;
 }
 
 }  // namespace fllm
