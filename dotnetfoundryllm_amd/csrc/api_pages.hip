@@ -191,14 +191,14 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         }
         const BatchPlan& pl = b->plan;
         const int n_plan_seqs = pl.n_seqs;
-        if (!attn_plan(pl, b->n_heads, p->d.n_kv_heads, b->window, p->ctx->n_cu, &b->attn)) {
+        if (!attn_plan(pl, b->n_heads, p->d.n_kv_heads, p->d.head_dim, b->window, p->ctx->n_cu, &b->attn)) {
             b->plan.n_seqs = b->plan.n_rows = b->plan.n_pos = 0;
             return fail(FLLM_E_ARG, "the batch is too large");
         }
         b->plan.n_seqs = 0;  // empty until everything is on its way
-        // sequences, items, tables: parts of 16, 32 and 4 bytes
+        // sequences, items, tables: parts of 16, 64 and 4 bytes
         const void* from[4] = {pl.seqs.data(), b->attn.items[0].data(), b->attn.items[1].data(), pl.tables.data()};
-        const uint64_t size[4] = {(pl.seqs.size() * sizeof(SeqPlan) + 31) / 32 * 32, b->attn.items[0].size() * sizeof(AttnItem),
+        const uint64_t size[4] = {(pl.seqs.size() * sizeof(SeqPlan) + 63) / 64 * 64, b->attn.items[0].size() * sizeof(AttnItem),
                                   b->attn.items[1].size() * sizeof(AttnItem), pl.tables.size() * sizeof(int32_t)};
         uint64_t at[5] = {0};
         for (int i = 0; i < 4; i++) at[i + 1] = at[i] + size[i];

@@ -30,6 +30,7 @@ namespace {
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 
@@ -87,23 +88,44 @@ template <> struct Frag<FLLM_TYPE_Q4_0> {  // elements 4 g .. + 3 in the low hal
     }
 };
 
+__device__ __forceinline__ uint32_t bits(h2 h) {
+    union { uint32_t u; h2 h; } c;
+    c.h = h;
+    return c.u;
+}
+
+// e such that 2^e brings a largest magnitude `top` into [2^14, 2^15); 0 for zeros and what is no number
+__device__ __forceinline__ int row_exponent(float top) {
+    if (!(top > 0.0f && top < INFINITY)) return 0;
+    const int e = 15 - __builtin_amdgcn_frexp_expf(top);  // top = f 2^k, f in [1/2, 1): e = 15 - k
+    return e > 120 ? 120 : e;
+}
+
 // x as fp16 halves: one rounded to nearest, or a high and a low one (both cut, together 21 to 22 bits)
 template <int NP>
-__device__ __forceinline__ void split8(const float x[8], h8 out[NP]) {
-    H8 hi, lo;
-    for (int i = 0; i < 4; i++) {
+__device__ __forceinline__ void split4(const f4 x, h2 out[NP][2]) {
+    for (int i = 0; i < 2; i++) {
         if (NP == 1) {
-            hi.p[i] = h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+            out[0][i] = h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
         } else {
             union { __fp16 __attribute__((ext_vector_type(2))) c; h2 h; } a, b;
             a.c = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-            hi.p[i] = a.h;
-            b.c = __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)a.h.x, x[2 * i + 1] - (float)a.h.y);
-            lo.p[i] = b.h;
+            b.c = __builtin_amdgcn_cvt_pkrtz(fmaf((float)a.h.x, -1.0f, x[2 * i]), fmaf((float)a.h.y, -1.0f, x[2 * i + 1]));
+            out[0][i] = a.h;
+            out[NP - 1][i] = b.h;
         }
     }
-    out[0] = hi.v;
-    if (NP == 2) out[NP - 1] = lo.v;
+}
+template <int NP>
+__device__ __forceinline__ void split8(const float x[8], h8 out[NP]) {
+    h2 a[NP][2], b[NP][2];
+    split4<NP>(f4{x[0], x[1], x[2], x[3]}, a);
+    split4<NP>(f4{x[4], x[5], x[6], x[7]}, b);
+    for (int n = 0; n < NP; n++) {
+        H8 h;
+        h.p[0] = a[n][0], h.p[1] = a[n][1], h.p[2] = b[n][0], h.p[3] = b[n][1];
+        out[n] = h.v;
+    }
 }
 
 // tanh to 1e-7: a series near zero, where the quotient would cancel
@@ -115,102 +137,144 @@ __device__ __forceinline__ float tanh_of(float x) {
     return fabsf(x) < 0.25f ? p : q;
 }
 
+__device__ __forceinline__ f4 load_row4(const RowsView& r, int64_t i) {
+    if (r.type == FLLM_TYPE_F32) return *(const f4*)(r.p + 4 * i);
+    const u2 u = *(const u2*)(r.p + 2 * i);
+    f4 v;
+    if (r.type == FLLM_TYPE_F16) {
+        union { uint32_t u; h2 h; } a, b;
+        a.u = u.x;
+        b.u = u.y;
+        v = f4{(float)a.h.x, (float)a.h.y, (float)b.h.x, (float)b.h.y};
+    } else {
+        v = f4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u)};
+    }
+    return v;
+}
+__device__ __forceinline__ void store_row4(const RowsView& r, int64_t i, f4 v) {
+    if (r.type == FLLM_TYPE_F32) {
+        *(f4*)(r.p + 4 * i) = v;
+        return;
+    }
+    uint32_t h[4];
+    for (int e = 0; e < 4; e++) {
+        union { _Float16 h; uint16_t u; } c;
+        c.h = (_Float16)v[e];
+        h[e] = r.type == FLLM_TYPE_F16 ? c.u : bf16_round(v[e]);
+    }
+    *(u2*)(r.p + 2 * i) = u2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+}
+
 struct FewArgs {
     PagesView pg;
     const int* tables;
-    const int4* seqs;
     const AttnItem* items;
-    int tab_w, group, window;
+    int group, window;
     RowsView q, out;
     float scale, softcap;
     float *part_o, *part_ml;
     unsigned* cnt;
 };
 
+// Wide heads take the registers of two waves: one wave a SIMD then has as many bytes on their way.
 template <int TYPE, int HDP, int NP, int TM>
-__global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
+__global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(FewArgs a) {
     constexpr int NB = HDP / 32, ND = HDP / 16;      // blocks of 32 elements, tiles of 16
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
-    constexpr int JN = QUANT ? 2 : 1;                // runs of 32 keys a step
+    // runs of 32 keys a step: 16 bytes of V a lane, 8 where registers are short
+    constexpr int JN = QUANT && HDP <= 128 && TM == 1 ? 2 : 1;
     constexpr int STEP = 32 * JN, RUN = 8 * JN;      // keys a step, consecutive keys a lane holds
     constexpr int NV = TYPE == FLLM_TYPE_Q4_0 ? NB : ND;  // loads of V a step (one byte row holds two elements in Q4_0)
-    __shared__ float s_o[4][16][HDP + 4], s_m[4][16], s_l[4][16];
+    constexpr bool QLDS = HDP * TM >= 256;           // q stays in LDS where registers are short
+    __shared__ union {
+        _Float16 q[NP][16 * TM][HDP + 8];  // the rows' halves
+        float o[4][16][HDP + 4];           // a row tile's result of each wave
+        float w[kAttnMaxSplit * 32];       // weights of the parts
+    } sm;
+    __shared__ float s_m[4][16], s_l[4][16], s_scale[16 * TM];
     __shared__ int s_last;
 
     const int kvh = blockIdx.x % a.pg.nkv;
     const AttnItem it = a.items[blockIdx.x / a.pg.nkv];
-    const int4 sq = a.seqs[it.seq];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
     const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
-    const int pos0 = sq.z - sq.y;
-    const int* table = a.tables + (int64_t)it.seq * a.tab_w;
-    const int last_block = (sq.z - 1) >> lp;
+    const int pos0 = it.pos0;
+    const int* table = a.tables + it.table;
+    const int last_block = (it.len - 1) >> lp;
 
-    // this lane's query of each row tile: its position (-1 where there is no row), its operand halves
+    // q as fp16 halves in LDS, 16 lanes a row: every row scaled by the power of two 2^e that brings its largest
+    // magnitude into [2^14, 2^15); zeros for the rows and elements that are not there
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+        const int r = 16 * m + (threadIdx.x >> 4), l16 = threadIdx.x & 15;
+        const bool live = r < it.nrows;
+        const int row = it.row0 + (live ? r : 0), tok = row / a.group, head = kvh * a.group + row % a.group;
+        const int64_t at = (int64_t)(it.tok0 + tok) * a.q.ld + (int64_t)head * hd;
+        f4 x[HDP / 64];
+#pragma unroll
+        for (int i = 0; i < HDP / 64; i++) {
+            const int d = 4 * l16 + 64 * i;
+            x[i] = load_row4(a.q, at + (d < hd ? d : 0));
+            if (!live || d >= hd) x[i] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        float top = 0.0f;
+        for (int i = 0; i < HDP / 64; i++)
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[i][e]));
+        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const int e = row_exponent(top);
+#pragma unroll
+        for (int i = 0; i < HDP / 64; i++) {
+            const f4 y = x[i] * ldexpf(1.0f, e);
+            h2 h[NP][2];
+            split4<NP>(y, h);
+            for (int n = 0; n < NP; n++) *(u2*)&sm.q[n][r][4 * l16 + 64 * i] = u2{bits(h[n][0]), bits(h[n][1])};
+        }
+        if (l16 == 0) s_scale[r] = ldexpf(a.scale, -e) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+    }
+    __syncthreads();
+    // this lane's query of each row tile: its position (-1 where there is no row), what undoes its scaling
     int pos[TM];
     float unscale[TM];
-    h8 qf[TM][NB][NP];
+    h8 qr[QLDS ? 1 : TM][QLDS ? 1 : NB][NP];
+    const auto q_frag = [&](int m, int c, int n) {
+        const _Float16* p = &sm.q[n][16 * m + col][32 * c];
+        if (TYPE != FLLM_TYPE_Q4_0) return *(const h8*)(p + 8 * g);
+        H8 f;  // the elements that Frag's 8 stand for
+        *(u2*)&f.u[0] = *(const u2*)(p + 4 * g);
+        *(u2*)&f.u[2] = *(const u2*)(p + 16 + 4 * g);
+        return f.v;
+    };
 #pragma unroll
     for (int m = 0; m < TM; m++) {
         const int r = 16 * m + col;
-        const bool live = r < it.nrows;
-        const int row = it.row0 + (live ? r : 0), tok = row / a.group, head = kvh * a.group + row % a.group;
-        pos[m] = live ? pos0 + tok : -1;
-        const int64_t at = (int64_t)(sq.x + tok) * a.q.ld + (int64_t)head * hd;
-        float x[NB][8], top = 0.0f;
+        pos[m] = r < it.nrows ? pos0 + (it.row0 + r) / a.group : -1;
+        unscale[m] = s_scale[r];
+        if (!QLDS) {
 #pragma unroll
-        for (int c = 0; c < NB; c++)
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                // the elements that Frag's 8 stand for
-                const int d = TYPE == FLLM_TYPE_Q4_0 ? 32 * c + 16 * half + 4 * g : 32 * c + 8 * g + 4 * half;
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if (live && c < nb) {
-                    if (a.q.type == FLLM_TYPE_F32) {
-                        const f4 f = *(const f4*)(a.q.p + 4 * (at + d));
-                        for (int i = 0; i < 4; i++) v[i] = f[i];
-                    } else {
-                        const u2 u = *(const u2*)(a.q.p + 2 * (at + d));
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t h = (i < 2 ? u.x : u.y) >> (16 * (i & 1)) & 0xFFFFu;
-                            v[i] = a.q.type == FLLM_TYPE_F16 ? half_exact(h) : bf16_exact(h);
-                        }
-                    }
-                }
-                for (int i = 0; i < 4; i++) {
-                    x[c][4 * half + i] = v[i];
-                    top = fmaxf(top, fabsf(v[i]));
-                }
-            }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        int e = 0;
-        (void)frexpf(top, &e);  // top = f 2^e, f in [1/2, 1)
-        e = top > 0.0f && top < INFINITY ? 15 - e : 0;
-        e = e > 120 ? 120 : e;
-        for (int c = 0; c < NB; c++) {
-            for (int i = 0; i < 8; i++) x[c][i] = ldexpf(x[c][i], e);
-            split8<NP>(x[c], qf[m][c]);
+            for (int c = 0; c < NB; c++)
+                for (int n = 0; n < NP; n++) qr[m][c][n] = q_frag(m, c, n);
         }
-        unscale[m] = ldexpf(a.scale, -e) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
     }
+    const auto q_of = [&](int m, int c, int n) { return QLDS ? q_frag(m, c, n) : qr[QLDS ? 0 : m][QLDS ? 0 : c][n]; };
     const float cap = a.softcap * kLog2e;
 
     f4 o[TM][ND];
     float mx[TM], sum[TM];
-    int vexp = -1000;  // quantised: o is in units of 2^vexp
+    int vexp = -30;  // quantised: o is in units of 2^(vexp - 14), vexp at least the exponent of any scale so far (2^-24 and up, or zeros)
     for (int m = 0; m < TM; m++) {
         mx[m] = kNoScore;
         sum[m] = 0.0f;
         for (int d = 0; d < ND; d++) o[m][d] = f4{0.f, 0.f, 0.f, 0.f};
     }
+    // Elements past head_dim stand for those of block 0 in K (times zeros of q) and V (results dropped).
     // keys that every row sees need no mask: [all_lo, all_hi)
     const int last_pos = pos0 + (it.row0 + it.nrows - 1) / a.group;
     const int64_t all_lo = (int64_t)last_pos - a.window + 1, all_hi = pos0 + it.row0 / a.group + 1;
     const int64_t any_lo = all_hi - a.window;  // the first key that any row sees
 
-    const int ksub = QUANT ? 16 : 8;  // keys of a lane group
+    constexpr int ksub = RUN;  // keys of a lane group
     for (int k0 = it.k0 + wave * STEP; k0 < it.k1; k0 += 4 * STEP) {
+        if (QLDS) asm volatile("" ::: "memory");  // or its reads would be kept in registers across the loop
         // K: row col of tile (j, t) is key ksub (col >> 2) + 8 j + 4 t + (col & 3); V: this lane holds the
         // keys ksub g .. + RUN. Both lie in one page each; past the table's end the last page stands in.
         const int kk = k0 + ksub * (col >> 2), kv = k0 + ksub * g;
@@ -225,30 +289,32 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
         for (int t = 0; t < 2 * JN; t++)
 #pragma unroll
             for (int c = 0; c < NB; c++)
-                if (c < nb) kf[t][c].load(kp + (uint32_t)((c * P + 4 * t) * KB));
-        // scales of this lane's keys, 16 to a block
-        u4 ks[QUANT ? NB : 1][2], vs[QUANT ? NB : 1][2];
+                kf[t][c].load(kp + (uint32_t)(((c < nb ? c : 0) * P + 4 * t) * KB));
+        // scales of this lane's keys, 8 to a vector
+        u4 ks[QUANT ? NB : 1][JN], vs[QUANT ? NB : 1][JN];
         if (QUANT) {
 #pragma unroll
             for (int c = 0; c < NB; c++)
-                if (c < nb)
-                    for (int i = 0; i < 2; i++) {
-                        ks[c][i] = *(const u4*)(a.pg.k + cv + a.pg.scale_off + (uint32_t)(2 * (c * P + pv)) + 16 * i);
-                        vs[c][i] = *(const u4*)(a.pg.v + cv + a.pg.scale_off + (uint32_t)(2 * (c * P + pv)) + 16 * i);
-                    }
+                for (int i = 0; i < JN; i++) {
+                    const uint32_t at = a.pg.scale_off + (uint32_t)(2 * ((c < nb ? c : 0) * P + pv)) + 16 * i;
+                    ks[c][i] = *(const u4*)(a.pg.k + cv + at);
+                    vs[c][i] = *(const u4*)(a.pg.v + cv + at);
+                }
         }
-        u4 vf[NV];  // 16 bytes: 8 halves or 16 codes of this lane's keys
+        constexpr int VW = TYPE == FLLM_TYPE_F16 ? 4 : 2 * JN;
+        typedef uint32_t uv __attribute__((ext_vector_type(VW)));
+        uv vf[NV];  // 8 halves, or the codes of this lane's keys
         constexpr int VE = TYPE == FLLM_TYPE_F16 ? 2 : 1;
         const uint8_t* vp = a.pg.v + cv + (uint32_t)((col * P + pv) * VE);
 #pragma unroll
         for (int d = 0; d < NV; d++)
-            if (d * (TYPE == FLLM_TYPE_Q4_0 ? 32 : 16) < hd) vf[d] = *(const u4*)(vp + (uint32_t)(d * 16 * P * VE));
+            vf[d] = *(const uv*)(vp + (uint32_t)((d < (TYPE == FLLM_TYPE_Q4_0 ? nb : 2 * nb) ? d : 0) * 16 * P * VE));
 
         const bool edge = k0 < all_lo || k0 + STEP > all_hi;
         if (edge) {
             // what lies outside the sequence may be anything: no scale and no half of it may be a NaN
             for (int i = 0; i < RUN; i++) {
-                const bool in = kv + i >= any_lo && kv + i < sq.z;
+                const bool in = kv + i >= any_lo && kv + i < it.len;
                 if (QUANT) {
                     const uint32_t keep = in ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
 #pragma unroll
@@ -263,8 +329,7 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
         if (QUANT) {  // the units of o: the largest scale so far
             h2 top = {(_Float16)0, (_Float16)0};
             for (int c = 0; c < NB; c++)
-                if (c < nb)
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < 4 * JN; i++) {
                         union { uint32_t u; h2 h; } s;
                         s.u = vs[c][i >> 2][i & 3] & 0x7FFF7FFFu;
                         top = __builtin_elementwise_max(top, s.h);
@@ -274,7 +339,7 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
             f = fmaxf(f, __shfl_xor(f, 32));
             const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(f) >> 23) - 126);  // f < 2^e
             if (e > vexp) {
-                const float down = ldexpf(1.0f, vexp - e > -140 ? vexp - e : -140);
+                const float down = ldexpf(1.0f, vexp - e);
                 for (int m = 0; m < TM; m++)
                     for (int d = 0; d < ND; d++) o[m][d] *= down;
                 vexp = e;
@@ -290,18 +355,17 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
                 f4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int c = 0; c < NB; c++) {
-                    if (c >= nb) continue;
                     const h8 kh = kf[t][c].half();
                     if (QUANT) {
                         f4 b = {0.f, 0.f, 0.f, 0.f};
-                        for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[m][c][n], b, 0, 0, 0);
+                        for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, c, n), b, 0, 0, 0);
                         for (int e = 0; e < 4; e++) {
                             union { uint32_t u; h2 h; } d;
                             d.u = ks[c][t >> 1][2 * (t & 1) + (e >> 1)];
                             acc[e] = fmaf(b[e], (float)(e & 1 ? d.h.y : d.h.x), acc[e]);
                         }
                     } else {
-                        for (int n = NP - 1; n >= 0; n--) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qf[m][c][n], acc, 0, 0, 0);
+                        for (int n = NP - 1; n >= 0; n--) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, c, n), acc, 0, 0, 0);
                     }
                 }
                 for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e] * unscale[m];
@@ -324,7 +388,8 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
                 l += s[i];
             }
             sum[m] = sum[m] * down + l;
-            for (int d = 0; d < ND; d++) o[m][d] *= down;
+            if (__any(down != 1.0f))  // the maximum seldom grows after the first steps
+                for (int d = 0; d < ND; d++) o[m][d] *= down;
 
             if (!QUANT) {
                 float w[8];
@@ -333,7 +398,6 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
                 split8<NP>(w, wf);
 #pragma unroll
                 for (int d = 0; d < ND; d++) {
-                    if (d * 16 >= hd) continue;
                     H8 v;
                     for (int i = 0; i < 4; i++) v.u[i] = vf[d][i];
                     for (int n = NP - 1; n >= 0; n--) o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[n], o[m][d], 0, 0, 0);
@@ -342,14 +406,13 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
                 for (int i = 0; i < RUN; i++) s[i] *= vunit;
 #pragma unroll
                 for (int c = 0; c < NB; c++) {
-                    if (c >= nb) continue;
                     h8 wf[JN][NP];
                     for (int j = 0; j < JN; j++) {
                         float w[8];
                         for (int i = 0; i < 8; i++) {
                             union { uint32_t u; h2 h; } d;
                             d.u = vs[c][j][i >> 1];
-                            w[i] = s[8 * j + i] * (float)(i & 1 ? d.h.y : d.h.x);
+                            w[i] = fmaf((float)(i & 1 ? d.h.y : d.h.x), s[8 * j + i], 0.0f);
                         }
                         split8<NP>(w, wf[j]);
                     }
@@ -372,18 +435,22 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
     }
 
     // the four waves' results, a row tile at a time
-    const float unit = ldexpf(1.0f, QUANT ? (vexp > -1000 ? vexp - 14 : 0) : -14);
-    const int64_t part0 = ((int64_t)it.part + (int64_t)it.split * it.nrows) * a.pg.nkv + kvh;
+    const float unit = ldexpf(1.0f, QUANT ? vexp - 14 : -14);
+    // the tile's partial rows under this kv head: [split][row]
+    const int64_t part0 = (int64_t)it.part * a.pg.nkv + (int64_t)kvh * it.nsplit * it.nrows;
+    const uint32_t n_part = (uint32_t)(it.nsplit * it.nrows);
+    const __amdgpu_buffer_rsrc_t ro = wt_rsrc(a.part_o + part0 * hd, n_part * hd * 4);
+    const __amdgpu_buffer_rsrc_t rml = wt_rsrc(a.part_ml + 2 * part0, n_part * 8);
 #pragma unroll
     for (int m = 0; m < TM; m++) {
         sum[m] += __shfl_xor(sum[m], 16);
         sum[m] += __shfl_xor(sum[m], 32);
-        if (m) __syncthreads();
+        __syncthreads();  // q, or the tile before, is done with
         if (g == 0) {
             s_m[wave][col] = mx[m];
             s_l[wave][col] = sum[m];
         }
-        for (int d = 0; d < ND; d++) *(f4*)&s_o[wave][col][16 * d + 4 * g] = o[m][d] * unit;
+        for (int d = 0; d < ND; d++) *(f4*)&sm.o[wave][col][16 * d + 4 * g] = o[m][d] * unit;
         __syncthreads();
         for (int u = threadIdx.x; u < 16 * (HDP / 4); u += 256) {
             const int r = u / (HDP / 4), d = u % (HDP / 4) * 4, row = 16 * m + r;
@@ -394,20 +461,17 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
             for (int w = 0; w < 4; w++) {
                 const float f = __builtin_amdgcn_exp2f(s_m[w][r] - top);
                 l += f * s_l[w][r];
-                acc += f * *(const f4*)&s_o[w][r][d];
+                acc += f * *(const f4*)&sm.o[w][r][d];
             }
             if (it.nsplit == 1) {
                 const int tr = it.row0 + row, tok = tr / a.group, head = kvh * a.group + tr % a.group;
-                const int64_t at = (int64_t)(sq.x + tok) * a.out.ld + (int64_t)head * hd + d;
+                const int64_t at = (int64_t)(it.tok0 + tok) * a.out.ld + (int64_t)head * hd + d;
                 const float inv = 1.0f / l;
-                for (int i = 0; i < 4; i++) row_store(a.out, at + i, acc[i] * inv);
+                store_row4(a.out, at, acc * inv);
             } else {
-                const int64_t pr = part0 + (int64_t)row * a.pg.nkv;
-                for (int i = 0; i < 4; i++) st_wt(a.part_o + pr * hd + d + i, acc[i]);
-                if (d == 0) {
-                    st_wt(a.part_ml + 2 * pr, top);
-                    st_wt(a.part_ml + 2 * pr + 1, l);
-                }
+                const uint32_t pr = (uint32_t)(it.split * it.nrows + row);
+                __builtin_amdgcn_raw_buffer_store_b128(acc, ro, (pr * hd + d) * 4, 0, CPOL_SC1);
+                if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(f2{top, l}, rml, pr * 8, 0, CPOL_SC1);
             }
         }
     }
@@ -416,31 +480,47 @@ __global__ __launch_bounds__(256) void k_attend_few(FewArgs a) {
     // the tile's last item joins the partial rows
     wt_complete();
     __syncthreads();
-    unsigned* cnt = a.cnt + (int64_t)it.part * a.pg.nkv + kvh;
+    unsigned* cnt = a.cnt + part0;
     if (threadIdx.x == 0)
         s_last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(it.nsplit - 1);
     __syncthreads();
     if (!s_last) return;
     if (threadIdx.x == 0) st_wt_u(cnt, 0u);
+    // weights of the parts, a wave per row: exp2(m - max) / sum
+    for (int row = wave; row < it.nrows; row += 4) {
+        float m1[kAttnMaxSplit / 64], l1[kAttnMaxSplit / 64], top = kNoScore, l = 0.0f;
+        for (int i = 0; i < kAttnMaxSplit / 64; i++) {
+            const int k = lane + 64 * i;
+            const float2 v = ld_wt2(rml, (uint32_t)((k < it.nsplit ? k : 0) * it.nrows + row) * 8);
+            m1[i] = k < it.nsplit ? v.x : kNoScore;
+            l1[i] = k < it.nsplit ? v.y : 0.0f;
+            top = fmaxf(top, m1[i]);
+        }
+        top = wave_max(top);
+        for (int i = 0; i < kAttnMaxSplit / 64; i++) {
+            m1[i] = __builtin_amdgcn_exp2f(m1[i] - top);
+            l += m1[i] * l1[i];
+        }
+        const float inv = 1.0f / wave_sum(l);
+        for (int i = 0; i < kAttnMaxSplit / 64; i++)
+            if (lane + 64 * i < it.nsplit) sm.w[row * kAttnMaxSplit + lane + 64 * i] = m1[i] * inv;
+    }
+    __syncthreads();
     for (int u = threadIdx.x; u < it.nrows * (hd / 4); u += 256) {
         const int row = u / (hd / 4), d = u % (hd / 4) * 4;
-        float top = kNoScore, l = 0.0f;
         f4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < it.nsplit; k++) {
-            const int64_t pr = ((int64_t)it.part + (int64_t)k * it.nrows + row) * a.pg.nkv + kvh;
-            const float m1 = __hip_atomic_load(a.part_ml + 2 * pr, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float l1 = __hip_atomic_load(a.part_ml + 2 * pr + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            f4 p;
-            for (int i = 0; i < 4; i++) p[i] = __hip_atomic_load(a.part_o + pr * hd + d + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const float nm = fmaxf(top, m1), f0 = __builtin_amdgcn_exp2f(top - nm), f1 = __builtin_amdgcn_exp2f(m1 - nm);
-            acc = acc * f0 + p * f1;
-            l = l * f0 + l1 * f1;
-            top = nm;
+        for (int k0 = 0; k0 < it.nsplit; k0 += 16) {  // 16 loads on their way; those past the end read zeros
+            float4 v[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = ld_wt4(ro, (uint32_t)(((k0 + i) * it.nrows + row) * hd + d) * 4);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float w = k0 + i < it.nsplit ? sm.w[row * kAttnMaxSplit + k0 + i] : 0.0f;
+                acc += w * f4{v[i].x, v[i].y, v[i].z, v[i].w};
+            }
         }
         const int tr = it.row0 + row, tok = tr / a.group, head = kvh * a.group + tr % a.group;
-        const int64_t at = (int64_t)(sq.x + tok) * a.out.ld + (int64_t)head * hd + d;
-        const float inv = 1.0f / l;
-        for (int i = 0; i < 4; i++) row_store(a.out, at + i, acc[i] * inv);
+        store_row4(a.out, (int64_t)(it.tok0 + tok) * a.out.ld + (int64_t)head * hd + d, acc);
     }
 }
 
@@ -476,7 +556,7 @@ hipError_t launch_few_np(const FewArgs& a, const AttnWork& w, hipStream_t st) {
 
 hipError_t launch_pages_attention(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q,
                                   const RowsView& out, float scale, float softcap, hipStream_t st) {
-    const FewArgs a{pg, b.tables, b.seqs, nullptr, b.tab_w, b.n_heads / pg.nkv, b.window, q, out, scale, softcap,
+    const FewArgs a{pg, b.tables, nullptr, b.n_heads / pg.nkv, b.window, q, out, scale, softcap,
                     w.part, w.part + w.part_rows * pg.nkv * pg.hd, w.cnt};
     switch (pg.type) {
         case FLLM_TYPE_F16: return launch_few_np<FLLM_TYPE_F16>(a, w, st);

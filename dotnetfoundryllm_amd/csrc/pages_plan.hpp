@@ -168,11 +168,14 @@ inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, 
 // The rows of a sequence under one kv head are its new tokens times the head group: row r is token
 // r / group, query head kvh * group + r % group. A tile is some of them; an item is a tile with a range
 // [k0, k1) of the keys that its rows see, cut at multiples of kKeyStep. A tile of several items leaves a partial
-// result of each: rows part + split * nrows .. of the partial rows, which the last item to finish joins.
+// result of each, nsplit * nrows rows from `part` on per kv head, which the last item to finish joins.
 struct AttnItem {
     int seq, row0, nrows, k0, k1, part, split, nsplit;
+    int tok0, pos0, len, table;  // of the sequence: its first new row and that row's position, its length, its table's start
+    int pad[4];
 };
 constexpr int kKeyStep = 64;
+constexpr int kAttnMaxSplit = 128;  // items of a tile
 
 struct AttnPlan {
     std::vector<AttnItem> items[2];  // tiles of up to 16 rows, of up to 32
@@ -180,8 +183,8 @@ struct AttnPlan {
 };
 
 // Items of the tiles of `tile` rows of sequence i, each of at most `steps` steps of keys.
-inline void attn_items(const SeqPlan& s, int i, int group, int window, int tile, int64_t steps, std::vector<AttnItem>* out,
-                       int64_t* part_rows) {
+inline void attn_items(const SeqPlan& s, int i, int table, int group, int window, int tile, int64_t steps,
+                       std::vector<AttnItem>* out, int64_t* part_rows) {
     const int64_t rows = (int64_t)s.n_new * group;
     for (int64_t r = 0; r < rows; r += tile) {
         const int n = (int)std::min<int64_t>(tile, rows - r);
@@ -190,41 +193,49 @@ inline void attn_items(const SeqPlan& s, int i, int group, int window, int tile,
         const int g0 = low > 0 ? (int)(low / kKeyStep) : 0;
         const int last = pos0 + (int)((r + n - 1) / group);
         const int g1 = last / kKeyStep + 1;
-        const int nsplit = (int)((g1 - g0 + steps - 1) / steps), per = (g1 - g0 + nsplit - 1) / nsplit;
+        const int nsplit = (int)std::min<int64_t>(kAttnMaxSplit, (g1 - g0 + steps - 1) / steps), per = (g1 - g0 + nsplit - 1) / nsplit;
         const int used = (g1 - g0 + per - 1) / per;
         for (int k = 0; k < used; k++)
             out->push_back({i, (int)r, n, (g0 + k * per) * kKeyStep, std::min((g0 + (k + 1) * per) * kKeyStep, last + 1),
-                            (int)*part_rows, k, used});
+                            (int)*part_rows, k, used, s.row0, pos0, s.len, table, {0, 0, 0, 0}});
         if (used > 1) *part_rows += (int64_t)used * n;
     }
 }
 
-// steps that all items of `tile`-row tiles over sequence s take under one kv head
-inline int64_t attn_steps(const SeqPlan& s, int group, int window, int tile) {
+// Items under one kv head that a sequence's tiles of `tile` rows become with at most `steps` steps of keys each.
+inline int64_t attn_count(const SeqPlan& s, int group, int window, int tile, int64_t steps) {
     int64_t sum = 0;
     const int64_t rows = (int64_t)s.n_new * group;
     for (int64_t r = 0; r < rows; r += tile) {
         const int64_t low = (int64_t)s.len - s.n_new + r / group - window + 1;
         const int64_t last = (int64_t)s.len - s.n_new + (std::min<int64_t>(rows, r + tile) - 1) / group;
-        sum += last / kKeyStep + 1 - (low > 0 ? low / kKeyStep : 0);
+        sum += std::min<int64_t>(kAttnMaxSplit, (last / kKeyStep + 1 - (low > 0 ? low / kKeyStep : 0) + steps - 1) / steps);
     }
     return sum;
 }
 
 // The items of a batch on a device of n_cu CUs. False where they or their partial rows are too many.
-inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int window, int n_cu, AttnPlan* p) {
+inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, int window, int n_cu, AttnPlan* p) {
     const int group = n_heads / n_kv;
     p->part_rows = 0;
-    int64_t steps = 0;
     const auto tile_of = [&](const SeqPlan& s) { return (int64_t)s.n_new * group <= 16 ? 16 : 32; };
-    for (const SeqPlan& s : b.seqs) steps += attn_steps(s, group, window, tile_of(s));
-    // as many steps an item as give every CU a few workgroups, one step at least for each of their waves
-    const int64_t want = std::max<int64_t>(4, steps * n_kv / ((int64_t)n_cu * 4));
+    // Two workgroups are resident on a CU, one of heads wider than 128: the shortest items whose workgroups all
+    // start at once (a key step for each of the four waves at least), so that the longest one is as short as it
+    // can be.
+    const int64_t slots = (head_dim > 128 ? 1 : 2) * (int64_t)n_cu;
+    int64_t lo = 4, hi = kPagesMaxLength / kKeyStep + 1;
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        int64_t n = 0;
+        for (const SeqPlan& s : b.seqs) n += attn_count(s, group, window, tile_of(s), mid);
+        if (n * n_kv <= slots) hi = mid;
+        else lo = mid + 1;
+    }
     for (int c = 0; c < 2; c++) p->items[c].clear();
     for (int i = 0; i < b.n_seqs; i++) {
         const SeqPlan& s = b.seqs[(size_t)i];
         const int tile = tile_of(s);
-        if (s.n_new) attn_items(s, i, group, window, tile, want, &p->items[tile == 16 ? 0 : 1], &p->part_rows);
+        if (s.n_new) attn_items(s, i, i * b.tab_w, group, window, tile, lo, &p->items[tile == 16 ? 0 : 1], &p->part_rows);
         if (p->part_rows > INT32_MAX / n_kv) return false;
     }
     for (auto& v : p->items) {

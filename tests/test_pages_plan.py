@@ -40,7 +40,7 @@ def items(so):
     out = []
     for c in range(len(TILE)):
         n = so.plan_items(c, None)
-        a = np.zeros((n, 8), np.int32)
+        a = np.zeros((n, 16), np.int32)
         so.plan_items(c, a.ctypes.data_as(C.c_void_p))
         out.append(a)
     return out
@@ -88,12 +88,13 @@ def check(so, new, length, heads, kv, window):
     group = heads // kv
     seen = {}      # (sequence, row) -> ranges
     parts = set()  # partial rows in use
-    limit = so.plan_part_rows()
+    limit, tab_w = so.plan_part_rows(), sizes(so)["tab_w"]
     for c, list_ in enumerate(items(so)):
-        for seq, row0, nrows, k0, k1, part, split, nsplit in list_.tolist():
+        for seq, row0, nrows, k0, k1, part, split, nsplit, tok0, pos0, ln, table in list_[:, :12].tolist():
             assert 0 <= seq < len(new) and 0 <= row0 and 1 <= nrows <= TILE[c] and row0 + nrows <= new[seq] * group
-            assert 0 <= k0 < k1 <= length[seq] and k0 % STEP == 0 and 0 <= split < nsplit
+            assert 0 <= k0 < k1 <= length[seq] and k0 % STEP == 0 and 0 <= split < nsplit <= 128
             assert k1 % STEP == 0 or split == nsplit - 1
+            assert (tok0, pos0, ln, table) == (sum(new[:seq]), length[seq] - new[seq], length[seq], seq * tab_w)
             for r in range(row0, row0 + nrows):
                 seen.setdefault((seq, r), []).append((k0, k1))
             if nsplit > 1:
