@@ -43,7 +43,7 @@ def _run(cmd, cwd):
 
 
 DEVICE_SRCS = ["csrc/kernels.hip", "csrc/gemv.hip", "csrc/attention.hip", "csrc/prefill.hip", "csrc/pf_gemm8.hip", "csrc/pages.hip",
-               "csrc/pages_attention.hip", "csrc/draft.hip", "csrc/api.hip", "csrc/api_pages.hip"]
+               "csrc/pages_attention.hip", "csrc/pages_attend_f16.hip", "csrc/pages_attend_q8_0.hip", "csrc/pages_attend_q4_0.hip", "csrc/draft.hip", "csrc/api.hip", "csrc/api_pages.hip"]
 
 
 def build_device_lib(verbose=False):

@@ -197,22 +197,23 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         }
         b->plan.n_seqs = 0;  // empty until everything is on its way
         // sequences, items, tables: parts of 16, 64 and 4 bytes
-        const void* from[4] = {pl.seqs.data(), b->attn.items[0].data(), b->attn.items[1].data(), pl.tables.data()};
-        const uint64_t size[4] = {(pl.seqs.size() * sizeof(SeqPlan) + 63) / 64 * 64, b->attn.items[0].size() * sizeof(AttnItem),
-                                  b->attn.items[1].size() * sizeof(AttnItem), pl.tables.size() * sizeof(int32_t)};
-        uint64_t at[5] = {0};
-        for (int i = 0; i < 4; i++) at[i + 1] = at[i] + size[i];
-        hipError_t e = batch_room(b, at[4]);
+        const auto& items = b->attn.items;
+        const void* from[5] = {pl.seqs.data(), items[0].data(), items[1].data(), items[2].data(), pl.tables.data()};
+        const uint64_t size[5] = {(pl.seqs.size() * sizeof(SeqPlan) + 63) / 64 * 64, items[0].size() * sizeof(AttnItem),
+                                  items[1].size() * sizeof(AttnItem), items[2].size() * sizeof(AttnItem), pl.tables.size() * sizeof(int32_t)};
+        uint64_t at[6] = {0};
+        for (int i = 0; i < 5; i++) at[i + 1] = at[i] + size[i];
+        hipError_t e = batch_room(b, at[5]);
         if (e != hipSuccess)
             return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "batch memory: %s", hipGetErrorString(e));
-        for (int i = 0; i < 4; i++)
+        for (int i = 0; i < 5; i++)
             if (size[i]) memcpy(b->pin + at[i], from[i], i ? size[i] : pl.seqs.size() * sizeof(SeqPlan));
-        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, at[4], hipMemcpyHostToDevice, p->ctx->stream));
+        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, at[5], hipMemcpyHostToDevice, p->ctx->stream));
         HIP_TRY(hipEventRecord(b->sent, p->ctx->stream));
         b->in_flight = true;
         b->plan.n_seqs = n_plan_seqs;
         b->view.seqs = (const int4*)b->dev;
-        b->view.tables = (const int*)(b->dev + at[3]);
+        b->view.tables = (const int*)(b->dev + at[4]);
         b->view.tab_w = pl.tab_w;
         b->view.n_seqs = n_plan_seqs;
         b->view.new_blocks = pl.new_blocks;
@@ -220,7 +221,7 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         b->view.n_rows = pl.n_rows;
         b->view.n_heads = b->n_heads;
         b->view.window = b->window;
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 3; i++) {
             b->work.items[i] = (const AttnItem*)(b->dev + at[1 + i]);
             b->work.n[i] = (int)b->attn.items[i].size();
         }

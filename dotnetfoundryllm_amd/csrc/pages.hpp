@@ -35,17 +35,25 @@ hipError_t launch_pages_append(const PagesView& pg, const BatchView& b, const Ro
 hipError_t launch_pages_read(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v,
                              hipStream_t st);
 struct AttnItem;
-// Attention items on the device (pages_plan.hpp): tiles of up to 16 rows, then of up to 32; part: room
+// Attention items on the device (pages_plan.hpp): tiles of up to 16 rows, of up to 32, of up to 128; part: room
 // for part_rows * nkv rows of head_dim floats, then a max and a sum for each; cnt: as many zeros, left as zeros.
 struct AttnWork {
-    const AttnItem* items[2];
-    int n[2];
+    const AttnItem* items[3];
+    int n[3];
     float* part;
     unsigned* cnt;
     int64_t part_rows;
 };
 hipError_t launch_pages_attention(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q,
                                   const RowsView& out, float scale, float softcap, hipStream_t st);
+
+// the same for one cache type each
+hipError_t launch_attend_f16(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q, const RowsView& out,
+                             float scale, float softcap, hipStream_t st);
+hipError_t launch_attend_q8_0(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q, const RowsView& out,
+                              float scale, float softcap, hipStream_t st);
+hipError_t launch_attend_q4_0(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q, const RowsView& out,
+                              float scale, float softcap, hipStream_t st);
 
 struct DraftView {
     int n_seqs, n_draft, vocab;

@@ -1,0 +1,941 @@
+// pages_attend.hpp — the kernels that attend from new tokens to the pages of their sequences; one translation
+// unit per cache type (pages_attend_f16.hip, pages_attend_q8_0.hip, pages_attend_q4_0.hip) instantiates them.
+//
+// Mathematics. o = sum_j w_j v_j / sum_j w_j, w_j = exp(s_j - m), in one pass over the keys with the
+// running maximum m: whatever has been summed is multiplied by exp(m_old - m_new) when m grows. The
+// products run on the fp16 matrix cores, transposed: S^T = K Q^T and O^T = V^T P^T, so that a lane
+// holds one query's scores (column l & 15 of the tile) and the weights are, as they lie in the score
+// registers, the second product's operand. All sums are f32.
+//
+// Factors. Every row of q is scaled by a power of two (largest magnitude into [2^14, 2^15)) and rounded
+// to fp16, for F32 rows as a high and a low half that together keep 22 bits (NP = 2: two products in place of
+// one). K and V enter exactly: the halves of an F16 cache, the codes of a quantised one as
+// integers, whose scales are applied in f32: to the scores block by block, and to the weights before they are
+// rounded (as one or two halves), so that a V block's product is weights-times-scales by codes.
+//
+// k_attend_few: up to 16 TM rows (decoding, drafted tokens), bound by the bytes of K and V. A wave
+// takes steps of 64 keys (32 of an F16 cache) for all rows straight from the pages into registers: the page
+// layouts (fllm.h) are such that 8 consecutive elements of an operand are contiguous in memory, so
+// there is no LDS stage and no barrier in the loop. The four waves of a workgroup take turns at the
+// steps of an item; their results meet in LDS, and those of a tile's items in memory, joined by
+// the item that finishes last (write-through stores and a counter, as the decode attention of
+// attn_body.hpp, so no second launch).
+#pragma once
+
+#include "attn_body.hpp"
+#include "pages.hpp"
+#include "pages_plan.hpp"
+
+namespace fllm {
+
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNoScore = -1e30f;  // the running maximum before any key
+
+union H8 {
+    h8 v;
+    h2 p[4];
+    uint32_t u[4];
+};
+
+// 4 bytes, each code + 128 or nibble, as fp16 integers: 0x6400 | byte is 1024 + byte exactly
+template <int OFF>
+__device__ __forceinline__ void bytes_to_half(uint32_t w, uint32_t* out) {
+    const h2 off = {(_Float16)OFF, (_Float16)OFF};
+    union { uint32_t u; h2 h; } a, b;
+    a.u = __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u);
+    b.u = __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u);
+    a.h = a.h - off;
+    b.h = b.h - off;
+    out[0] = a.u;
+    out[1] = b.u;
+}
+
+// A lane's 8 operand elements out of what it loads of a cell: 16, 8 or 4 bytes.
+template <int TYPE> struct Frag;
+template <> struct Frag<FLLM_TYPE_F16> {
+    u4 w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *(const u4*)p; }
+    __device__ __forceinline__ h8 half() const {
+        H8 r;
+        for (int i = 0; i < 4; i++) r.u[i] = w[i];
+        return r.v;
+    }
+};
+template <> struct Frag<FLLM_TYPE_Q8_0> {
+    u2 w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *(const u2*)p; }
+    __device__ __forceinline__ h8 half() const {
+        H8 r;
+        bytes_to_half<1152>(w.x ^ 0x80808080u, r.u);
+        bytes_to_half<1152>(w.y ^ 0x80808080u, r.u + 2);
+        return r.v;
+    }
+};
+template <> struct Frag<FLLM_TYPE_Q4_0> {  // elements 4 g .. + 3 in the low halves, 16 + 4 g .. in the high ones
+    uint32_t w;
+    __device__ __forceinline__ void load(const uint8_t* p) { w = *(const uint32_t*)p; }
+    __device__ __forceinline__ h8 half() const {
+        H8 r;
+        bytes_to_half<1032>(w & 0x0F0F0F0Fu, r.u);
+        bytes_to_half<1032>(w >> 4 & 0x0F0F0F0Fu, r.u + 2);
+        return r.v;
+    }
+};
+
+__device__ __forceinline__ uint32_t bits(h2 h) {
+    union { uint32_t u; h2 h; } c;
+    c.h = h;
+    return c.u;
+}
+
+// e such that 2^e brings a largest magnitude `top` into [2^14, 2^15); 0 for zeros and what is no number
+__device__ __forceinline__ int row_exponent(float top) {
+    if (!(top > 0.0f && top < INFINITY)) return 0;
+    const int e = 15 - __builtin_amdgcn_frexp_expf(top);  // top = f 2^k, f in [1/2, 1): e = 15 - k
+    return e > 120 ? 120 : e;
+}
+
+// x as fp16 halves: one rounded to nearest, or a high and a low one (both cut, together 21 to 22 bits)
+template <int NP>
+__device__ __forceinline__ void split4(const f4 x, h2 out[NP][2]) {
+    for (int i = 0; i < 2; i++) {
+        if (NP == 1) {
+            out[0][i] = h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+        } else {
+            union { __fp16 __attribute__((ext_vector_type(2))) c; h2 h; } a, b;
+            a.c = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
+            b.c = __builtin_amdgcn_cvt_pkrtz(fmaf((float)a.h.x, -1.0f, x[2 * i]), fmaf((float)a.h.y, -1.0f, x[2 * i + 1]));
+            out[0][i] = a.h;
+            out[NP - 1][i] = b.h;
+        }
+    }
+}
+template <int NP>
+__device__ __forceinline__ void split8(const float x[8], h8 out[NP]) {
+    h2 a[NP][2], b[NP][2];
+    split4<NP>(f4{x[0], x[1], x[2], x[3]}, a);
+    split4<NP>(f4{x[4], x[5], x[6], x[7]}, b);
+    for (int n = 0; n < NP; n++) {
+        H8 h;
+        h.p[0] = a[n][0], h.p[1] = a[n][1], h.p[2] = b[n][0], h.p[3] = b[n][1];
+        out[n] = h.v;
+    }
+}
+
+// tanh to 1e-7: a series near zero, where the quotient would cancel
+__device__ __forceinline__ float tanh_of(float x) {
+    const float y = x * x;
+    const float p = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
+    const float q = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+    return fabsf(x) < 0.25f ? p : q;
+}
+
+__device__ __forceinline__ f4 load_row4(const RowsView& r, int64_t i) {
+    if (r.type == FLLM_TYPE_F32) return *(const f4*)(r.p + 4 * i);
+    const u2 u = *(const u2*)(r.p + 2 * i);
+    f4 v;
+    if (r.type == FLLM_TYPE_F16) {
+        union { uint32_t u; h2 h; } a, b;
+        a.u = u.x;
+        b.u = u.y;
+        v = f4{(float)a.h.x, (float)a.h.y, (float)b.h.x, (float)b.h.y};
+    } else {
+        v = f4{__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xFFFF0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xFFFF0000u)};
+    }
+    return v;
+}
+__device__ __forceinline__ void store_row4(const RowsView& r, int64_t i, f4 v) {
+    if (r.type == FLLM_TYPE_F32) {
+        *(f4*)(r.p + 4 * i) = v;
+        return;
+    }
+    uint32_t h[4];
+    for (int e = 0; e < 4; e++) {
+        union { _Float16 h; uint16_t u; } c;
+        c.h = (_Float16)v[e];
+        h[e] = r.type == FLLM_TYPE_F16 ? c.u : bf16_round(v[e]);
+    }
+    *(u2*)(r.p + 2 * i) = u2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+}
+
+struct AttnArgsP {
+    PagesView pg;
+    const int* tables;
+    const AttnItem* items;
+    int group, window;
+    RowsView q, out;
+    float scale, softcap;
+    float *part_o, *part_ml;
+    unsigned* cnt;
+};
+
+// Counts this workgroup's partial rows, whose stores were all issued before, as there; true for the workgroup that
+// completes the tile's `n`, which also leaves the counter at zero for the next call.
+__device__ __forceinline__ bool last_of_tile(unsigned* cnt, int n, int* s_last) {
+    wt_complete();
+    __syncthreads();
+    if (threadIdx.x == 0)
+        *s_last = __hip_atomic_fetch_add(cnt, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(n - 1);
+    __syncthreads();
+    if (*s_last && threadIdx.x == 0) st_wt_u(cnt, 0u);
+    return *s_last != 0;
+}
+
+// Joins a tile's partial rows [split][row] (ro: head_dim floats, rml: max and sum) into out. w: MAXS floats a row.
+template <int MAXS>
+__device__ __forceinline__ void join_parts(const AttnArgsP& a, const AttnItem& it, int kvh, __amdgpu_buffer_rsrc_t ro,
+                                           __amdgpu_buffer_rsrc_t rml, float* w) {
+    constexpr int N = (MAXS + 63) / 64;
+    const int lane = threadIdx.x & 63, hd = a.pg.hd;
+    // weights of the parts, a wave per row: exp2(m - max) / sum
+    for (int row = threadIdx.x >> 6; row < it.nrows; row += 4) {
+        float m1[N], l1[N], top = kNoScore, l = 0.0f;
+        for (int i = 0; i < N; i++) {
+            const int k = lane + 64 * i;
+            const float2 v = ld_wt2(rml, (uint32_t)((k < it.nsplit ? k : 0) * it.nrows + row) * 8);
+            m1[i] = k < it.nsplit ? v.x : kNoScore;
+            l1[i] = k < it.nsplit ? v.y : 0.0f;
+            top = fmaxf(top, m1[i]);
+        }
+        top = wave_max(top);
+        for (int i = 0; i < N; i++) {
+            m1[i] = __builtin_amdgcn_exp2f(m1[i] - top);
+            l += m1[i] * l1[i];
+        }
+        const float inv = 1.0f / wave_sum(l);
+        for (int i = 0; i < N; i++)
+            if (lane + 64 * i < it.nsplit) w[row * MAXS + lane + 64 * i] = m1[i] * inv;
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < it.nrows * (hd / 4); u += 256) {
+        const int row = u / (hd / 4), d = u % (hd / 4) * 4;
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int k0 = 0; k0 < it.nsplit; k0 += 16) {  // 16 loads on their way; those past the end read zeros
+            float4 v[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) v[i] = ld_wt4(ro, (uint32_t)(((k0 + i) * it.nrows + row) * hd + d) * 4);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float f = k0 + i < it.nsplit ? w[row * MAXS + k0 + i] : 0.0f;
+                acc += f * f4{v[i].x, v[i].y, v[i].z, v[i].w};
+            }
+        }
+        const int tr = it.row0 + row, tok = tr / a.group, head = kvh * a.group + tr % a.group;
+        store_row4(a.out, (int64_t)(it.tok0 + tok) * a.out.ld + (int64_t)head * hd + d, acc);
+    }
+}
+
+// Wide heads take the registers of two waves: one wave a SIMD then has as many bytes on their way.
+template <int TYPE, int HDP, int NP, int TM>
+__global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP a) {
+    constexpr int NB = HDP / 32, ND = HDP / 16;      // blocks of 32 elements, tiles of 16
+    constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
+    // runs of 32 keys a step: 16 bytes of V a lane, 8 where registers are short
+    constexpr int JN = QUANT && HDP <= 128 && TM == 1 ? 2 : 1;
+    constexpr int STEP = 32 * JN, RUN = 8 * JN;      // keys a step, consecutive keys a lane holds
+    constexpr int NV = TYPE == FLLM_TYPE_Q4_0 ? NB : ND;  // loads of V a step (one byte row holds two elements in Q4_0)
+    constexpr bool QLDS = HDP * TM >= 256;           // q stays in LDS where registers are short
+    __shared__ union {
+        _Float16 q[NP][16 * TM][HDP + 8];  // the rows' halves
+        float o[4][16][HDP + 4];           // a row tile's result of each wave
+        float w[kAttnSplit[0] * 32];       // weights of the parts
+    } sm;
+    __shared__ float s_m[4][16], s_l[4][16], s_scale[16 * TM];
+    __shared__ int s_last;
+
+    const int kvh = blockIdx.x % a.pg.nkv;
+    const AttnItem it = a.items[blockIdx.x / a.pg.nkv];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
+    const int pos0 = it.pos0;
+    const int* table = a.tables + it.table;
+    const int last_block = (it.len - 1) >> lp;
+
+    // q as fp16 halves in LDS, 16 lanes a row: every row scaled by the power of two 2^e that brings its largest
+    // magnitude into [2^14, 2^15); zeros for the rows and elements that are not there
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+        const int r = 16 * m + (threadIdx.x >> 4), l16 = threadIdx.x & 15;
+        const bool live = r < it.nrows;
+        const int row = it.row0 + (live ? r : 0), tok = row / a.group, head = kvh * a.group + row % a.group;
+        const int64_t at = (int64_t)(it.tok0 + tok) * a.q.ld + (int64_t)head * hd;
+        f4 x[HDP / 64];
+#pragma unroll
+        for (int i = 0; i < HDP / 64; i++) {
+            const int d = 4 * l16 + 64 * i;
+            x[i] = load_row4(a.q, at + (d < hd ? d : 0));
+            if (!live || d >= hd) x[i] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+        float top = 0.0f;
+        for (int i = 0; i < HDP / 64; i++)
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(x[i][e]));
+        for (int o = 1; o < 16; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const int e = row_exponent(top);
+#pragma unroll
+        for (int i = 0; i < HDP / 64; i++) {
+            const f4 y = x[i] * ldexpf(1.0f, e);
+            h2 h[NP][2];
+            split4<NP>(y, h);
+            for (int n = 0; n < NP; n++) *(u2*)&sm.q[n][r][4 * l16 + 64 * i] = u2{bits(h[n][0]), bits(h[n][1])};
+        }
+        if (l16 == 0) s_scale[r] = ldexpf(a.scale, -e) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+    }
+    __syncthreads();
+    // this lane's query of each row tile: its position (-1 where there is no row), what undoes its scaling
+    int pos[TM];
+    float unscale[TM];
+    h8 qr[QLDS ? 1 : TM][QLDS ? 1 : NB][NP];
+    const auto q_frag = [&](int m, int c, int n) {
+        const _Float16* p = &sm.q[n][16 * m + col][32 * c];
+        if (TYPE != FLLM_TYPE_Q4_0) return *(const h8*)(p + 8 * g);
+        H8 f;  // the elements that Frag's 8 stand for
+        *(u2*)&f.u[0] = *(const u2*)(p + 4 * g);
+        *(u2*)&f.u[2] = *(const u2*)(p + 16 + 4 * g);
+        return f.v;
+    };
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+        const int r = 16 * m + col;
+        pos[m] = r < it.nrows ? pos0 + (it.row0 + r) / a.group : -1;
+        unscale[m] = s_scale[r];
+        if (!QLDS) {
+#pragma unroll
+            for (int c = 0; c < NB; c++)
+                for (int n = 0; n < NP; n++) qr[m][c][n] = q_frag(m, c, n);
+        }
+    }
+    const auto q_of = [&](int m, int c, int n) { return QLDS ? q_frag(m, c, n) : qr[QLDS ? 0 : m][QLDS ? 0 : c][n]; };
+    const float cap = a.softcap * kLog2e;
+
+    f4 o[TM][ND];
+    float mx[TM], sum[TM];
+    int vexp = -30;  // quantised: o is in units of 2^(vexp - 14), vexp at least the exponent of any scale so far (2^-24 and up, or zeros)
+    for (int m = 0; m < TM; m++) {
+        mx[m] = kNoScore;
+        sum[m] = 0.0f;
+        for (int d = 0; d < ND; d++) o[m][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // Elements past head_dim stand for those of block 0 in K (times zeros of q) and V (results dropped).
+    // keys that every row sees need no mask: [all_lo, all_hi)
+    const int last_pos = pos0 + (it.row0 + it.nrows - 1) / a.group;
+    const int64_t all_lo = (int64_t)last_pos - a.window + 1, all_hi = pos0 + it.row0 / a.group + 1;
+    const int64_t any_lo = all_hi - a.window;  // the first key that any row sees
+
+    constexpr int ksub = RUN;  // keys of a lane group
+    for (int k0 = it.k0 + wave * STEP; k0 < it.k1; k0 += 4 * STEP) {
+        if (QLDS) asm volatile("" ::: "memory");  // or its reads would be kept in registers across the loop
+        // K: row col of tile (j, t) is key ksub (col >> 2) + 8 j + 4 t + (col & 3); V: this lane holds the
+        // keys ksub g .. + RUN. Both lie in one page each; past the table's end the last page stands in.
+        const int kk = k0 + ksub * (col >> 2), kv = k0 + ksub * g;
+        const int bk = min(kk >> lp, last_block), bv = min(kv >> lp, last_block);
+        const uint64_t ck = ((uint64_t)(uint32_t)table[bk] * a.pg.nkv + kvh) * a.pg.cell;
+        const uint64_t cv = ((uint64_t)(uint32_t)table[bv] * a.pg.nkv + kvh) * a.pg.cell;
+        const int pk = (kk & (P - 1)) + (col & 3), pv = kv & (P - 1);
+        constexpr int KB = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;  // bytes of a block's codes
+        const uint8_t* kp = a.pg.k + ck + (uint32_t)(pk * KB + g * (KB / 4));
+        Frag<TYPE> kf[2 * JN][NB];
+#pragma unroll
+        for (int t = 0; t < 2 * JN; t++)
+#pragma unroll
+            for (int c = 0; c < NB; c++)
+                kf[t][c].load(kp + (uint32_t)(((c < nb ? c : 0) * P + 4 * t) * KB));
+        // scales of this lane's keys, 8 to a vector
+        u4 ks[QUANT ? NB : 1][JN], vs[QUANT ? NB : 1][JN];
+        if (QUANT) {
+#pragma unroll
+            for (int c = 0; c < NB; c++)
+                for (int i = 0; i < JN; i++) {
+                    const uint32_t at = a.pg.scale_off + (uint32_t)(2 * ((c < nb ? c : 0) * P + pv)) + 16 * i;
+                    ks[c][i] = *(const u4*)(a.pg.k + cv + at);
+                    vs[c][i] = *(const u4*)(a.pg.v + cv + at);
+                }
+        }
+        constexpr int VW = TYPE == FLLM_TYPE_F16 ? 4 : 2 * JN;
+        typedef uint32_t uv __attribute__((ext_vector_type(VW)));
+        uv vf[NV];  // 8 halves, or the codes of this lane's keys
+        constexpr int VE = TYPE == FLLM_TYPE_F16 ? 2 : 1;
+        const uint8_t* vp = a.pg.v + cv + (uint32_t)((col * P + pv) * VE);
+#pragma unroll
+        for (int d = 0; d < NV; d++)
+            vf[d] = *(const uv*)(vp + (uint32_t)((d < (TYPE == FLLM_TYPE_Q4_0 ? nb : 2 * nb) ? d : 0) * 16 * P * VE));
+
+        const bool edge = k0 < all_lo || k0 + STEP > all_hi;
+        if (edge) {
+            // what lies outside the sequence may be anything: no scale and no half of it may be a NaN
+            for (int i = 0; i < RUN; i++) {
+                const bool in = kv + i >= any_lo && kv + i < it.len;
+                if (QUANT) {
+                    const uint32_t keep = in ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+                    for (int c = 0; c < NB; c++) vs[c][i >> 3][(i & 7) >> 1] &= keep;
+                } else {
+                    const uint32_t keep = in ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+#pragma unroll
+                    for (int d = 0; d < NV; d++) vf[d][i >> 1] &= keep;
+                }
+            }
+        }
+        if (QUANT) {  // the units of o: the largest scale so far
+            h2 top = {(_Float16)0, (_Float16)0};
+            for (int c = 0; c < NB; c++)
+                    for (int i = 0; i < 4 * JN; i++) {
+                        union { uint32_t u; h2 h; } s;
+                        s.u = vs[c][i >> 2][i & 3] & 0x7FFF7FFFu;
+                        top = __builtin_elementwise_max(top, s.h);
+                    }
+            float f = fmaxf((float)top.x, (float)top.y);
+            f = fmaxf(f, __shfl_xor(f, 16));
+            f = fmaxf(f, __shfl_xor(f, 32));
+            const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(f) >> 23) - 126);  // f < 2^e
+            if (e > vexp) {
+                const float down = ldexpf(1.0f, vexp - e);
+                for (int m = 0; m < TM; m++)
+                    for (int d = 0; d < ND; d++) o[m][d] *= down;
+                vexp = e;
+            }
+        }
+        const float vunit = ldexpf(1.0f, QUANT ? 14 - vexp : 14);
+
+#pragma unroll
+        for (int m = 0; m < TM; m++) {
+            float s[RUN];
+#pragma unroll
+            for (int t = 0; t < 2 * JN; t++) {
+                f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NB; c++) {
+                    const h8 kh = kf[t][c].half();
+                    if (QUANT) {
+                        f4 b = {0.f, 0.f, 0.f, 0.f};
+                        for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, c, n), b, 0, 0, 0);
+                        for (int e = 0; e < 4; e++) {
+                            union { uint32_t u; h2 h; } d;
+                            d.u = ks[c][t >> 1][2 * (t & 1) + (e >> 1)];
+                            acc[e] = fmaf(b[e], (float)(e & 1 ? d.h.y : d.h.x), acc[e]);
+                        }
+                    } else {
+                        for (int n = NP - 1; n >= 0; n--) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, c, n), acc, 0, 0, 0);
+                    }
+                }
+                for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e] * unscale[m];
+            }
+            if (a.softcap > 0.0f)
+                for (int i = 0; i < RUN; i++) s[i] = cap * tanh_of(s[i]);
+            if (edge)
+                for (int i = 0; i < RUN; i++)
+                    if (kv + i > pos[m] || (int64_t)kv + i <= (int64_t)pos[m] - a.window) s[i] = -INFINITY;
+            float top = s[0];
+            for (int i = 1; i < RUN; i++) top = fmaxf(top, s[i]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float nm = fmaxf(mx[m], top);
+            const float down = __builtin_amdgcn_exp2f(mx[m] - nm);
+            mx[m] = nm;
+            float l = 0.0f;
+            for (int i = 0; i < RUN; i++) {
+                s[i] = __builtin_amdgcn_exp2f(s[i] - nm);
+                l += s[i];
+            }
+            sum[m] = sum[m] * down + l;
+            if (__any(down != 1.0f))  // the maximum seldom grows after the first steps
+                for (int d = 0; d < ND; d++) o[m][d] *= down;
+
+            if (!QUANT) {
+                float w[8];
+                for (int i = 0; i < 8; i++) w[i] = s[i] * vunit;
+                h8 wf[NP];
+                split8<NP>(w, wf);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    H8 v;
+                    for (int i = 0; i < 4; i++) v.u[i] = vf[d][i];
+                    for (int n = NP - 1; n >= 0; n--) o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[n], o[m][d], 0, 0, 0);
+                }
+            } else {
+                for (int i = 0; i < RUN; i++) s[i] *= vunit;
+#pragma unroll
+                for (int c = 0; c < NB; c++) {
+                    h8 wf[JN][NP];
+                    for (int j = 0; j < JN; j++) {
+                        float w[8];
+                        for (int i = 0; i < 8; i++) {
+                            union { uint32_t u; h2 h; } d;
+                            d.u = vs[c][j][i >> 1];
+                            w[i] = fmaf((float)(i & 1 ? d.h.y : d.h.x), s[8 * j + i], 0.0f);
+                        }
+                        split8<NP>(w, wf[j]);
+                    }
+                    for (int h = 0; h < 2; h++)
+                        for (int j = 0; j < JN; j++) {
+                            H8 v;
+                            if (TYPE == FLLM_TYPE_Q8_0) {
+                                bytes_to_half<1152>(vf[TYPE == FLLM_TYPE_Q4_0 ? 0 : 2 * c + h][2 * j] ^ 0x80808080u, v.u);
+                                bytes_to_half<1152>(vf[TYPE == FLLM_TYPE_Q4_0 ? 0 : 2 * c + h][2 * j + 1] ^ 0x80808080u, v.u + 2);
+                            } else {
+                                bytes_to_half<1032>(vf[c][2 * j] >> 4 * h & 0x0F0F0F0Fu, v.u);
+                                bytes_to_half<1032>(vf[c][2 * j + 1] >> 4 * h & 0x0F0F0F0Fu, v.u + 2);
+                            }
+                            for (int n = NP - 1; n >= 0; n--)
+                                o[m][2 * c + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[j][n], o[m][2 * c + h], 0, 0, 0);
+                        }
+                }
+            }
+        }
+    }
+
+    // the four waves' results, a row tile at a time
+    const float unit = ldexpf(1.0f, QUANT ? vexp - 14 : -14);
+    // the tile's partial rows under this kv head: [split][row]
+    const int64_t part0 = (int64_t)it.part * a.pg.nkv + (int64_t)kvh * it.nsplit * it.nrows;
+    const uint32_t n_part = (uint32_t)(it.nsplit * it.nrows);
+    const __amdgpu_buffer_rsrc_t ro = wt_rsrc(a.part_o + part0 * hd, n_part * hd * 4);
+    const __amdgpu_buffer_rsrc_t rml = wt_rsrc(a.part_ml + 2 * part0, n_part * 8);
+#pragma unroll
+    for (int m = 0; m < TM; m++) {
+        sum[m] += __shfl_xor(sum[m], 16);
+        sum[m] += __shfl_xor(sum[m], 32);
+        __syncthreads();  // q, or the tile before, is done with
+        if (g == 0) {
+            s_m[wave][col] = mx[m];
+            s_l[wave][col] = sum[m];
+        }
+        for (int d = 0; d < ND; d++) *(f4*)&sm.o[wave][col][16 * d + 4 * g] = o[m][d] * unit;
+        __syncthreads();
+        for (int u = threadIdx.x; u < 16 * (HDP / 4); u += 256) {
+            const int r = u / (HDP / 4), d = u % (HDP / 4) * 4, row = 16 * m + r;
+            if (row >= it.nrows || d >= hd) continue;
+            const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+            f4 acc = {0.f, 0.f, 0.f, 0.f};
+            float l = 0.0f;
+            for (int w = 0; w < 4; w++) {
+                const float f = __builtin_amdgcn_exp2f(s_m[w][r] - top);
+                l += f * s_l[w][r];
+                acc += f * *(const f4*)&sm.o[w][r][d];
+            }
+            if (it.nsplit == 1) {
+                const int tr = it.row0 + row, tok = tr / a.group, head = kvh * a.group + tr % a.group;
+                const int64_t at = (int64_t)(it.tok0 + tok) * a.out.ld + (int64_t)head * hd + d;
+                const float inv = 1.0f / l;
+                store_row4(a.out, at, acc * inv);
+            } else {
+                const uint32_t pr = (uint32_t)(it.split * it.nrows + row);
+                __builtin_amdgcn_raw_buffer_store_b128(acc, ro, (pr * hd + d) * 4, 0, CPOL_SC1);
+                if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(f2{top, l}, rml, pr * 8, 0, CPOL_SC1);
+            }
+        }
+    }
+    if (it.nsplit == 1) return;
+
+    if (!last_of_tile(a.cnt + part0, it.nsplit, &s_last)) return;
+    join_parts<kAttnSplit[0]>(a, it, kvh, ro, rml, sm.w);
+}
+
+// ---- many rows -----------------------------------------------------------------------------
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+
+constexpr int kManyRows = kAttnTile[2], kManySplit = kAttnSplit[2];
+
+// LDS planes of a step: K [keys][HDP], V [HDP][keys], halves in chunks of 8. Chunk c of a row lies at
+// c ^ swizzle(row), so that the 16 rows that a quarter of a wave reads cover the banks once.
+template <int HDP>
+__device__ __forceinline__ int k_chunk(int key, int c) {
+    return key * (HDP / 8) + (c ^ (HDP == 64 ? key >> 1 & 7 : key & 15));
+}
+template <int STEP>
+__device__ __forceinline__ int v_chunk(int d, int c) {
+    return STEP == 64 ? d * 8 + (c ^ (d >> 1 & 7)) : d * 4 + (c ^ (d >> 2 & 3));
+}
+
+// 8 codes (two words) as fp16 integers; Q4_0: of the low (half 0) or high nibbles
+template <int TYPE>
+__device__ __forceinline__ H8 codes8(uint32_t a, uint32_t b, int half) {
+    H8 r;
+    if (TYPE == FLLM_TYPE_Q8_0) {
+        bytes_to_half<1152>(a ^ 0x80808080u, r.u);
+        bytes_to_half<1152>(b ^ 0x80808080u, r.u + 2);
+    } else {
+        bytes_to_half<1032>(a >> 4 * half & 0x0F0F0F0Fu, r.u);
+        bytes_to_half<1032>(b >> 4 * half & 0x0F0F0F0Fu, r.u + 2);
+    }
+    return r;
+}
+
+// codes times scales (one per element, times 2^s), as halves in planes `gap` chunks apart
+template <int KP>
+__device__ __forceinline__ void scaled_out(const H8& c, const uint32_t* d, int step, float unit, u4* to, int gap) {
+    H8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        union { uint32_t u; h2 h; } s;
+        s.u = d[i * step];
+        if (KP == 1) {
+            const h2 t = s.h * h2{(_Float16)unit, (_Float16)unit};
+            hi.p[i] = c.p[i] * t;
+        } else {
+            const float x = fmaf((float)c.p[i].x, (float)s.h.x * unit, 0.0f), y = fmaf((float)c.p[i].y, (float)s.h.y * unit, 0.0f);
+            union { __fp16 __attribute__((ext_vector_type(2))) c; h2 h; } a, b;
+            a.c = __builtin_amdgcn_cvt_pkrtz(x, y);
+            b.c = __builtin_amdgcn_cvt_pkrtz(fmaf((float)a.h.x, -1.0f, x), fmaf((float)a.h.y, -1.0f, y));
+            hi.p[i] = a.h;
+            lo.p[i] = b.h;
+        }
+    }
+    to[0] = u4{hi.u[0], hi.u[1], hi.u[2], hi.u[3]};
+    if (KP == 2) to[gap] = u4{lo.u[0], lo.u[1], lo.u[2], lo.u[3]};
+}
+
+// keys a step: 64, or 32 where q, o and the codes on their way leave too few registers
+constexpr int many_step(int hdp, int np) { return hdp > 128 || (hdp == 128 && np == 2) ? 32 : 64; }
+
+template <int TYPE, int HDP, int NP>
+__global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgsP a) {
+    constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
+    constexpr int NB = HDP / 32, KS = HDP / 16;
+    constexpr int KP = QUANT ? NP : 1;                       // planes of K and V
+    constexpr int STEP = many_step(HDP, NP), T = STEP / 32;  // keys a step, tiles of 32
+    constexpr int PIECES = STEP / 16;
+    constexpr int KCH = STEP * HDP / 8, VCH = KCH;           // chunks of 8 halves a plane
+    constexpr int KU = (STEP * NB + 255) / 256;              // (key, block) units a thread
+    constexpr int VROWS = TYPE == FLLM_TYPE_Q4_0 ? HDP / 2 : HDP;
+    constexpr int VU = (VROWS * PIECES + 255) / 256;              // (row, 16 keys) units a thread
+    constexpr int KW = TYPE == FLLM_TYPE_F16 ? 4 : TYPE == FLLM_TYPE_Q8_0 ? 2 : 1;  // 16-byte words of a K unit
+    constexpr int VW = TYPE == FLLM_TYPE_F16 ? 2 : 1;                               // of a V unit
+    __shared__ union {
+        struct {
+            u4 k[KP * KCH], v[KP * VCH];
+        } t;
+        float w[kManySplit * kManyRows];
+    } sm;
+    __shared__ int s_last;
+
+    const int kvh = blockIdx.x % a.pg.nkv;
+    const AttnItem it = a.items[blockIdx.x / a.pg.nkv];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, h = lane >> 5;
+    const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
+    const int* table = a.tables + it.table;
+    const int last_block = (it.len - 1) >> lp;
+
+    // this lane's query
+    const int r = 32 * wave + col;
+    const bool live = r < it.nrows;
+    const int qrow = it.row0 + (live ? r : 0), qtok = qrow / a.group, head = kvh * a.group + qrow % a.group;
+    const int pos = live ? it.pos0 + qtok : -1;
+    float unscale;
+    h8 q[KS][NP];
+    {
+        const int64_t at = (int64_t)(it.tok0 + qtok) * a.q.ld + (int64_t)head * hd;
+        float x[KS][8], top = 0.0f;
+        if (a.q.type == FLLM_TYPE_F32) {
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int d = 16 * k + 8 * h;
+                const float* p = (const float*)a.q.p + at + (d < hd ? d : 0);
+                const f4 u = *(const f4*)p, v = *(const f4*)(p + 4);
+                for (int i = 0; i < 4; i++) x[k][i] = u[i], x[k][4 + i] = v[i];
+            }
+        } else {
+            const bool f16 = a.q.type == FLLM_TYPE_F16;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const int d = 16 * k + 8 * h;
+                const u4 u = *(const u4*)(a.q.p + 2 * (at + (d < hd ? d : 0)));
+                for (int i = 0; i < 4; i++) {
+                    union { uint32_t u; h2 h; } c;
+                    c.u = u[i];
+                    x[k][2 * i] = f16 ? (float)c.h.x : __uint_as_float(u[i] << 16);
+                    x[k][2 * i + 1] = f16 ? (float)c.h.y : __uint_as_float(u[i] & 0xFFFF0000u);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+            for (int i = 0; i < 8; i++) {
+                if (!live || 16 * k + 8 * h >= hd) x[k][i] = 0.0f;
+                top = fmaxf(top, fabsf(x[k][i]));
+            }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int e = row_exponent(top);
+        const float up = ldexpf(1.0f, e);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            for (int i = 0; i < 8; i++) x[k][i] *= up;
+            split8<NP>(x[k], q[k]);
+        }
+        unscale = ldexpf(a.scale, -e) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+    }
+    const float cap = a.softcap * kLog2e;
+
+    f16v o[HDP / 32];
+    for (int d = 0; d < HDP / 32; d++)
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float mx = kNoScore, sum = 0.0f;
+    int vexp = -30;
+    // keys that every row of the wave, any row of it and any row of the tile sees
+    const int w0 = it.row0 + min(32 * wave, it.nrows - 1), w1 = it.row0 + min(32 * wave + 31, it.nrows - 1);
+    const int64_t all_hi = it.pos0 + w0 / a.group + 1, all_lo = (int64_t)it.pos0 + w1 / a.group - a.window + 1;
+    const int64_t any_hi = 32 * wave < it.nrows ? it.pos0 + w1 / a.group + 1 : 0, any_lo = all_hi - a.window;
+    const int64_t tile_lo = (int64_t)it.pos0 + it.row0 / a.group + 1 - a.window;
+
+    // ---- a step's codes and scales on their way to LDS
+    u4 kr[KU][KW], vr[VU][VW], ks, vs;
+    uint32_t kd[KU];             // K: the unit's scale
+    u4 vd[QUANT ? VU : 1][2];    // V: 16 keys' scales
+    int pk, pv[VU], ps;          // pages of the next step
+    const auto pages_at = [&](int k0) {
+        pk = table[min((k0 + (tid % STEP)) >> lp, last_block)];
+        for (int i = 0; i < VU; i++) pv[i] = table[min((k0 + 16 * ((tid + 256 * i) / VROWS & (PIECES - 1))) >> lp, last_block)];
+        if (QUANT) ps = table[min((k0 + 8 * (lane & (STEP / 8 - 1))) >> lp, last_block)];
+    };
+    const auto cell = [&](int page) { return ((uint64_t)(uint32_t)page * a.pg.nkv + kvh) * a.pg.cell; };
+    const auto load = [&](int k0) {
+        constexpr int KB = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;
+        const int key = k0 + (tid % STEP);
+        const uint8_t* kc = a.pg.k + cell(pk);
+#pragma unroll
+        for (int i = 0; i < KU; i++) {
+            const int blk = tid / STEP + 256 / STEP * i, at = (blk < nb ? blk : 0) * P + (key & (P - 1));
+            for (int w = 0; w < KW; w++) kr[i][w] = *(const u4*)(kc + (uint32_t)(at * KB + 16 * w));
+            if (QUANT) kd[i] = *(const uint16_t*)(kc + a.pg.scale_off + (uint32_t)(2 * at));
+        }
+#pragma unroll
+        for (int i = 0; i < VU; i++) {
+            const int u = tid + 256 * i, row = u % VROWS, key16 = k0 + 16 * (u / VROWS & (PIECES - 1));
+            const int rows = TYPE == FLLM_TYPE_Q4_0 ? hd / 2 : hd;
+            const uint8_t* vc = a.pg.v + cell(pv[i]);
+            const int at = (row < rows ? row : 0) * P + (key16 & (P - 1));
+            for (int w = 0; w < VW; w++) vr[i][w] = *(const u4*)(vc + (uint32_t)(at * (TYPE == FLLM_TYPE_F16 ? 2 : 1) + 16 * w));
+            if (QUANT) {
+                const int blk = TYPE == FLLM_TYPE_Q4_0 ? row >> 4 : row >> 5;
+                const uint8_t* sc = vc + a.pg.scale_off + (uint32_t)(2 * ((blk < nb ? blk : 0) * P + (key16 & (P - 1))));
+                vd[i][0] = *(const u4*)sc;
+                vd[i][1] = *(const u4*)(sc + 16);
+            }
+        }
+        if (QUANT) {
+            const int blk = lane / (STEP / 8), at = 2 * ((blk < nb ? blk : 0) * P + ((k0 + 8 * (lane & (STEP / 8 - 1))) & (P - 1)));
+            ks = *(const u4*)(a.pg.k + cell(ps) + a.pg.scale_off + (uint32_t)at);
+            vs = *(const u4*)(a.pg.v + cell(ps) + a.pg.scale_off + (uint32_t)at);
+        }
+    };
+    // s with largest scale * 2^s * 127 < 2^15, over the keys of the step that the sequence has
+    const auto top_scale = [&](u4 s, int k0) {
+        us2 top = {0, 0};
+        for (int i = 0; i < 4; i++) {
+            union { uint32_t u; us2 h; } c;
+            c.u = s[i] & 0x7FFF7FFFu;
+            const int64_t key = k0 + 8 * (lane & (STEP / 8 - 1)) + 2 * i;
+            if (key < tile_lo || key >= it.len) c.h.x = 0;
+            if (key + 1 < tile_lo || key + 1 >= it.len) c.h.y = 0;
+            top = __builtin_elementwise_max(top, c.h);
+        }
+        float m = (float)max((int)top.x, (int)top.y);
+        m = wave_max(m);
+        return ((int)m >> 10) - 14;  // every scale < 2^this
+    };
+
+    pages_at(it.k0);
+    load(it.k0);
+    if (it.k0 + STEP < it.k1) pages_at(it.k0 + STEP);
+    for (int k0 = it.k0; k0 < it.k1; k0 += STEP) {
+        float kunit = 1.0f, vunit = 1.0f;  // what the planes' values are multiplied by
+        if (QUANT) {
+            const int ek = __builtin_amdgcn_readfirstlane(top_scale(ks, k0)), ev = __builtin_amdgcn_readfirstlane(top_scale(vs, k0));
+            kunit = ldexpf(1.0f, min(8 - ek, 15));
+            if (ev > vexp) {  // o is in units of the largest V scale so far
+                const float down = ldexpf(1.0f, max(vexp, -7) - max(ev, -7));
+                for (int d = 0; d < HDP / 32; d++) o[d] *= down;
+                vexp = ev;
+            }
+            vunit = ldexpf(1.0f, min(8 - vexp, 15));
+        }
+        if (k0 != it.k0) __syncthreads();  // the step before is read
+#pragma unroll
+        for (int i = 0; i < KU; i++) {
+            const int key = tid % STEP, blk = tid / STEP + 256 / STEP * i;
+            if (STEP * NB % 256 && blk >= NB) continue;
+            if (!QUANT) {
+                for (int w = 0; w < KW; w++) sm.t.k[k_chunk<HDP>(key, 4 * blk + w)] = kr[i][w];
+            } else {
+                const uint32_t d = kd[i] | kd[i] << 16;
+                for (int c = 0; c < 4; c++) {
+                    const H8 x = TYPE == FLLM_TYPE_Q8_0 ? codes8<TYPE>(kr[i][c >> 1 & (KW - 1)][2 * (c & 1)], kr[i][c >> 1 & (KW - 1)][2 * (c & 1) + 1], 0)
+                                                        : codes8<TYPE>(kr[i][0][2 * (c & 1)], kr[i][0][2 * (c & 1) + 1], c >> 1);
+                    scaled_out<KP>(x, &d, 0, kunit, &sm.t.k[k_chunk<HDP>(key, 4 * blk + c)], KCH);
+                }
+            }
+        }
+        const bool outside = k0 < tile_lo || k0 + STEP > it.len;
+#pragma unroll
+        for (int i = 0; i < VU; i++) {
+            const int u = tid + 256 * i, row = u % VROWS, piece = u / VROWS;
+            if (VROWS * PIECES % 256 && piece >= PIECES) continue;
+            if (outside)  // what lies outside the sequence may be anything: zeros instead
+                for (int j = 0; j < 16; j++) {
+                    const int64_t key = k0 + 16 * piece + j;
+                    const uint32_t keep = key >= tile_lo && key < it.len ? 0xFFFFFFFFu : j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                    if (QUANT) vd[i][j >> 3][(j & 7) >> 1] &= keep;
+                    else vr[i][j >> 3 & (VW - 1)][(j & 7) >> 1] &= keep;
+                }
+            if (!QUANT) {
+                for (int w = 0; w < VW; w++) sm.t.v[v_chunk<STEP>(row, 2 * piece + w)] = vr[i][w];
+            } else {
+                for (int c = 0; c < 2; c++) {
+                    const uint32_t d[4] = {vd[i][c].x, vd[i][c].y, vd[i][c].z, vd[i][c].w};
+                    if (TYPE == FLLM_TYPE_Q8_0) {
+                        scaled_out<KP>(codes8<TYPE>(vr[i][0][2 * c], vr[i][0][2 * c + 1], 0), d, 1, vunit, &sm.t.v[v_chunk<STEP>(row, 2 * piece + c)], VCH);
+                    } else {
+                        const int at = (row >> 4) * 32 + (row & 15);
+                        for (int n = 0; n < 2; n++)
+                            scaled_out<KP>(codes8<TYPE>(vr[i][0][2 * c], vr[i][0][2 * c + 1], n), d, 1, vunit, &sm.t.v[v_chunk<STEP>(at + 16 * n, 2 * piece + c)], VCH);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        if (k0 + STEP < it.k1) {
+            load(k0 + STEP);
+            if (k0 + 2 * STEP < it.k1) pages_at(k0 + 2 * STEP);
+        }
+        if (k0 >= any_hi || k0 + STEP <= any_lo) continue;  // no row of this wave sees the step
+
+        // S^T = K Q^T: row rho of a 32-key tile is the key with bits 2 and 3 of rho swapped, so that a lane's 8
+        // registers 8 s .. are the consecutive keys 16 s + 8 h ..: the second product's operand
+        f16v s[T];
+        const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                union { u4 u; h8 h; } kf[KP];
+                for (int p = 0; p < KP; p++) kf[p].u = sm.t.k[p * KCH + k_chunk<HDP>(32 * t + krow, 2 * k + h)];
+                if (KP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[KP - 1].h, q[k][0], s[t], 0, 0, 0);
+                if (NP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0].h, q[k][NP - 1], s[t], 0, 0, 0);
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0].h, q[k][0], s[t], 0, 0, 0);
+            }
+        }
+        const float us = unscale / kunit;
+        const bool edge = k0 < all_lo || k0 + STEP > all_hi;
+        float top = kNoScore;
+#pragma unroll
+        for (int t = 0; t < T; t++)
+            for (int i = 0; i < 16; i++) {
+                s[t][i] *= us;
+                if (a.softcap > 0.0f) s[t][i] = cap * tanh_of(s[t][i]);
+                if (edge) {
+                    const int key = k0 + 32 * t + 16 * (i >> 3) + 8 * h + (i & 7);
+                    if (key > pos || (int64_t)key <= (int64_t)pos - a.window) s[t][i] = -INFINITY;
+                }
+                top = fmaxf(top, s[t][i]);
+            }
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float nm = fmaxf(mx, top), down = __builtin_amdgcn_exp2f(mx - nm);
+        mx = nm;
+        float l = 0.0f;
+#pragma unroll
+        for (int t = 0; t < T; t++)
+            for (int i = 0; i < 16; i++) {
+                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - nm);
+                l += s[t][i];
+            }
+        sum = sum * down + l;
+        if (__any(down != 1.0f))
+            for (int d = 0; d < HDP / 32; d++) o[d] *= down;
+
+        // O^T += V^T P^T
+#pragma unroll
+        for (int k = 0; k < 2 * T; k++) {
+            float w[8];
+            for (int i = 0; i < 8; i++) w[i] = s[k >> 1][8 * (k & 1) + i] * (NP == 2 ? 16384.0f : 1.0f);
+            h8 wf[NP];
+            split8<NP>(w, wf);
+#pragma unroll
+            for (int d = 0; d < HDP / 32; d++) {
+                union { u4 u; h8 h; } vf[KP];
+                for (int p = 0; p < KP; p++) vf[p].u = sm.t.v[p * VCH + v_chunk<STEP>(32 * d + col, 2 * k + h)];
+                if (KP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[KP - 1].h, wf[0], o[d], 0, 0, 0);
+                if (NP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0].h, wf[NP - 1], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0].h, wf[0], o[d], 0, 0, 0);
+            }
+        }
+    }
+
+    // results: o in units of 2^-(its scaling)
+    sum += __shfl_xor(sum, 32);
+    const float unit = ldexpf(1.0f, (QUANT ? -min(8 - vexp, 15) : 0) - (NP == 2 ? 14 : 0));
+    if (it.nsplit == 1) {
+        const float inv = unit / sum;
+        const int64_t at = (int64_t)(it.tok0 + qtok) * a.out.ld + (int64_t)head * hd;
+        if (live)
+#pragma unroll
+            for (int d = 0; d < HDP / 32; d++)
+                for (int b = 0; b < 4; b++)
+                    if (32 * d < hd) store_row4(a.out, at + 32 * d + 8 * b + 4 * h, f4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]} * inv);
+        return;
+    }
+    const int64_t part0 = (int64_t)it.part * a.pg.nkv + (int64_t)kvh * it.nsplit * it.nrows;
+    const uint32_t n_part = (uint32_t)(it.nsplit * it.nrows);
+    const __amdgpu_buffer_rsrc_t ro = wt_rsrc(a.part_o + part0 * hd, n_part * hd * 4);
+    const __amdgpu_buffer_rsrc_t rml = wt_rsrc(a.part_ml + 2 * part0, n_part * 8);
+    if (live) {
+        const uint32_t pr = (uint32_t)(it.split * it.nrows + r);
+#pragma unroll
+        for (int d = 0; d < HDP / 32; d++)
+            for (int b = 0; b < 4; b++)
+                if (32 * d < hd)
+                    __builtin_amdgcn_raw_buffer_store_b128(f4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]} * unit, ro,
+                                                           (pr * hd + 32 * d + 8 * b + 4 * h) * 4, 0, CPOL_SC1);
+        if (h == 0) __builtin_amdgcn_raw_buffer_store_b64(f2{mx, sum}, rml, pr * 8, 0, CPOL_SC1);
+    }
+    if (!last_of_tile(a.cnt + part0, it.nsplit, &s_last)) return;
+    join_parts<kManySplit>(a, it, kvh, ro, rml, sm.w);
+}
+
+inline AttnArgsP attend_args(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q, const RowsView& out,
+                             float scale, float softcap) {
+    return AttnArgsP{pg, b.tables, nullptr, b.n_heads / pg.nkv, b.window, q, out, scale, softcap,
+                     w.part, w.part + w.part_rows * pg.nkv * pg.hd, w.cnt};
+}
+
+template <int TYPE, int HDP, int NP>
+hipError_t launch_items(AttnArgsP a, const AttnWork& w, hipStream_t st) {
+    for (int c = 2; c >= 0; c--) {
+        if (w.n[c] == 0) continue;
+        a.items = w.items[c];
+        const dim3 grid((unsigned)w.n[c] * (unsigned)a.pg.nkv);
+        if (c == 0) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1>), grid, dim3(256), 0, st, a);
+        else if (c == 1) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP>), grid, dim3(256), 0, st, a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+template <int TYPE, int NP>
+hipError_t launch_items_hd(const AttnArgsP& a, const AttnWork& w, hipStream_t st) {
+    if (a.pg.hd <= 64) return launch_items<TYPE, 64, NP>(a, w, st);
+    if (a.pg.hd <= 128) return launch_items<TYPE, 128, NP>(a, w, st);
+    return launch_items<TYPE, 256, NP>(a, w, st);
+}
+
+template <int TYPE>
+hipError_t launch_items_of(const AttnArgsP& a, const AttnWork& w, hipStream_t st) {
+    // 16-bit rows: 11-bit factors lose less than their outputs' rounding
+    return a.q.type == FLLM_TYPE_F32 || a.out.type == FLLM_TYPE_F32 ? launch_items_hd<TYPE, 2>(a, w, st)
+                                                                    : launch_items_hd<TYPE, 1>(a, w, st);
+}
+
+}  // namespace
+}  // namespace fllm

@@ -175,17 +175,19 @@ struct AttnItem {
     int pad[4];
 };
 constexpr int kKeyStep = 64;
-constexpr int kAttnMaxSplit = 128;  // items of a tile
+constexpr int kAttnTile[3] = {16, 32, 128};
+constexpr int kAttnSplit[3] = {128, 128, 32};  // most items of a tile
 
 struct AttnPlan {
-    std::vector<AttnItem> items[2];  // tiles of up to 16 rows, of up to 32
+    std::vector<AttnItem> items[3];  // tiles of up to kAttnTile[c] rows
     int64_t part_rows = 0;           // partial rows per kv head
 };
 
-// Items of the tiles of `tile` rows of sequence i, each of at most `steps` steps of keys.
-inline void attn_items(const SeqPlan& s, int i, int table, int group, int window, int tile, int64_t steps,
+// Items of the tiles of class c of sequence i, each of at most `steps` steps of keys where the splits allow it.
+inline void attn_items(const SeqPlan& s, int i, int table, int group, int window, int c, int64_t steps,
                        std::vector<AttnItem>* out, int64_t* part_rows) {
     const int64_t rows = (int64_t)s.n_new * group;
+    const int tile = kAttnTile[c];
     for (int64_t r = 0; r < rows; r += tile) {
         const int n = (int)std::min<int64_t>(tile, rows - r);
         const int pos0 = s.len - s.n_new;
@@ -193,7 +195,7 @@ inline void attn_items(const SeqPlan& s, int i, int table, int group, int window
         const int g0 = low > 0 ? (int)(low / kKeyStep) : 0;
         const int last = pos0 + (int)((r + n - 1) / group);
         const int g1 = last / kKeyStep + 1;
-        const int nsplit = (int)std::min<int64_t>(kAttnMaxSplit, (g1 - g0 + steps - 1) / steps), per = (g1 - g0 + nsplit - 1) / nsplit;
+        const int nsplit = (int)std::min<int64_t>(kAttnSplit[c], (g1 - g0 + steps - 1) / steps), per = (g1 - g0 + nsplit - 1) / nsplit;
         const int used = (g1 - g0 + per - 1) / per;
         for (int k = 0; k < used; k++)
             out->push_back({i, (int)r, n, (g0 + k * per) * kKeyStep, std::min((g0 + (k + 1) * per) * kKeyStep, last + 1),
@@ -202,40 +204,66 @@ inline void attn_items(const SeqPlan& s, int i, int table, int group, int window
     }
 }
 
-// Items under one kv head that a sequence's tiles of `tile` rows become with at most `steps` steps of keys each.
-inline int64_t attn_count(const SeqPlan& s, int group, int window, int tile, int64_t steps) {
-    int64_t sum = 0;
+struct AttnCount {
+    int64_t items = 0, steps = 0, longest = 0;
+};
+// What a sequence's tiles of class c become under one kv head with at most `steps` steps of keys an item.
+inline void attn_count(const SeqPlan& s, int group, int window, int c, int64_t steps, AttnCount* n) {
     const int64_t rows = (int64_t)s.n_new * group;
-    for (int64_t r = 0; r < rows; r += tile) {
+    for (int64_t r = 0; r < rows; r += kAttnTile[c]) {
         const int64_t low = (int64_t)s.len - s.n_new + r / group - window + 1;
-        const int64_t last = (int64_t)s.len - s.n_new + (std::min<int64_t>(rows, r + tile) - 1) / group;
-        sum += std::min<int64_t>(kAttnMaxSplit, (last / kKeyStep + 1 - (low > 0 ? low / kKeyStep : 0) + steps - 1) / steps);
+        const int64_t last = (int64_t)s.len - s.n_new + (std::min<int64_t>(rows, r + kAttnTile[c]) - 1) / group;
+        const int64_t all = last / kKeyStep + 1 - (low > 0 ? low / kKeyStep : 0);
+        const int64_t k = std::min<int64_t>(kAttnSplit[c], (all + steps - 1) / steps);
+        n->items += k;
+        n->steps += all;
+        n->longest = std::max(n->longest, (all + k - 1) / k);
     }
-    return sum;
 }
 
 // The items of a batch on a device of n_cu CUs. False where they or their partial rows are too many.
 inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, int window, int n_cu, AttnPlan* p) {
     const int group = n_heads / n_kv;
     p->part_rows = 0;
-    const auto tile_of = [&](const SeqPlan& s) { return (int64_t)s.n_new * group <= 16 ? 16 : 32; };
-    // Two workgroups are resident on a CU, one of heads wider than 128: the shortest items whose workgroups all
-    // start at once (a key step for each of the four waves at least), so that the longest one is as short as it
-    // can be.
+    const auto class_of = [&](const SeqPlan& s) {
+        const int64_t rows = (int64_t)s.n_new * group;
+        return rows <= kAttnTile[0] ? 0 : rows <= kAttnTile[1] ? 1 : 2;
+    };
+    // two workgroups are resident on a CU, one of heads wider than 128
     const int64_t slots = (head_dim > 128 ? 1 : 2) * (int64_t)n_cu;
-    int64_t lo = 4, hi = kPagesMaxLength / kKeyStep + 1;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) / 2;
-        int64_t n = 0;
-        for (const SeqPlan& s : b.seqs) n += attn_count(s, group, window, tile_of(s), mid);
-        if (n * n_kv <= slots) hi = mid;
-        else lo = mid + 1;
+    // Few rows: the shortest items whose workgroups all start at once (a key step for each of the four waves at
+    // least), so that the longest one is as short as it can be.
+    int64_t few = 4, hi = kPagesMaxLength / kKeyStep + 1;
+    while (few < hi) {
+        const int64_t mid = (few + hi) / 2;
+        AttnCount n;
+        for (const SeqPlan& s : b.seqs)
+            if (class_of(s) < 2) attn_count(s, group, window, class_of(s), mid, &n);
+        if (n.items * n_kv <= slots) hi = mid;
+        else few = mid + 1;
     }
-    for (int c = 0; c < 2; c++) p->items[c].clear();
+    // Many rows: tiles whole, or cut where that ends sooner. Longest first, a grid of more items than slots ends
+    // about half a longest item after the mean; a part of a tile costs about 3 steps more (its partial rows).
+    const auto ends = [&](int64_t steps, AttnCount* n) {
+        for (const SeqPlan& s : b.seqs)
+            if (class_of(s) == 2) attn_count(s, group, window, 2, steps, n);
+        return n->items * n_kv <= slots ? (double)n->longest
+                                        : (double)(n->steps + 3 * n->items) * n_kv / (double)slots + 0.5 * (double)n->longest;
+    };
+    AttnCount whole;
+    int64_t many = hi = kPagesMaxLength / kKeyStep + 1;
+    double best = ends(many, &whole);
+    for (int k = 1; k <= 3 && whole.items; k++) {
+        const int64_t steps = std::max<int64_t>(4, whole.steps * n_kv / (slots * k) + 1);
+        AttnCount n;
+        const double t = ends(steps, &n) + 3.0;
+        if (t < 0.95 * best) best = t, many = steps;
+    }
+    for (auto& v : p->items) v.clear();
     for (int i = 0; i < b.n_seqs; i++) {
         const SeqPlan& s = b.seqs[(size_t)i];
-        const int tile = tile_of(s);
-        if (s.n_new) attn_items(s, i, i * b.tab_w, group, window, tile, lo, &p->items[tile == 16 ? 0 : 1], &p->part_rows);
+        const int c = class_of(s);
+        if (s.n_new) attn_items(s, i, i * b.tab_w, group, window, c, c == 2 ? many : few, &p->items[c], &p->part_rows);
         if (p->part_rows > INT32_MAX / n_kv) return false;
     }
     for (auto& v : p->items) {

@@ -12,7 +12,7 @@ import dotnetfoundryllm_amd._native as N
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 NO_WINDOW = 0x7FFFFFFF
-TILE = (16, 32)  # rows of the item classes
+TILE, SPLIT = (16, 32, 128), (128, 128, 32)  # rows of the item classes, most items of a tile
 STEP = 64
 
 
@@ -92,7 +92,7 @@ def check(so, new, length, heads, kv, window):
     for c, list_ in enumerate(items(so)):
         for seq, row0, nrows, k0, k1, part, split, nsplit, tok0, pos0, ln, table in list_[:, :12].tolist():
             assert 0 <= seq < len(new) and 0 <= row0 and 1 <= nrows <= TILE[c] and row0 + nrows <= new[seq] * group
-            assert 0 <= k0 < k1 <= length[seq] and k0 % STEP == 0 and 0 <= split < nsplit <= 128
+            assert 0 <= k0 < k1 <= length[seq] and k0 % STEP == 0 and 0 <= split < nsplit <= SPLIT[c]
             assert k1 % STEP == 0 or split == nsplit - 1
             assert (tok0, pos0, ln, table) == (sum(new[:seq]), length[seq] - new[seq], length[seq], seq * tab_w)
             for r in range(row0, row0 + nrows):
