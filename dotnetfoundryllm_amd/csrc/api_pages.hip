@@ -397,6 +397,7 @@ extern "C" int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d) {
     NOT_NULL(d);
     if (d->n_seqs < 0 || d->n_draft < 0 || d->vocab < 1)
         return fail(FLLM_E_ARG_RANGE, "%d sequences, %d drafted tokens, vocabulary %d", d->n_seqs, d->n_draft, d->vocab);
+    if (d->vocab > kDraftVocab) return fail(FLLM_E_NOT_SUPPORTED, "vocabularies above %d are not supported", kDraftVocab);
     const int64_t n = d->n_seqs, nd = n * d->n_draft, nt = n * ((int64_t)d->n_draft + 1);
     RowsView target{}, draft{};
     int32_t rc;
@@ -428,6 +429,12 @@ extern "C" int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d) {
     v.u_sample = (const float*)d->u_sample->ptr;
     v.out_tokens = (int*)d->out_tokens->ptr;
     v.out_counts = (int*)d->out_counts->ptr;
-    HIP_TRY(launch_draft_verify(v, ctx->stream));
+    int seg = 0;
+    const int n_seg = draft_segments(v.n_seqs, v.vocab, ctx->n_cu, &seg);
+    std::lock_guard<std::mutex> lock(ctx->ws.mu);
+    hipError_t e = workspace_room(ctx, (uint64_t)n * (uint64_t)n_seg * 16, (uint64_t)n);
+    if (e != hipSuccess)
+        return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "draft workspace: %s", hipGetErrorString(e));
+    HIP_TRY(launch_draft_verify(v, seg, n_seg, (double*)ctx->ws.part, ctx->ws.cnt, ctx->stream));
     return FLLM_OK;
 }

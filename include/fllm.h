@@ -472,7 +472,7 @@ typedef struct fllm_draft_desc {
     fllm_buf* out_counts;    /* int32 [n_seqs]: kept tokens */
 } fllm_draft_desc;
 /* Enqueued on the context's stream. Negative sizes, vocab < 1 -> FLLM_E_ARG_RANGE; buffers too small,
- * misaligned rows -> FLLM_E_ARG; other types than F32 -> FLLM_E_NOT_SUPPORTED. */
+ * misaligned rows -> FLLM_E_ARG; other types than F32, vocabularies above 1048576 -> FLLM_E_NOT_SUPPORTED. */
 FLLM_API int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d);
 
 /* ---- per-kernel timing of the decode step ----------------------------------- */

@@ -362,6 +362,7 @@ def run_verify(ctx, target, draft, tokens, counts, ua, us, ld=None, skew=0):
 @pytest.mark.parametrize("n,nd,v,greedy,ld,skew", [
     (1, 4, 128256, False, 0, 0), (3, 1, 1, False, 0, 0), (5, 8, 5, False, 9, 1), (40, 5, 1000, True, 0, 2),
     (7, 3, 4097, False, 4099, 3), (2, 0, 333, False, 0, 0), (130, 2, 64, False, 0, 0), (2, 6, 152064, True, 152065, 1),
+    (1, 1, 1 << 20, False, 0, 0), (12, 1, 70001, False, 0, 1), (1, 70, 40, False, 0, 0), (3, 130, 9, True, 0, 0),
 ])
 def test_draft_verify(ctx, n, nd, v, greedy, ld, skew):
     rng = np.random.default_rng(v + n)
@@ -495,7 +496,7 @@ def test_draft_verify_refuses(ctx):
             (-1, 1, 8, {}, F.ArgumentOutOfRangeException), (1, -1, 8, {}, F.ArgumentOutOfRangeException),
             (1, 1, 0, {}, F.ArgumentOutOfRangeException), (1, 1, 9, {}, F.ArgumentException), (5, 1, 8, {}, F.ArgumentException),
             (1, 1, 8, {"draft": F.Rows(b, 4)}, F.ArgumentException), (1, 1, 8, {"tokens": None}, F.ArgumentNullException),
-            (1, 1, 8, {"target": F.Rows(b, 8, F.F16)}, F.NotSupportedException),
+            (1, 1, 8, {"target": F.Rows(b, 8, F.F16)}, F.NotSupportedException), (1, 1, (1 << 20) + 1, {}, F.NotSupportedException),
             (1, 1, 8, {"target": F.Rows(b, 8, F.F32, 2)}, F.ArgumentException)]:
         with pytest.raises(err):
             F.draft_verify(ctx, n, nd, v, **{**ok, **more})
