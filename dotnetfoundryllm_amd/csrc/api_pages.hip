@@ -219,6 +219,7 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         b->view.new_blocks = pl.new_blocks;
         b->view.all_blocks = pl.all_blocks;
         b->view.n_rows = pl.n_rows;
+        b->view.max_new = pl.max_new;
         b->view.n_heads = b->n_heads;
         b->view.window = b->window;
         for (int i = 0; i < 3; i++) {

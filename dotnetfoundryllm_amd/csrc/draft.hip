@@ -50,19 +50,31 @@ struct Ids16 {
     }
 };
 
+// v + the value that DPP control CTRL moves here in the rows of mask ROWS (elsewhere v + 0)
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp_add(double v) {
+    union { double d; int i[2]; } a, b;
+    a.d = v;
+    b.i[0] = __builtin_amdgcn_update_dpp(0, a.i[0], CTRL, ROWS, 0xF, false);
+    b.i[1] = __builtin_amdgcn_update_dpp(0, a.i[1], CTRL, ROWS, 0xF, false);
+    return v + b.d;
+}
+
 // running sums over the workgroup's 256 threads of N values at once: what lies before this thread's v[k]
 // in before[k], each sum in total[k]
 template <int N>
 __device__ __forceinline__ void scan256(const double v[N], double before[N], double total[N], double (*s_wave)[4]) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double run[N];
-    for (int k = 0; k < N; k++) run[k] = v[k];
-    for (int o = 1; o < 64; o <<= 1)
 #pragma unroll
-        for (int k = 0; k < N; k++) {
-            const double u = __shfl_up(run[k], o);
-            if (lane >= o) run[k] += u;
-        }
+    for (int k = 0; k < N; k++) {
+        run[k] = dpp_add<0x111>(v[k]);  // row_shr 1, 2, 4, 8: running sums of 16 lanes
+        run[k] = dpp_add<0x112>(run[k]);
+        run[k] = dpp_add<0x114>(run[k]);
+        run[k] = dpp_add<0x118>(run[k]);
+        run[k] = dpp_add<DPP_BCAST15, 0xA>(run[k]);
+        run[k] = dpp_add<DPP_BCAST31, 0xC>(run[k]);
+    }
     __syncthreads();
     if (lane == 63)
         for (int k = 0; k < N; k++) s_wave[k][wave] = run[k];
@@ -83,29 +95,29 @@ __global__ __launch_bounds__(256) void k_draft_verify(DraftView d, int seg, int 
     __shared__ double s_wave[4][4], s_want;
     __shared__ int s_seg, s_last, s_found, s_pos, s_id;
     const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-    const int n = d.counts ? min(max(d.counts[s], 0), d.n_draft) : d.n_draft;
+    const int given = d.counts ? d.counts[s] : d.n_draft;
+    const float u_sample = d.u_sample[s];
 
     // the tokens kept, a lane each; every wave finds them by itself
-    int c = n;
-    for (int i0 = 0; i0 < n; i0 += 64) {
+    int c = 0, n = 0;
+    for (int i0 = 0; i0 < d.n_draft; i0 += 64) {
         const int i = i0 + lane;
-        bool no = false;
-        if (i < n) {
+        bool no = true;
+        if (i < d.n_draft) {
             const int t = d.tokens[(int64_t)s * d.n_draft + i];
             const float u = d.u_accept[(int64_t)s * d.n_draft + i];
-            no = t < 0 || t >= d.vocab;
-            if (!no) {
+            if (t >= 0 && t < d.vocab) {
                 const double p = d.target[((int64_t)s * (d.n_draft + 1) + i) * d.target_ld + t];
                 const double q = d.draft ? d.draft[((int64_t)s * d.n_draft + i) * d.draft_ld + t] : 1.0;
                 no = !((double)u * q < p);
             }
         }
-        const unsigned long long b = __ballot(no);
-        if (b) {
-            c = i0 + __builtin_ctzll(b);
-            break;
-        }
+        n = min(max(given, 0), d.n_draft);
+        const unsigned long long b = __ballot(no || i >= n);
+        c = b ? min(i0 + __builtin_ctzll(b), n) : min(i0 + 64, n);
+        if (b || c == n) break;
     }
+    n = min(max(given, 0), d.n_draft);
     Weights w;
     w.t = d.target + ((int64_t)s * (d.n_draft + 1) + c) * d.target_ld;
     w.rest = c < n;
@@ -151,7 +163,7 @@ __global__ __launch_bounds__(256) void k_draft_verify(DraftView d, int seg, int 
     }
     const int kind = w.rest || c == n ? 0 : 1;
     const double own = kind ? mine[1] : mine[0], ahead = kind ? before[1] : before[0];
-    const double want = (double)d.u_sample[s] * (kind ? total[1] : total[0]);
+    const double want = (double)u_sample * (kind ? total[1] : total[0]);
     // the first whose running sum passes `want`; were rounding to leave none, the last positive one
     if (own > 0.0) {
         if (ahead + own > want) atomicMin(&s_seg, tid);

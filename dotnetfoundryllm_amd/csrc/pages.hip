@@ -1,21 +1,24 @@
 // pages.hip — rows into and out of the pages of the paged K/V cache.
 //
-// A workgroup takes the positions of one page that the call covers, for one kv head and one of K and
-// V: up to page_size rows of head_dim. Both kernels are bound by memory traffic for many rows and by the
-// launch for few. K keeps the rows' direction, so its codes go straight to their place, 8 lanes to a
-// block of 32. V is stored with the positions along the row (what the attention's second product
-// reads), so its codes are turned in LDS and leave as runs of positions, 16 bytes at a time where the
-// run covers them.
+// A workgroup takes the positions of one page that the call covers, for one kv head and one of K and V: up to
+// page_size rows of head_dim. Both kernels are bound by memory traffic for many rows and by the launch's chain of
+// loads (lengths, page, rows) for few. On the dense side a lane moves 16 bytes (F32 rows: 4 elements, a wave 1 KiB
+// of consecutive ones). K keeps the rows' direction, so its codes go straight to their place. V lies with the
+// positions along the row (what the attention's second product reads): its codes pass through LDS as [position][row],
+// and a thread turns 4 rows by 16 positions in registers (byte permutes), so that the pages are read and written 16
+// bytes at a time too.
 #include "pages.hpp"
 
 namespace fllm {
 
 namespace {
 
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+
 struct Tile {
-    int off, n;       // first position in the page, number of positions
-    int64_t row;      // their first row in the dense matrix
-    uint64_t cell;    // the cell's offset
+    int off, n;     // first position in the page, number of positions
+    int64_t row;    // their first row in the dense matrix
+    uint64_t cell;  // the cell's offset
 };
 
 // The tile of sequence s that workgroup column bx covers; false where it covers none.
@@ -29,19 +32,8 @@ __device__ __forceinline__ bool tile_of(const PagesView& pg, const BatchView& b,
     t->off = lo - (pb << pg.page_log2);
     t->n = hi - lo;
     t->row = (int64_t)(new_only ? q.x : q.w) + (lo - first);
-    t->cell = ((uint64_t)b.tables[(int64_t)s * b.tab_w + pb] * pg.nkv + head) * pg.cell;
+    t->cell = ((uint64_t)(uint32_t)b.tables[(int64_t)s * b.tab_w + pb] * pg.nkv + head) * pg.cell;
     return true;
-}
-
-__device__ __forceinline__ void load4(const RowsView& r, int64_t i, float x[4]) {
-    if (r.type == FLLM_TYPE_F32) {
-        const float4 f = *(const float4*)(r.p + 4 * i);
-        x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-        return;
-    }
-    const uint2 u = *(const uint2*)(r.p + 2 * i);
-    const uint32_t h[4] = {u.x & 0xFFFFu, u.x >> 16, u.y & 0xFFFFu, u.y >> 16};
-    for (int e = 0; e < 4; e++) x[e] = r.type == FLLM_TYPE_F16 ? half_exact(h[e]) : bf16_exact(h[e]);
 }
 
 __device__ __forceinline__ uint32_t half_bits(float f) {
@@ -50,15 +42,27 @@ __device__ __forceinline__ uint32_t half_bits(float f) {
     __builtin_memcpy(&u, &h, 2);
     return u;
 }
+__device__ __forceinline__ float half_float(uint32_t u) {
+    const uint16_t b = (uint16_t)u;
+    _Float16 h;
+    __builtin_memcpy(&h, &b, 2);
+    return (float)h;
+}
 
-__device__ __forceinline__ void store4(const RowsView& r, int64_t i, const float x[4]) {
+// 8 elements of a row
+__device__ __forceinline__ void load8(const RowsView& r, int64_t i, float x[8]) {
     if (r.type == FLLM_TYPE_F32) {
-        *(float4*)(r.p + 4 * i) = make_float4(x[0], x[1], x[2], x[3]);
+        const float4 a = *(const float4*)(r.p + 4 * i), b = *(const float4*)(r.p + 4 * i + 16);
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+        x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
         return;
     }
-    uint32_t h[4];
-    for (int e = 0; e < 4; e++) h[e] = r.type == FLLM_TYPE_F16 ? half_bits(x[e]) : bf16_round(x[e]);
-    *(uint2*)(r.p + 2 * i) = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    const uint4 u = *(const uint4*)(r.p + 2 * i);
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int e = 0; e < 4; e++) {
+        x[2 * e] = r.type == FLLM_TYPE_F16 ? half_float(w[e] & 0xFFFFu) : __uint_as_float(w[e] << 16);
+        x[2 * e + 1] = r.type == FLLM_TYPE_F16 ? half_float(w[e] >> 16) : __uint_as_float(w[e] & 0xFFFF0000u);
+    }
 }
 
 // The integer nearest to x / d (ties to even), clamped: the rounded product with the reciprocal is at
@@ -68,208 +72,303 @@ __device__ __forceinline__ int code_of(float x, float d, float inv, float half, 
     const float c = fminf(fmaxf(rintf(x * inv), -300.0f), 300.0f);
     const float r = fmaf(-c, d, x);
     const float s = d < 0.0f ? -r : r;  // remainder in units of |d|
+    const bool odd = (int)c & 1;
     float q = c;
-    if (s > half || (s == half && ((int)c & 1))) q += 1.0f;
-    else if (s < -half || (s == -half && ((int)c & 1))) q -= 1.0f;
+    if (s > half || (s == half && odd)) q += 1.0f;
+    else if (s < -half || (s == -half && odd)) q -= 1.0f;
     return (int)fminf(fmaxf(q, (float)lo), (float)hi);
 }
 
-// The scale of a block of 32 over its 8 lanes, 4 elements each: its bits in half precision.
+// within a quad of lanes (DPP): the value of the lane whose number differs in bit 0, in bit 1
+__device__ __forceinline__ uint32_t quad_xor1(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true); }
+__device__ __forceinline__ uint32_t quad_xor2(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true); }
+
+// The scale of a block of 32 over its 4 lanes, 8 elements each: its bits in half precision.
 template <int TYPE>
-__device__ __forceinline__ uint32_t block_scale(const float x[4], int e) {
-    // order by magnitude, then by the lower index; the sign rides in the low bit. A NaN or an infinity
-    // has the largest magnitude bits, so it leads.
-    unsigned long long key = 0;
-    for (int i = 0; i < 4; i++) {
-        const uint32_t u = __float_as_uint(x[i]);
-        const unsigned long long k = (unsigned long long)(u & 0x7FFFFFFFu) << 32 | (unsigned)(31 - (4 * e + i)) << 1 | u >> 31;
-        key = k > key ? k : key;
+__device__ __forceinline__ uint32_t block_scale(const float x[8], int e) {
+    uint32_t top = 0;  // magnitudes compare as integers; a NaN's is above all
+    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(x[i]) & 0x7FFFFFFFu);
+    top = max(top, quad_xor1(top));
+    top = max(top, quad_xor2(top));
+    if (top >= 0x7F800000u) return 0x7E00u;  // not finite: a NaN scale
+    float d;
+    if (TYPE == FLLM_TYPE_Q8_0) {
+        d = __uint_as_float(top) / 127.0f;
+    } else {
+        uint32_t at = ~0u;  // the first element of that magnitude, its sign in the low bit
+        for (int i = 7; i >= 0; i--)
+            if ((__float_as_uint(x[i]) & 0x7FFFFFFFu) == top) at = (uint32_t)(8 * e + i) << 1 | __float_as_uint(x[i]) >> 31;
+        at = min(at, quad_xor1(at));
+        at = min(at, quad_xor2(at));
+        d = __uint_as_float(top) * (at & 1u ? 0.125f : -0.125f);
     }
-    for (int o = 1; o < 8; o <<= 1) {
-        const unsigned long long k = __shfl_xor(key, o);
-        key = k > key ? k : key;
-    }
-    const float m = __uint_as_float((uint32_t)(key >> 32));
-    if (!(m < __uint_as_float(0x7F800000u))) return 0x7E00u;  // not finite: a NaN scale
-    const float d = TYPE == FLLM_TYPE_Q8_0 ? m / 127.0f : m * ((key & 1) ? 0.125f : -0.125f);
     const uint32_t h = half_bits(d);
     return (h & 0x7FFFu) == 0x7C00u ? (h & 0x8000u) | 0x7BFFu : h;
 }
 
+// 4 words of 4 bytes each as their transpose
+__device__ __forceinline__ void turn4(const uint32_t w[4], uint32_t o[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+    const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    o[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+    o[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+    o[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+    o[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+}
+
+// V's rows of a cell (two elements a byte row in Q4_0), bytes of one position in a row
+template <int TYPE> __device__ __host__ constexpr int v_rows(int hd) { return TYPE == FLLM_TYPE_Q4_0 ? hd / 2 : hd; }
+template <int TYPE> __device__ __host__ constexpr int v_bytes() { return TYPE == FLLM_TYPE_F16 ? 2 : 1; }
+template <int TYPE> __device__ __host__ constexpr int lds_pitch(int hd) { return v_rows<TYPE>(hd) * v_bytes<TYPE>() + 16; }
+
 template <int TYPE>
-__global__ __launch_bounds__(256) void k_pages_append(PagesView pg, BatchView b, RowsView rk, RowsView rv) {
-    extern __shared__ __align__(16) uint8_t turned[];
+__global__ __launch_bounds__(256) void k_pages_append(PagesView pg, BatchView b, int nb_log2, RowsView rk, RowsView rv) {
+    extern __shared__ __align__(16) uint8_t turned[];  // V's codes, [position][row]
     const int head = blockIdx.z >> 1, kind = blockIdx.z & 1;
     const int P = 1 << pg.page_log2, nb = pg.hd >> 5;
     const RowsView& src = kind ? rv : rk;
-    constexpr int ESZ = TYPE == FLLM_TYPE_F16 ? 2 : 1;
-    const int pitch = P * ESZ + 16;  // of a V row in LDS
+    const int pitch = lds_pitch<TYPE>(pg.hd);
     for (int s = blockIdx.y; s < b.n_seqs; s += gridDim.y) {
         Tile t;
         if (!tile_of(pg, b, true, s, blockIdx.x, head, &t)) continue;
         uint8_t* cell = (kind ? pg.v : pg.k) + t.cell;
-        const int e = threadIdx.x & 7;
-        for (int u = threadIdx.x >> 3; u < t.n * nb; u += blockDim.x >> 3) {
-            const int i = u % t.n, blk = u / t.n, pos = t.off + i;
-            float x[4];
-            load4(src, (t.row + i) * src.ld + head * pg.hd + blk * 32 + 4 * e, x);
-            uint32_t c[4];
+        const int e = threadIdx.x & 3;
+        for (int u = threadIdx.x >> 2; u < t.n << nb_log2; u += blockDim.x >> 2) {
+            const int i = u >> nb_log2, blk = u & ((1 << nb_log2) - 1), pos = t.off + i;
+            if (blk >= nb) continue;
+            float x[8];
+            load8(src, (t.row + i) * src.ld + head * pg.hd + blk * 32 + 8 * e, x);
+            uint4 c;
             if (TYPE == FLLM_TYPE_F16) {
-                for (int j = 0; j < 4; j++) c[j] = half_bits(x[j]);
+                c = make_uint4(half_bits(x[0]) | half_bits(x[1]) << 16, half_bits(x[2]) | half_bits(x[3]) << 16,
+                               half_bits(x[4]) | half_bits(x[5]) << 16, half_bits(x[6]) | half_bits(x[7]) << 16);
             } else {
                 const uint32_t h = block_scale<TYPE>(x, e);
-                const float d = half_exact(h);
+                const float d = half_float(h);
                 const bool live = d != 0.0f && d == d;
                 const float inv = live ? 1.0f / d : 0.0f, half = 0.5f * fabsf(d);
-                for (int j = 0; j < 4; j++) {
+                uint32_t w[2] = {0, 0};
+                for (int j = 0; j < 8; j++) {
                     const int q = !live ? 0 : TYPE == FLLM_TYPE_Q8_0 ? code_of(x[j], d, inv, half, -127, 127)
                                                                      : code_of(x[j], d, inv, half, -8, 7);
-                    c[j] = TYPE == FLLM_TYPE_Q8_0 ? (uint32_t)q & 0xFFu : (uint32_t)(q + 8);
+                    w[j >> 2] |= (TYPE == FLLM_TYPE_Q8_0 ? (uint32_t)q & 0xFFu : (uint32_t)(q + 8)) << 8 * (j & 3);
                 }
                 if (e == 0) *(uint16_t*)(cell + pg.scale_off + 2 * (blk * P + pos)) = (uint16_t)h;
-            }
-            if (TYPE == FLLM_TYPE_Q4_0) {  // the upper 16 elements' codes join the lower ones' bytes
-                for (int j = 0; j < 4; j++) c[j] |= (uint32_t)__shfl_down(c[j], 4, 8) << 4;
-                if (e >= 4) continue;
-            }
-            if (kind == 0) {
-                if (TYPE == FLLM_TYPE_F16)
-                    *(uint2*)(cell + 2 * ((blk * P + pos) * 32 + 4 * e)) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-                else
-                    *(uint32_t*)(cell + (blk * P + pos) * (TYPE == FLLM_TYPE_Q4_0 ? 16 : 32) + 4 * e) =
-                        c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-            } else {
-                for (int j = 0; j < 4; j++) {
-                    uint8_t* at = turned + (blk * (TYPE == FLLM_TYPE_Q4_0 ? 16 : 32) + 4 * e + j) * pitch + pos * ESZ;
-                    if (TYPE == FLLM_TYPE_F16) *(uint16_t*)at = (uint16_t)c[j];
-                    else *at = (uint8_t)c[j];
+                if (TYPE == FLLM_TYPE_Q4_0) {  // the upper 16 elements' codes join the lower ones' bytes
+                    w[0] |= quad_xor2(w[0]) << 4;
+                    w[1] |= quad_xor2(w[1]) << 4;
+                    if (e >= 2) continue;
                 }
+                c.x = w[0], c.y = w[1];
             }
+            constexpr int PER = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;  // bytes of a block
+            uint8_t* to = kind ? turned + pos * pitch + blk * PER : cell + (blk * P + pos) * PER;
+            if (TYPE == FLLM_TYPE_F16) *(uint4*)(to + 16 * e) = c;
+            else *(uint2*)(to + 8 * e) = make_uint2(c.x, c.y);
         }
         if (kind == 0) continue;
         __syncthreads();
-        const int rows = TYPE == FLLM_TYPE_Q4_0 ? pg.hd / 2 : pg.hd, chunks = P * ESZ / 16, per = 16 / ESZ;
-        for (int u = threadIdx.x; u < rows * chunks; u += blockDim.x) {
-            const int row = u / chunks, c = u % chunks, lo = max(t.off, c * per), hi = min(t.off + t.n, (c + 1) * per);
-            if (lo >= hi) continue;
-            const uint8_t* from = turned + row * pitch;
-            uint8_t* to = cell + row * P * ESZ;
-            if (hi - lo == per) {
-                *(uint4*)(to + c * 16) = *(const uint4*)(from + c * 16);
-            } else {
-                for (int i = lo; i < hi; i++) {
-                    if (TYPE == FLLM_TYPE_F16) ((uint16_t*)to)[i] = ((const uint16_t*)from)[i];
-                    else to[i] = from[i];
+        // 4 rows by 16 bytes of positions a thread
+        constexpr int VB = v_bytes<TYPE>(), RUN = 16 / VB;
+        const int pieces = P / RUN, units = v_rows<TYPE>(pg.hd) / 4 * pieces, lo0 = t.off / RUN;
+        const int held = (t.off + t.n - 1) / RUN - lo0 + 1;  // pieces with new positions
+        for (int u = threadIdx.x; u < units / pieces * held; u += blockDim.x) {
+            const int row = u / held * 4, piece = lo0 + u % held;
+            const uint8_t* from = turned + piece * RUN * pitch + row * VB;
+            uint8_t* to = cell + (row * P + piece * RUN) * VB;
+            if (piece * RUN >= t.off && (piece + 1) * RUN <= t.off + t.n) {
+                uint32_t o[4][4];
+                if (TYPE == FLLM_TYPE_F16) {
+                    for (int j = 0; j < 4; j++) {
+                        const uint2 a = *(const uint2*)(from + 2 * j * pitch), c = *(const uint2*)(from + (2 * j + 1) * pitch);
+                        o[0][j] = __builtin_amdgcn_perm(c.x, a.x, 0x05040100u);
+                        o[1][j] = __builtin_amdgcn_perm(c.x, a.x, 0x07060302u);
+                        o[2][j] = __builtin_amdgcn_perm(c.y, a.y, 0x05040100u);
+                        o[3][j] = __builtin_amdgcn_perm(c.y, a.y, 0x07060302u);
+                    }
+                } else {
+                    for (int j = 0; j < 4; j++) {
+                        uint32_t w[4], q[4];
+                        for (int k = 0; k < 4; k++) w[k] = *(const uint32_t*)(from + (4 * j + k) * pitch);
+                        turn4(w, q);
+                        for (int k = 0; k < 4; k++) o[k][j] = q[k];
+                    }
                 }
+                for (int k = 0; k < 4; k++) *(uint4*)(to + k * P * VB) = make_uint4(o[k][0], o[k][1], o[k][2], o[k][3]);
+            } else {
+                for (int i = max(0, t.off - piece * RUN); i < min(RUN, t.off + t.n - piece * RUN); i++)
+                    for (int k = 0; k < 4; k++) {
+                        if (TYPE == FLLM_TYPE_F16) ((uint16_t*)to)[k * P + i] = *(const uint16_t*)(from + i * pitch + 2 * k);
+                        else to[k * P + i] = from[i * pitch + k];
+                    }
             }
         }
         __syncthreads();
     }
 }
 
-template <int TYPE>
-__global__ __launch_bounds__(256) void k_pages_read(PagesView pg, BatchView b, bool new_only, RowsView rk, RowsView rv) {
+// EL: elements a lane writes, 16 bytes of the dense rows
+template <int TYPE, int EL>
+__global__ __launch_bounds__(256) void k_pages_read(PagesView pg, BatchView b, bool new_only, int el_log2, RowsView rk, RowsView rv) {
     extern __shared__ __align__(16) uint8_t turned[];
     const int head = blockIdx.z >> 1, kind = blockIdx.z & 1;
     const RowsView& dst = kind ? rv : rk;
     if (!dst.p) return;
-    const int P = 1 << pg.page_log2, nb = pg.hd >> 5;
-    constexpr int ESZ = TYPE == FLLM_TYPE_F16 ? 2 : 1;
-    const int pitch = P * ESZ + 16;
+    const int P = 1 << pg.page_log2;
+    const int pitch = lds_pitch<TYPE>(pg.hd);
+    constexpr int VB = v_bytes<TYPE>(), RUN = 16 / VB;
+    constexpr int PER = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;
     for (int s = blockIdx.y; s < b.n_seqs; s += gridDim.y) {
         Tile t;
         if (!tile_of(pg, b, new_only, s, blockIdx.x, head, &t)) continue;
         const uint8_t* cell = (kind ? pg.v : pg.k) + t.cell;
         if (kind) {
-            const int rows = TYPE == FLLM_TYPE_Q4_0 ? pg.hd / 2 : pg.hd, chunks = P * ESZ / 16;
-            for (int u = threadIdx.x; u < rows * chunks; u += blockDim.x)
-                *(uint4*)(turned + (u / chunks) * pitch + (u % chunks) * 16) = *(const uint4*)(cell + 16 * u);
-            __syncthreads();
-        }
-        const int e = threadIdx.x & 7;
-        for (int u = threadIdx.x >> 3; u < t.n * nb; u += blockDim.x >> 3) {
-            const int i = u / nb, blk = u % nb, pos = t.off + i;
-            float x[4];
-            if (TYPE == FLLM_TYPE_F16) {
-                for (int j = 0; j < 4; j++)
-                    x[j] = half_exact(kind ? *(const uint16_t*)(turned + (blk * 32 + 4 * e + j) * pitch + 2 * pos)
-                                           : ((const uint16_t*)cell)[(blk * P + pos) * 32 + 4 * e + j]);
-            } else {
-                const float d = half_exact(*(const uint16_t*)(cell + pg.scale_off + 2 * (blk * P + pos)));
-                const int per = TYPE == FLLM_TYPE_Q4_0 ? 16 : 32, e4 = 4 * e & (per - 1);
-                uint32_t w = 0;
-                if (kind == 0) w = *(const uint32_t*)(cell + (blk * P + pos) * per + e4);
-                else
-                    for (int j = 0; j < 4; j++) w |= (uint32_t)turned[(blk * per + e4 + j) * pitch + pos] << 8 * j;
+            const int lo0 = t.off / RUN, held = (t.off + t.n - 1) / RUN - lo0 + 1;
+            for (int u = threadIdx.x; u < v_rows<TYPE>(pg.hd) / 4 * held; u += blockDim.x) {
+                const int row = u / held * 4, piece = lo0 + u % held;
+                const uint8_t* from = cell + (row * P + piece * RUN) * VB;
+                uint8_t* to = turned + piece * RUN * pitch + row * VB;
+                uint32_t w[4][4];
+                for (int k = 0; k < 4; k++) {
+                    const uint4 v = *(const uint4*)(from + k * P * VB);
+                    w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+                }
                 for (int j = 0; j < 4; j++) {
-                    const uint32_t c = w >> 8 * j & 0xFFu;
-                    const int q = TYPE == FLLM_TYPE_Q8_0 ? (int)(int8_t)c : (int)(e < 4 ? c & 15u : c >> 4) - 8;
-                    x[j] = (float)q * d;
+                    if (TYPE == FLLM_TYPE_F16) {
+                        *(uint2*)(to + 2 * j * pitch) = make_uint2(__builtin_amdgcn_perm(w[1][j], w[0][j], 0x05040100u),
+                                                                   __builtin_amdgcn_perm(w[3][j], w[2][j], 0x05040100u));
+                        *(uint2*)(to + (2 * j + 1) * pitch) = make_uint2(__builtin_amdgcn_perm(w[1][j], w[0][j], 0x07060302u),
+                                                                         __builtin_amdgcn_perm(w[3][j], w[2][j], 0x07060302u));
+                    } else {
+                        const uint32_t in[4] = {w[0][j], w[1][j], w[2][j], w[3][j]};
+                        uint32_t q[4];
+                        turn4(in, q);
+                        for (int k = 0; k < 4; k++) *(uint32_t*)(to + (4 * j + k) * pitch) = q[k];
+                    }
                 }
             }
-            store4(dst, (t.row + i) * dst.ld + head * pg.hd + blk * 32 + 4 * e, x);
+            __syncthreads();
+        }
+        // a lane per EL elements, 2^el_log2 lanes (some idle) a row; 4 of them on their way
+        const int live = pg.hd / EL, all = t.n << el_log2;
+        for (int u0 = threadIdx.x; u0 < all; u0 += 4 * blockDim.x) {
+            uint32_t w[4][EL / 2];
+            uint32_t h[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int u = u0 + k * (int)blockDim.x, lane = u & ((1 << el_log2) - 1);
+                if (u >= all || lane >= live) continue;
+                const int pos = t.off + (u >> el_log2), d = lane * EL, blk = d >> 5, in = d & 31;
+                const uint8_t* row = kind ? turned + pos * pitch + blk * PER : cell + (blk * P + pos) * PER;
+                if (TYPE == FLLM_TYPE_F16) {
+                    for (int j = 0; j < EL / 2; j += 2) {
+                        const uint2 v = *(const uint2*)(row + 2 * in + 4 * j);
+                        w[k][j] = v.x, w[k][j + 1] = v.y;
+                    }
+                } else {
+                    h[k] = *(const uint16_t*)(cell + pg.scale_off + 2 * (blk * P + pos));
+                    for (int j = 0; j < EL / 4; j++) w[k][j] = *(const uint32_t*)(row + (in & (PER - 1)) + 4 * j);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int u = u0 + k * (int)blockDim.x, lane = u & ((1 << el_log2) - 1);
+                if (u >= all || lane >= live) continue;
+                float x[EL];
+                if (TYPE == FLLM_TYPE_F16) {
+                    for (int j = 0; j < EL / 2; j++) {
+                        x[2 * j] = half_float(w[k][j] & 0xFFFFu);
+                        x[2 * j + 1] = half_float(w[k][j] >> 16);
+                    }
+                } else {
+                    const float d = half_float(h[k]);
+                    const int up = TYPE == FLLM_TYPE_Q4_0 && (lane * EL & 16) ? 4 : 0;
+                    for (int j = 0; j < EL; j++) {
+                        const uint32_t c = w[k][j >> 2] >> 8 * (j & 3);
+                        const int q = TYPE == FLLM_TYPE_Q8_0 ? (int)(int8_t)(c & 0xFFu) : (int)(c >> up & 15u) - 8;
+                        x[j] = (float)q * d;
+                    }
+                }
+                uint8_t* to = dst.p + ((t.row + (u >> el_log2)) * dst.ld + head * pg.hd + lane * EL) * (16 / EL);
+                if (EL == 4) {
+                    *(float4*)to = make_float4(x[0], x[1], x[2], x[3]);
+                } else {
+                    uint32_t o[EL];
+                    for (int j = 0; j < EL; j++) o[j] = dst.type == FLLM_TYPE_F16 ? half_bits(x[j]) : bf16_round(x[j]);
+                    *(uint4*)to = make_uint4(o[0] | o[1] << 16, o[2] | o[3] << 16, o[EL - 4] | o[EL - 3] << 16, o[EL - 2] | o[EL - 1] << 16);
+                }
+            }
         }
         __syncthreads();
     }
 }
 
-// A tile of few rows has little work for 256 threads: one wave starts sooner and leaves the CU to others.
-int threads_for(const PagesView& pg, int rows) { return rows * (pg.hd >> 5) * 8 <= 64 ? 64 : 256; }
-
-size_t turned_bytes(const PagesView& pg) {
-    const size_t rows = pg.type == FLLM_TYPE_Q4_0 ? pg.hd / 2 : pg.hd, esz = pg.type == FLLM_TYPE_F16 ? 2 : 1;
-    return rows * (((size_t)1 << pg.page_log2) * esz + 16);
+int log2_up(int n) {
+    int k = 0;
+    while (1 << k < n) k++;
+    return k;
 }
 
-template <typename K>
-hipError_t lds_limit(K kernel, size_t bytes) {
-    return bytes <= 65536 ? hipSuccess
-                          : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+// A tile of few rows has little work for 256 threads: one wave starts sooner and leaves the CU to others.
+int threads_for(const PagesView& pg, int rows) { return rows * (pg.hd >> 5) <= 16 ? 64 : 256; }
+
+template <int TYPE>
+hipError_t append(const PagesView& pg, const BatchView& b, const RowsView& k, const RowsView& v, hipStream_t st) {
+    const dim3 grid(b.new_blocks, b.n_seqs < 65535 ? b.n_seqs : 65535, 2 * pg.nkv);
+    const size_t lds = (size_t)lds_pitch<TYPE>(pg.hd) << pg.page_log2;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)k_pages_append<TYPE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(k_pages_append<TYPE>, grid, dim3(threads_for(pg, b.max_new)), lds, st, pg, b, log2_up(pg.hd / 32), k, v);
+    return hipGetLastError();
+}
+
+template <int TYPE, int EL>
+hipError_t read(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v, hipStream_t st) {
+    const dim3 grid(new_only ? b.new_blocks : b.all_blocks, b.n_seqs < 65535 ? b.n_seqs : 65535, 2 * pg.nkv);
+    const size_t lds = (size_t)lds_pitch<TYPE>(pg.hd) << pg.page_log2;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)k_pages_read<TYPE, EL>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    const int rows = new_only ? b.max_new : 1 << pg.page_log2;
+    hipLaunchKernelGGL((k_pages_read<TYPE, EL>), grid, dim3(threads_for(pg, rows)), lds, st, pg, b, new_only, log2_up(pg.hd / EL), k, v);
+    return hipGetLastError();
+}
+
+template <int TYPE>
+hipError_t read_both(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v, hipStream_t st) {
+    // rows of one width go out in one launch
+    const bool wide_k = k.type == FLLM_TYPE_F32, wide_v = v.type == FLLM_TYPE_F32;
+    if (!k.p || !v.p || wide_k == wide_v)
+        return (k.p ? wide_k : wide_v) ? read<TYPE, 4>(pg, b, new_only, k, v, st) : read<TYPE, 8>(pg, b, new_only, k, v, st);
+    const RowsView none{};
+    const hipError_t e = wide_k ? read<TYPE, 4>(pg, b, new_only, k, none, st) : read<TYPE, 8>(pg, b, new_only, k, none, st);
+    if (e != hipSuccess) return e;
+    return wide_v ? read<TYPE, 4>(pg, b, new_only, none, v, st) : read<TYPE, 8>(pg, b, new_only, none, v, st);
 }
 
 }  // namespace
 
 hipError_t launch_pages_append(const PagesView& pg, const BatchView& b, const RowsView& k, const RowsView& v, hipStream_t st) {
     if (b.n_rows == 0) return hipSuccess;
-    const dim3 grid(b.new_blocks, b.n_seqs < 65535 ? b.n_seqs : 65535, 2 * pg.nkv);
-    const int thr = threads_for(pg, b.n_rows <= b.n_seqs ? 1 : 1 << pg.page_log2);
-    const size_t lds = turned_bytes(pg);
-#define FLLM_APPEND(T)                                                                       \
-    case T: {                                                                                \
-        hipError_t e = lds_limit(k_pages_append<T>, lds);                                    \
-        if (e != hipSuccess) return e;                                                       \
-        hipLaunchKernelGGL(k_pages_append<T>, grid, dim3(thr), lds, st, pg, b, k, v);        \
-        return hipGetLastError();                                                            \
-    }
     switch (pg.type) {
-        FLLM_APPEND(FLLM_TYPE_F16)
-        FLLM_APPEND(FLLM_TYPE_Q8_0)
-        FLLM_APPEND(FLLM_TYPE_Q4_0)
+        case FLLM_TYPE_F16: return append<FLLM_TYPE_F16>(pg, b, k, v, st);
+        case FLLM_TYPE_Q8_0: return append<FLLM_TYPE_Q8_0>(pg, b, k, v, st);
+        case FLLM_TYPE_Q4_0: return append<FLLM_TYPE_Q4_0>(pg, b, k, v, st);
     }
-#undef FLLM_APPEND
     return hipErrorNotSupported;
 }
 
 hipError_t launch_pages_read(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v,
                              hipStream_t st) {
-    const int blocks = new_only ? b.new_blocks : b.all_blocks;
-    if (blocks == 0) return hipSuccess;
-    const dim3 grid(blocks, b.n_seqs < 65535 ? b.n_seqs : 65535, 2 * pg.nkv);
-    const int thr = threads_for(pg, new_only && b.n_rows <= b.n_seqs ? 1 : 1 << pg.page_log2);
-    const size_t lds = turned_bytes(pg);
-#define FLLM_READ(T)                                                                              \
-    case T: {                                                                                     \
-        hipError_t e = lds_limit(k_pages_read<T>, lds);                                           \
-        if (e != hipSuccess) return e;                                                            \
-        hipLaunchKernelGGL(k_pages_read<T>, grid, dim3(thr), lds, st, pg, b, new_only, k, v);     \
-        return hipGetLastError();                                                                 \
-    }
+    if ((new_only ? b.new_blocks : b.all_blocks) == 0) return hipSuccess;
     switch (pg.type) {
-        FLLM_READ(FLLM_TYPE_F16)
-        FLLM_READ(FLLM_TYPE_Q8_0)
-        FLLM_READ(FLLM_TYPE_Q4_0)
+        case FLLM_TYPE_F16: return read_both<FLLM_TYPE_F16>(pg, b, new_only, k, v, st);
+        case FLLM_TYPE_Q8_0: return read_both<FLLM_TYPE_Q8_0>(pg, b, new_only, k, v, st);
+        case FLLM_TYPE_Q4_0: return read_both<FLLM_TYPE_Q4_0>(pg, b, new_only, k, v, st);
     }
-#undef FLLM_READ
     return hipErrorNotSupported;
 }
 

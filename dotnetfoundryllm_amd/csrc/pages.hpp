@@ -21,7 +21,7 @@ struct BatchView {
     const int4* seqs;
     int tab_w, n_seqs;
     int new_blocks, all_blocks;  // most pages of a sequence that hold new tokens, that hold any
-    int n_rows;                  // new tokens of all sequences
+    int n_rows, max_new;         // new tokens of all sequences, most of one
     int n_heads, window;
 };
 struct RowsView {
