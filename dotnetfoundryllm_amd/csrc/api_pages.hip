@@ -191,29 +191,33 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         }
         const BatchPlan& pl = b->plan;
         const int n_plan_seqs = pl.n_seqs;
-        if (!attn_plan(pl, b->n_heads, p->d.n_kv_heads, p->d.head_dim, b->window, p->ctx->n_cu, &b->attn)) {
+        if (!attn_plan(pl, b->n_heads, p->d.n_kv_heads, p->d.head_dim, p->d.type != FLLM_TYPE_F16, b->window, p->ctx->n_cu, &b->attn)) {
             b->plan.n_seqs = b->plan.n_rows = b->plan.n_pos = 0;
             return fail(FLLM_E_ARG, "the batch is too large");
         }
         b->plan.n_seqs = 0;  // empty until everything is on its way
         // sequences, items, tables: parts of 16, 64 and 4 bytes
-        const auto& items = b->attn.items;
-        const void* from[5] = {pl.seqs.data(), items[0].data(), items[1].data(), items[2].data(), pl.tables.data()};
-        const uint64_t size[5] = {(pl.seqs.size() * sizeof(SeqPlan) + 63) / 64 * 64, items[0].size() * sizeof(AttnItem),
-                                  items[1].size() * sizeof(AttnItem), items[2].size() * sizeof(AttnItem), pl.tables.size() * sizeof(int32_t)};
-        uint64_t at[6] = {0};
-        for (int i = 0; i < 5; i++) at[i + 1] = at[i] + size[i];
-        hipError_t e = batch_room(b, at[5]);
+        constexpr int N = kAttnClasses + 2;
+        const void* from[N] = {pl.seqs.data()};
+        uint64_t size[N] = {(pl.seqs.size() * sizeof(SeqPlan) + 63) / 64 * 64}, at[N + 1] = {0};
+        for (int i = 0; i < kAttnClasses; i++) {
+            from[1 + i] = b->attn.items[i].data();
+            size[1 + i] = b->attn.items[i].size() * sizeof(AttnItem);
+        }
+        from[N - 1] = pl.tables.data();
+        size[N - 1] = pl.tables.size() * sizeof(int32_t);
+        for (int i = 0; i < N; i++) at[i + 1] = at[i] + size[i];
+        hipError_t e = batch_room(b, at[N]);
         if (e != hipSuccess)
             return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "batch memory: %s", hipGetErrorString(e));
-        for (int i = 0; i < 5; i++)
+        for (int i = 0; i < N; i++)
             if (size[i]) memcpy(b->pin + at[i], from[i], i ? size[i] : pl.seqs.size() * sizeof(SeqPlan));
-        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, at[5], hipMemcpyHostToDevice, p->ctx->stream));
+        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, at[N], hipMemcpyHostToDevice, p->ctx->stream));
         HIP_TRY(hipEventRecord(b->sent, p->ctx->stream));
         b->in_flight = true;
         b->plan.n_seqs = n_plan_seqs;
         b->view.seqs = (const int4*)b->dev;
-        b->view.tables = (const int*)(b->dev + at[4]);
+        b->view.tables = (const int*)(b->dev + at[N - 1]);
         b->view.tab_w = pl.tab_w;
         b->view.n_seqs = n_plan_seqs;
         b->view.new_blocks = pl.new_blocks;
@@ -222,7 +226,7 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         b->view.max_new = pl.max_new;
         b->view.n_heads = b->n_heads;
         b->view.window = b->window;
-        for (int i = 0; i < 3; i++) {
+        for (int i = 0; i < kAttnClasses; i++) {
             b->work.items[i] = (const AttnItem*)(b->dev + at[1 + i]);
             b->work.n[i] = (int)b->attn.items[i].size();
         }

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.hpp"
+#include "pages_plan.hpp"
 
 namespace fllm {
 
@@ -34,12 +35,11 @@ struct RowsView {
 hipError_t launch_pages_append(const PagesView& pg, const BatchView& b, const RowsView& k, const RowsView& v, hipStream_t st);
 hipError_t launch_pages_read(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v,
                              hipStream_t st);
-struct AttnItem;
-// Attention items on the device (pages_plan.hpp): tiles of up to 16 rows, of up to 32, of up to 128; part: room
+// Attention items on the device (pages_plan.hpp), a list for each class of tiles; part: room
 // for part_rows * nkv rows of head_dim floats, then a max and a sum for each; cnt: as many zeros, left as zeros.
 struct AttnWork {
-    const AttnItem* items[3];
-    int n[3];
+    const AttnItem* items[kAttnClasses];
+    int n[kAttnClasses];
     float* part;
     unsigned* cnt;
     int64_t part_rows;

@@ -36,8 +36,10 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
+enum { DPP_ROR4 = 0x124, DPP_ROR8 = 0x128 };  // rotation within 16 lanes
 constexpr float kNoScore = -1e30f;  // the running maximum before any key
 
 union H8 {
@@ -102,6 +104,20 @@ __device__ __forceinline__ int row_exponent(float top) {
     if (!(top > 0.0f && top < INFINITY)) return 0;
     const int e = 15 - __builtin_amdgcn_frexp_expf(top);  // top = f 2^k, f in [1/2, 1): e = 15 - k
     return e > 120 ? 120 : e;
+}
+
+// 8 codes (two words) as fp16 integers; Q4_0: of the low (half 0) or high nibbles
+template <int TYPE>
+__device__ __forceinline__ H8 codes8(uint32_t a, uint32_t b, int half) {
+    H8 r;
+    if (TYPE == FLLM_TYPE_Q8_0) {
+        bytes_to_half<1152>(a ^ 0x80808080u, r.u);
+        bytes_to_half<1152>(b ^ 0x80808080u, r.u + 2);
+    } else {
+        bytes_to_half<1032>(a >> 4 * half & 0x0F0F0F0Fu, r.u);
+        bytes_to_half<1032>(b >> 4 * half & 0x0F0F0F0Fu, r.u + 2);
+    }
+    return r;
 }
 
 // x as fp16 halves: one rounded to nearest, or a high and a low one (both cut, together 21 to 22 bits)
@@ -236,13 +252,21 @@ __device__ __forceinline__ void join_parts(const AttnArgsP& a, const AttnItem& i
 }
 
 // Wide heads take the registers of two waves: one wave a SIMD then has as many bytes on their way.
-template <int TYPE, int HDP, int NP, int TM>
+//
+// Columns. A quantised cache has a scale per key and block of 32 elements, so that every block needs operands of its
+// own. Tiles of RC < 16 rows leave columns of the matrix tiles over: the rows are repeated in SUB groups of columns and
+// group j works on the blocks [j BPS, (j + 1) BPS) alone. Its q is zero in the other blocks, so one chain of products
+// gives each column its block's dot product, to be scaled once and summed over the groups; its weights are
+// multiplied by its own blocks' scales, and of each product with V only the columns whose group the block belongs
+// to are kept. A lane then loads and applies BPS scales a key in place of NB.
+template <int TYPE, int HDP, int NP, int TM, int RC>
 __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP a) {
     constexpr int NB = HDP / 32, ND = HDP / 16;      // blocks of 32 elements, tiles of 16
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
     // runs of 32 keys a step: 16 bytes of V a lane, 8 where registers are short
     constexpr int JN = QUANT && HDP <= 128 && TM == 1 ? 2 : 1;
     constexpr int STEP = 32 * JN, RUN = 8 * JN;      // keys a step, consecutive keys a lane holds
+    constexpr int SUB = !QUANT || 16 / RC < 1 ? 1 : 16 / RC < NB ? 16 / RC : NB, BPS = NB / SUB;
     constexpr int NV = TYPE == FLLM_TYPE_Q4_0 ? NB : ND;  // loads of V a step (one byte row holds two elements in Q4_0)
     constexpr bool QLDS = HDP * TM >= 256;           // q stays in LDS where registers are short
     __shared__ union {
@@ -292,20 +316,25 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
     }
     __syncthreads();
     // this lane's query of each row tile: its position (-1 where there is no row), what undoes its scaling
+    const int cq = RC < 16 ? col % RC : col, sub = RC < 16 ? col / RC % SUB : 0;
     int pos[TM];
     float unscale[TM];
     h8 qr[QLDS ? 1 : TM][QLDS ? 1 : NB][NP];
     const auto q_frag = [&](int m, int c, int n) {
-        const _Float16* p = &sm.q[n][16 * m + col][32 * c];
-        if (TYPE != FLLM_TYPE_Q4_0) return *(const h8*)(p + 8 * g);
+        const _Float16* p = &sm.q[n][16 * m + cq][32 * c];
         H8 f;  // the elements that Frag's 8 stand for
-        *(u2*)&f.u[0] = *(const u2*)(p + 4 * g);
-        *(u2*)&f.u[2] = *(const u2*)(p + 16 + 4 * g);
+        if (TYPE != FLLM_TYPE_Q4_0) {
+            f.v = *(const h8*)(p + 8 * g);
+        } else {
+            *(u2*)&f.u[0] = *(const u2*)(p + 4 * g);
+            *(u2*)&f.u[2] = *(const u2*)(p + 16 + 4 * g);
+        }
+        if (SUB > 1 && c / BPS != sub) f.u[0] = f.u[1] = f.u[2] = f.u[3] = 0;
         return f.v;
     };
 #pragma unroll
     for (int m = 0; m < TM; m++) {
-        const int r = 16 * m + col;
+        const int r = 16 * m + cq;
         pos[m] = r < it.nrows ? pos0 + (it.row0 + r) / a.group : -1;
         unscale[m] = s_scale[r];
         if (!QLDS) {
@@ -350,12 +379,13 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
             for (int c = 0; c < NB; c++)
                 kf[t][c].load(kp + (uint32_t)(((c < nb ? c : 0) * P + 4 * t) * KB));
         // scales of this lane's keys, 8 to a vector
-        u4 ks[QUANT ? NB : 1][JN], vs[QUANT ? NB : 1][JN];
+        u4 ks[QUANT ? BPS : 1][JN], vs[QUANT ? BPS : 1][JN];
         if (QUANT) {
 #pragma unroll
-            for (int c = 0; c < NB; c++)
+            for (int c = 0; c < BPS; c++)
                 for (int i = 0; i < JN; i++) {
-                    const uint32_t at = a.pg.scale_off + (uint32_t)(2 * ((c < nb ? c : 0) * P + pv)) + 16 * i;
+                    const int blk = sub * BPS + c;
+                    const uint32_t at = a.pg.scale_off + (uint32_t)(2 * ((blk < nb ? blk : 0) * P + pv)) + 16 * i;
                     ks[c][i] = *(const u4*)(a.pg.k + cv + at);
                     vs[c][i] = *(const u4*)(a.pg.v + cv + at);
                 }
@@ -377,7 +407,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
                 if (QUANT) {
                     const uint32_t keep = in ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
 #pragma unroll
-                    for (int c = 0; c < NB; c++) vs[c][i >> 3][(i & 7) >> 1] &= keep;
+                    for (int c = 0; c < BPS; c++) vs[c][i >> 3][(i & 7) >> 1] &= keep;
                 } else {
                     const uint32_t keep = in ? 0xFFFFFFFFu : i & 1 ? 0x0000FFFFu : 0xFFFF0000u;
 #pragma unroll
@@ -386,17 +416,14 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
             }
         }
         if (QUANT) {  // the units of o: the largest scale so far
-            h2 top = {(_Float16)0, (_Float16)0};
-            for (int c = 0; c < NB; c++)
-                    for (int i = 0; i < 4 * JN; i++) {
-                        union { uint32_t u; h2 h; } s;
-                        s.u = vs[c][i >> 2][i & 3] & 0x7FFF7FFFu;
-                        top = __builtin_elementwise_max(top, s.h);
-                    }
-            float f = fmaxf((float)top.x, (float)top.y);
-            f = fmaxf(f, __shfl_xor(f, 16));
-            f = fmaxf(f, __shfl_xor(f, 32));
-            const int e = __builtin_amdgcn_readfirstlane((int)(__float_as_uint(f) >> 23) - 126);  // f < 2^e
+            us2 top = {0, 0};  // magnitudes compare as integers
+            for (int c = 0; c < BPS; c++)
+                for (int i = 0; i < 4 * JN; i++) {
+                    union { uint32_t u; us2 h; } s;
+                    s.u = vs[c][i >> 2][i & 3] & 0x7FFF7FFFu;
+                    top = __builtin_elementwise_max(top, s.h);
+                }
+            const int e = ((int)wave_max((float)max((int)top.x, (int)top.y)) >> 10) - 14;  // every scale < 2^e
             if (e > vexp) {
                 const float down = ldexpf(1.0f, vexp - e);
                 for (int m = 0; m < TM; m++)
@@ -412,20 +439,30 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
 #pragma unroll
             for (int t = 0; t < 2 * JN; t++) {
                 f4 acc = {0.f, 0.f, 0.f, 0.f};
+                if (QUANT) {
 #pragma unroll
-                for (int c = 0; c < NB; c++) {
-                    const h8 kh = kf[t][c].half();
-                    if (QUANT) {
+                    for (int p = 0; p < BPS; p++) {
                         f4 b = {0.f, 0.f, 0.f, 0.f};
-                        for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, c, n), b, 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < SUB; j++) {
+                            const h8 kh = kf[t][j * BPS + p].half();
+                            for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, j * BPS + p, n), b, 0, 0, 0);
+                        }
                         for (int e = 0; e < 4; e++) {
                             union { uint32_t u; h2 h; } d;
-                            d.u = ks[c][t >> 1][2 * (t & 1) + (e >> 1)];
+                            d.u = ks[p][t >> 1][2 * (t & 1) + (e >> 1)];
                             acc[e] = fmaf(b[e], (float)(e & 1 ? d.h.y : d.h.x), acc[e]);
                         }
-                    } else {
-                        for (int n = NP - 1; n >= 0; n--) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, c, n), acc, 0, 0, 0);
                     }
+                    for (int e = 0; e < 4; e++) {  // over the groups of columns
+                        if (SUB > 1 && SUB * RC > 8) acc[e] += dpp<DPP_ROR8>(0.0f, acc[e]);
+                        if (SUB > 1 && RC == 4) acc[e] += dpp<DPP_ROR4>(0.0f, acc[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < NB; c++)
+                        for (int n = NP - 1; n >= 0; n--)
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][c].half(), q_of(m, c, n), acc, 0, 0, 0);
                 }
                 for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e] * unscale[m];
             }
@@ -464,30 +501,27 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
             } else {
                 for (int i = 0; i < RUN; i++) s[i] *= vunit;
 #pragma unroll
-                for (int c = 0; c < NB; c++) {
+                for (int p = 0; p < BPS; p++) {
                     h8 wf[JN][NP];
                     for (int j = 0; j < JN; j++) {
                         float w[8];
                         for (int i = 0; i < 8; i++) {
                             union { uint32_t u; h2 h; } d;
-                            d.u = vs[c][j][i >> 1];
+                            d.u = vs[p][j][i >> 1];
                             w[i] = fmaf((float)(i & 1 ? d.h.y : d.h.x), s[8 * j + i], 0.0f);
                         }
                         split8<NP>(w, wf[j]);
                     }
-                    for (int h = 0; h < 2; h++)
-                        for (int j = 0; j < JN; j++) {
-                            H8 v;
-                            if (TYPE == FLLM_TYPE_Q8_0) {
-                                bytes_to_half<1152>(vf[TYPE == FLLM_TYPE_Q4_0 ? 0 : 2 * c + h][2 * j] ^ 0x80808080u, v.u);
-                                bytes_to_half<1152>(vf[TYPE == FLLM_TYPE_Q4_0 ? 0 : 2 * c + h][2 * j + 1] ^ 0x80808080u, v.u + 2);
-                            } else {
-                                bytes_to_half<1032>(vf[c][2 * j] >> 4 * h & 0x0F0F0F0Fu, v.u);
-                                bytes_to_half<1032>(vf[c][2 * j + 1] >> 4 * h & 0x0F0F0F0Fu, v.u + 2);
+#pragma unroll
+                    for (int u = 0; u < SUB; u++)
+                        for (int h = 0; h < 2; h++)
+                            for (int j = 0; j < JN; j++) {
+                                const int c = u * BPS + p;
+                                const uv& word = vf[TYPE == FLLM_TYPE_Q4_0 ? c : 2 * c + h];
+                                const H8 v = codes8<TYPE>(word[2 * j], word[2 * j + 1], h);
+                                for (int n = NP - 1; n >= 0; n--)
+                                    o[m][2 * c + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[j][n], o[m][2 * c + h], 0, 0, 0);
                             }
-                            for (int n = NP - 1; n >= 0; n--)
-                                o[m][2 * c + h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[j][n], o[m][2 * c + h], 0, 0, 0);
-                        }
                 }
             }
         }
@@ -505,13 +539,15 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
         sum[m] += __shfl_xor(sum[m], 16);
         sum[m] += __shfl_xor(sum[m], 32);
         __syncthreads();  // q, or the tile before, is done with
-        if (g == 0) {
-            s_m[wave][col] = mx[m];
-            s_l[wave][col] = sum[m];
+        if (g == 0 && col < RC) {
+            s_m[wave][cq] = mx[m];
+            s_l[wave][cq] = sum[m];
         }
-        for (int d = 0; d < ND; d++) *(f4*)&sm.o[wave][col][16 * d + 4 * g] = o[m][d] * unit;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            if (SUB == 1 || (col < RC * SUB && d / 2 / BPS == sub)) *(f4*)&sm.o[wave][cq][16 * d + 4 * g] = o[m][d] * unit;
         __syncthreads();
-        for (int u = threadIdx.x; u < 16 * (HDP / 4); u += 256) {
+        for (int u = threadIdx.x; u < (RC < 16 ? RC : 16) * (HDP / 4); u += 256) {
             const int r = u / (HDP / 4), d = u % (HDP / 4) * 4, row = 16 * m + r;
             if (row >= it.nrows || d >= hd) continue;
             const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
@@ -542,9 +578,8 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
 
 // ---- many rows -----------------------------------------------------------------------------
 typedef float f16v __attribute__((ext_vector_type(16)));
-typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
-constexpr int kManyRows = kAttnTile[2], kManySplit = kAttnSplit[2];
+constexpr int kManyRows = kAttnTile[kAttnClasses - 1], kManySplit = kAttnSplit[kAttnClasses - 1];
 
 // LDS planes of a step: K [keys][HDP], V [HDP][keys], halves in chunks of 8. Chunk c of a row lies at
 // c ^ swizzle(row), so that the 16 rows that a quarter of a wave reads cover the banks once.
@@ -555,20 +590,6 @@ __device__ __forceinline__ int k_chunk(int key, int c) {
 template <int STEP>
 __device__ __forceinline__ int v_chunk(int d, int c) {
     return STEP == 64 ? d * 8 + (c ^ (d >> 1 & 7)) : d * 4 + (c ^ (d >> 2 & 3));
-}
-
-// 8 codes (two words) as fp16 integers; Q4_0: of the low (half 0) or high nibbles
-template <int TYPE>
-__device__ __forceinline__ H8 codes8(uint32_t a, uint32_t b, int half) {
-    H8 r;
-    if (TYPE == FLLM_TYPE_Q8_0) {
-        bytes_to_half<1152>(a ^ 0x80808080u, r.u);
-        bytes_to_half<1152>(b ^ 0x80808080u, r.u + 2);
-    } else {
-        bytes_to_half<1032>(a >> 4 * half & 0x0F0F0F0Fu, r.u);
-        bytes_to_half<1032>(b >> 4 * half & 0x0F0F0F0Fu, r.u + 2);
-    }
-    return r;
 }
 
 // codes times scales (one per element, times 2^s), as halves in planes `gap` chunks apart
@@ -910,12 +931,16 @@ inline AttnArgsP attend_args(const PagesView& pg, const BatchView& b, const Attn
 
 template <int TYPE, int HDP, int NP>
 hipError_t launch_items(AttnArgsP a, const AttnWork& w, hipStream_t st) {
-    for (int c = 2; c >= 0; c--) {
+    // the long-running tiles first
+    for (int c = kAttnClasses - 1; c >= 0; c--) {
         if (w.n[c] == 0) continue;
         a.items = w.items[c];
         const dim3 grid((unsigned)w.n[c] * (unsigned)a.pg.nkv);
-        if (c == 0) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1>), grid, dim3(256), 0, st, a);
-        else if (c == 1) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2>), grid, dim3(256), 0, st, a);
+        constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
+        if (c == 0) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, QUANT ? 4 : 16>), grid, dim3(256), 0, st, a);
+        else if (c == 1) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, QUANT ? 8 : 16>), grid, dim3(256), 0, st, a);
+        else if (c == 2) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, 16>), grid, dim3(256), 0, st, a);
+        else if (c == 3) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2, 16>), grid, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP>), grid, dim3(256), 0, st, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

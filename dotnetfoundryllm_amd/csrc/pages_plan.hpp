@@ -175,11 +175,12 @@ struct AttnItem {
     int pad[4];
 };
 constexpr int kKeyStep = 64;
-constexpr int kAttnTile[3] = {16, 32, 128};
-constexpr int kAttnSplit[3] = {128, 128, 32};  // most items of a tile
+constexpr int kAttnClasses = 5;
+constexpr int kAttnTile[kAttnClasses] = {4, 8, 16, 32, 128};       // rows of a tile
+constexpr int kAttnSplit[kAttnClasses] = {128, 128, 128, 128, 32};  // most items of one
 
 struct AttnPlan {
-    std::vector<AttnItem> items[3];  // tiles of up to kAttnTile[c] rows
+    std::vector<AttnItem> items[kAttnClasses];  // tiles of up to kAttnTile[c] rows
     int64_t part_rows = 0;           // partial rows per kv head
 };
 
@@ -222,12 +223,15 @@ inline void attn_count(const SeqPlan& s, int group, int window, int c, int64_t s
 }
 
 // The items of a batch on a device of n_cu CUs. False where they or their partial rows are too many.
-inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, int window, int n_cu, AttnPlan* p) {
+inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, bool quant, int window, int n_cu, AttnPlan* p) {
     const int group = n_heads / n_kv;
     p->part_rows = 0;
+    constexpr int kMany = kAttnClasses - 1;
+    // the smallest tile that holds the sequence's rows; an F16 cache has no use for the two smallest (pages_attend.hpp)
     const auto class_of = [&](const SeqPlan& s) {
-        const int64_t rows = (int64_t)s.n_new * group;
-        return rows <= kAttnTile[0] ? 0 : rows <= kAttnTile[1] ? 1 : 2;
+        int c = quant ? 0 : 2;
+        while (c < kMany && (int64_t)s.n_new * group > kAttnTile[c]) c++;
+        return c;
     };
     // two workgroups are resident on a CU, one of heads wider than 128
     const int64_t slots = (head_dim > 128 ? 1 : 2) * (int64_t)n_cu;
@@ -238,7 +242,7 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, i
         const int64_t mid = (few + hi) / 2;
         AttnCount n;
         for (const SeqPlan& s : b.seqs)
-            if (class_of(s) < 2) attn_count(s, group, window, class_of(s), mid, &n);
+            if (class_of(s) < kMany) attn_count(s, group, window, class_of(s), mid, &n);
         if (n.items * n_kv <= slots) hi = mid;
         else few = mid + 1;
     }
@@ -246,7 +250,7 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, i
     // about half a longest item after the mean; a part of a tile costs about 3 steps more (its partial rows).
     const auto ends = [&](int64_t steps, AttnCount* n) {
         for (const SeqPlan& s : b.seqs)
-            if (class_of(s) == 2) attn_count(s, group, window, 2, steps, n);
+            if (class_of(s) == kMany) attn_count(s, group, window, kMany, steps, n);
         return n->items * n_kv <= slots ? (double)n->longest
                                         : (double)(n->steps + 3 * n->items) * n_kv / (double)slots + 0.5 * (double)n->longest;
     };
@@ -263,7 +267,7 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, i
     for (int i = 0; i < b.n_seqs; i++) {
         const SeqPlan& s = b.seqs[(size_t)i];
         const int c = class_of(s);
-        if (s.n_new) attn_items(s, i, i * b.tab_w, group, window, c, c == 2 ? many : few, &p->items[c], &p->part_rows);
+        if (s.n_new) attn_items(s, i, i * b.tab_w, group, window, c, c == kMany ? many : few, &p->items[c], &p->part_rows);
         if (p->part_rows > INT32_MAX / n_kv) return false;
     }
     for (auto& v : p->items) {

@@ -13,7 +13,7 @@ static BatchError g_err;
 extern "C" int32_t plan_set(const fllm_pages_desc* d, int32_t n_heads, int32_t window, int32_t n_cu, int32_t n_seqs,
                             const int32_t* n_new, const int32_t* lengths, const int32_t* tables, int64_t ld) {
     if (batch_plan(*d, window, n_seqs, n_new, lengths, tables, ld, &g_plan, &g_err)) return g_err.code;
-    return attn_plan(g_plan, n_heads, d->n_kv_heads, d->head_dim, window, n_cu, &g_attn) ? 0 : -100;
+    return attn_plan(g_plan, n_heads, d->n_kv_heads, d->head_dim, d->type != FLLM_TYPE_F16, window, n_cu, &g_attn) ? 0 : -100;
 }
 extern "C" const char* plan_error() { return g_err.text; }
 extern "C" int64_t plan_items(int32_t c, AttnItem* out) {

@@ -12,7 +12,7 @@ import dotnetfoundryllm_amd._native as N
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 NO_WINDOW = 0x7FFFFFFF
-TILE, SPLIT = (16, 32, 128), (128, 128, 32)  # rows of the item classes, most items of a tile
+TILE, SPLIT = (4, 8, 16, 32, 128), (128, 128, 128, 128, 32)  # rows of the item classes, most items of a tile
 STEP = 64
 
 
@@ -128,7 +128,8 @@ def test_items_cover_every_row_and_key_once(lib):
         rng.shuffle(order)
         for i, k in enumerate(need):
             table[i, :k] = [order.pop() for _ in range(k)]
-        assert plan(lib, new, length, table, heads, kv, 64, page, max(1, sum(need)), window, rng.choice([1, 64, 256])) == 0
+        assert plan(lib, new, length, table, heads, kv, rng.choice([64, 256]), page, max(1, sum(need)), window, rng.choice([1, 64, 256]),
+                    rng.choice([N.F16, N.Q8_0, N.Q4_0])) == 0
         s = sizes(lib)
         assert (s["rows"], s["pos"], s["all_blocks"], s["max_new"]) == (sum(new), sum(length), max(need), max(new))
         assert s["new_blocks"] == max([0] + [-(-ln // page) - (ln - x) // page for x, ln in zip(new, length) if x])
