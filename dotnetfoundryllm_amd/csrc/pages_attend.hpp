@@ -229,8 +229,8 @@ __device__ __forceinline__ void join_parts(const AttnArgsP& a, const AttnItem& i
             l += m1[i] * l1[i];
         }
         const float inv = 1.0f / wave_sum(l);
-        for (int i = 0; i < N; i++)
-            if (lane + 64 * i < it.nsplit) w[row * MAXS + lane + 64 * i] = m1[i] * inv;
+        for (int i = 0; i < N; i++)  // zeros past the end
+            if (lane + 64 * i < MAXS) w[row * MAXS + lane + 64 * i] = lane + 64 * i < it.nsplit ? m1[i] * inv : 0.0f;
     }
     __syncthreads();
     for (int u = threadIdx.x; u < it.nrows * (hd / 4); u += 256) {
@@ -242,7 +242,7 @@ __device__ __forceinline__ void join_parts(const AttnArgsP& a, const AttnItem& i
             for (int i = 0; i < 16; i++) v[i] = ld_wt4(ro, (uint32_t)(((k0 + i) * it.nrows + row) * hd + d) * 4);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const float f = k0 + i < it.nsplit ? w[row * MAXS + k0 + i] : 0.0f;
+                const float f = w[row * MAXS + k0 + i];
                 acc += f * f4{v[i].x, v[i].y, v[i].z, v[i].w};
             }
         }
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
     constexpr int NB = HDP / 32, ND = HDP / 16;      // blocks of 32 elements, tiles of 16
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
     // runs of 32 keys a step: 16 bytes of V a lane, 8 where registers are short
-    constexpr int JN = QUANT && HDP <= 128 && TM == 1 ? 2 : 1;
+    constexpr int JN = QUANT && HDP <= 128 && RC < 16 ? 2 : 1;
     constexpr int STEP = 32 * JN, RUN = 8 * JN;      // keys a step, consecutive keys a lane holds
     constexpr int SUB = !QUANT || 16 / RC < 1 ? 1 : 16 / RC < NB ? 16 / RC : NB, BPS = NB / SUB;
     constexpr int NV = TYPE == FLLM_TYPE_Q4_0 ? NB : ND;  // loads of V a step (one byte row holds two elements in Q4_0)
@@ -284,6 +284,67 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
     const int pos0 = it.pos0;
     const int* table = a.tables + it.table;
     const int last_block = (it.len - 1) >> lp;
+
+    // this lane's row of a tile, and the group of columns that it is in
+    const int cq = RC < 16 ? col % RC : col, sub = RC < 16 ? col / RC % SUB : 0;
+    constexpr int ksub = RUN;  // keys of a lane group
+    // K: row col of tile (j, t) is key ksub (col >> 2) + 8 j + 4 t + (col & 3) of the step; V: this lane holds the keys
+    // ksub g .. + RUN. Both lie in one page each; past the table's end the last page stands in. A step's K is loaded
+    // as soon as the step before has its scores, its V once the step before is added up, so that both are on their way
+    // through the other half of a step; the page numbers are a step ahead of them.
+    constexpr int KB = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;  // bytes of a block's codes
+    constexpr int VW = TYPE == FLLM_TYPE_F16 ? 4 : 2 * JN, VE = TYPE == FLLM_TYPE_F16 ? 2 : 1;
+    typedef uint32_t uv __attribute__((ext_vector_type(VW)));
+    Frag<TYPE> kf[2 * JN][NB];
+    u4 ks[QUANT ? BPS : 1][JN], vs[QUANT ? BPS : 1][JN];  // scales of this lane's keys, 8 to a vector
+    uv vf[NV];                                            // 8 halves, or the codes of this lane's keys
+    int tk, tv;                                           // pages of the next step
+    uint64_t cv;                                          // the step's cell for this lane's keys
+    const auto pages_at = [&](int k0) {
+        tk = table[min((k0 + ksub * (col >> 2)) >> lp, last_block)];
+        tv = table[min((k0 + ksub * g) >> lp, last_block)];
+    };
+    const auto load_k = [&](int k0) {
+        const int kk = k0 + ksub * (col >> 2), pv = (k0 + ksub * g) & (P - 1);
+        const uint64_t ck = ((uint64_t)(uint32_t)tk * a.pg.nkv + kvh) * a.pg.cell;
+        cv = ((uint64_t)(uint32_t)tv * a.pg.nkv + kvh) * a.pg.cell;
+        const uint8_t* kp = a.pg.k + ck + (uint32_t)(((kk & (P - 1)) + (col & 3)) * KB + g * (KB / 4));
+#pragma unroll
+        for (int t = 0; t < 2 * JN; t++)
+#pragma unroll
+            for (int c = 0; c < NB; c++) kf[t][c].load(kp + (uint32_t)(((c < nb ? c : 0) * P + 4 * t) * KB));
+        if (QUANT)
+#pragma unroll
+            for (int c = 0; c < BPS; c++)
+                for (int i = 0; i < JN; i++) {
+                    const int blk = sub * BPS + c;
+                    ks[c][i] = *(const u4*)(a.pg.k + cv + a.pg.scale_off + (uint32_t)(2 * ((blk < nb ? blk : 0) * P + pv)) + 16 * i);
+                }
+    };
+    const auto load_v = [&](int k0) {
+        const int pv = (k0 + ksub * g) & (P - 1);
+        if (QUANT)
+#pragma unroll
+            for (int c = 0; c < BPS; c++)
+                for (int i = 0; i < JN; i++) {
+                    const int blk = sub * BPS + c;
+                    vs[c][i] = *(const u4*)(a.pg.v + cv + a.pg.scale_off + (uint32_t)(2 * ((blk < nb ? blk : 0) * P + pv)) + 16 * i);
+                }
+        const uint8_t* vp = a.pg.v + cv + (uint32_t)((col * P + pv) * VE);
+#pragma unroll
+        for (int d = 0; d < NV; d++)
+            vf[d] = *(const uv*)(vp + (uint32_t)((d < (TYPE == FLLM_TYPE_Q4_0 ? nb : 2 * nb) ? d : 0) * 16 * P * VE));
+    };
+    const int first = it.k0 + wave * STEP;
+    constexpr bool AHEAD = !(QUANT && TM == 2 && HDP > 64);  // there the registers do not allow it
+    if (first < it.k1) {
+        pages_at(first);
+        if (AHEAD) {
+            load_k(first);
+            load_v(first);
+            pages_at(first + 4 * STEP < it.k1 ? first + 4 * STEP : first);
+        }
+    }
 
     // q as fp16 halves in LDS, 16 lanes a row: every row scaled by the power of two 2^e that brings its largest
     // magnitude into [2^14, 2^15); zeros for the rows and elements that are not there
@@ -316,7 +377,6 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
     }
     __syncthreads();
     // this lane's query of each row tile: its position (-1 where there is no row), what undoes its scaling
-    const int cq = RC < 16 ? col % RC : col, sub = RC < 16 ? col / RC % SUB : 0;
     int pos[TM];
     float unscale[TM];
     h8 qr[QLDS ? 1 : TM][QLDS ? 1 : NB][NP];
@@ -360,44 +420,50 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
     const int64_t all_lo = (int64_t)last_pos - a.window + 1, all_hi = pos0 + it.row0 / a.group + 1;
     const int64_t any_lo = all_hi - a.window;  // the first key that any row sees
 
-    constexpr int ksub = RUN;  // keys of a lane group
-    for (int k0 = it.k0 + wave * STEP; k0 < it.k1; k0 += 4 * STEP) {
+    for (int k0 = first; k0 < it.k1; k0 += 4 * STEP) {
         if (QLDS) asm volatile("" ::: "memory");  // or its reads would be kept in registers across the loop
-        // K: row col of tile (j, t) is key ksub (col >> 2) + 8 j + 4 t + (col & 3); V: this lane holds the
-        // keys ksub g .. + RUN. Both lie in one page each; past the table's end the last page stands in.
-        const int kk = k0 + ksub * (col >> 2), kv = k0 + ksub * g;
-        const int bk = min(kk >> lp, last_block), bv = min(kv >> lp, last_block);
-        const uint64_t ck = ((uint64_t)(uint32_t)table[bk] * a.pg.nkv + kvh) * a.pg.cell;
-        const uint64_t cv = ((uint64_t)(uint32_t)table[bv] * a.pg.nkv + kvh) * a.pg.cell;
-        const int pk = (kk & (P - 1)) + (col & 3), pv = kv & (P - 1);
-        constexpr int KB = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;  // bytes of a block's codes
-        const uint8_t* kp = a.pg.k + ck + (uint32_t)(pk * KB + g * (KB / 4));
-        Frag<TYPE> kf[2 * JN][NB];
-#pragma unroll
-        for (int t = 0; t < 2 * JN; t++)
-#pragma unroll
-            for (int c = 0; c < NB; c++)
-                kf[t][c].load(kp + (uint32_t)(((c < nb ? c : 0) * P + 4 * t) * KB));
-        // scales of this lane's keys, 8 to a vector
-        u4 ks[QUANT ? BPS : 1][JN], vs[QUANT ? BPS : 1][JN];
-        if (QUANT) {
-#pragma unroll
-            for (int c = 0; c < BPS; c++)
-                for (int i = 0; i < JN; i++) {
-                    const int blk = sub * BPS + c;
-                    const uint32_t at = a.pg.scale_off + (uint32_t)(2 * ((blk < nb ? blk : 0) * P + pv)) + 16 * i;
-                    ks[c][i] = *(const u4*)(a.pg.k + cv + at);
-                    vs[c][i] = *(const u4*)(a.pg.v + cv + at);
-                }
+        const int kv = k0 + ksub * g;
+        // unconditionally, or the waits for this step's loads would wait for the next one's too: the last step again
+        const int next = k0 + 4 * STEP < it.k1 ? k0 + 4 * STEP : k0;
+        if (!AHEAD) {
+            load_k(k0);
+            load_v(k0);
+            pages_at(next);
         }
-        constexpr int VW = TYPE == FLLM_TYPE_F16 ? 4 : 2 * JN;
-        typedef uint32_t uv __attribute__((ext_vector_type(VW)));
-        uv vf[NV];  // 8 halves, or the codes of this lane's keys
-        constexpr int VE = TYPE == FLLM_TYPE_F16 ? 2 : 1;
-        const uint8_t* vp = a.pg.v + cv + (uint32_t)((col * P + pv) * VE);
+        float s[TM][RUN];
 #pragma unroll
-        for (int d = 0; d < NV; d++)
-            vf[d] = *(const uv*)(vp + (uint32_t)((d < (TYPE == FLLM_TYPE_Q4_0 ? nb : 2 * nb) ? d : 0) * 16 * P * VE));
+        for (int m = 0; m < TM; m++)
+#pragma unroll
+            for (int t = 0; t < 2 * JN; t++) {
+                f4 acc = {0.f, 0.f, 0.f, 0.f};
+                if (QUANT) {
+#pragma unroll
+                    for (int p = 0; p < BPS; p++) {
+                        f4 b = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int j = 0; j < SUB; j++) {
+                            const h8 kh = kf[t][j * BPS + p].half();
+                            for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, j * BPS + p, n), b, 0, 0, 0);
+                        }
+                        for (int e = 0; e < 4; e++) {
+                            union { uint32_t u; h2 h; } d;
+                            d.u = ks[p][t >> 1][2 * (t & 1) + (e >> 1)];
+                            acc[e] = fmaf(b[e], (float)(e & 1 ? d.h.y : d.h.x), acc[e]);
+                        }
+                    }
+                    for (int e = 0; e < 4; e++) {  // over the groups of columns
+                        if (SUB > 1 && SUB * RC > 8) acc[e] += dpp<DPP_ROR8>(0.0f, acc[e]);
+                        if (SUB > 1 && RC == 4) acc[e] += dpp<DPP_ROR4>(0.0f, acc[e]);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < NB; c++)
+                        for (int n = NP - 1; n >= 0; n--)
+                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][c].half(), q_of(m, c, n), acc, 0, 0, 0);
+                }
+                for (int e = 0; e < 4; e++) s[m][4 * t + e] = acc[e] * unscale[m];
+            }
+        if (AHEAD) load_k(next);
 
         const bool edge = k0 < all_lo || k0 + STEP > all_hi;
         if (edge) {
@@ -435,44 +501,13 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
 
 #pragma unroll
         for (int m = 0; m < TM; m++) {
-            float s[RUN];
-#pragma unroll
-            for (int t = 0; t < 2 * JN; t++) {
-                f4 acc = {0.f, 0.f, 0.f, 0.f};
-                if (QUANT) {
-#pragma unroll
-                    for (int p = 0; p < BPS; p++) {
-                        f4 b = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int j = 0; j < SUB; j++) {
-                            const h8 kh = kf[t][j * BPS + p].half();
-                            for (int n = NP - 1; n >= 0; n--) b = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, q_of(m, j * BPS + p, n), b, 0, 0, 0);
-                        }
-                        for (int e = 0; e < 4; e++) {
-                            union { uint32_t u; h2 h; } d;
-                            d.u = ks[p][t >> 1][2 * (t & 1) + (e >> 1)];
-                            acc[e] = fmaf(b[e], (float)(e & 1 ? d.h.y : d.h.x), acc[e]);
-                        }
-                    }
-                    for (int e = 0; e < 4; e++) {  // over the groups of columns
-                        if (SUB > 1 && SUB * RC > 8) acc[e] += dpp<DPP_ROR8>(0.0f, acc[e]);
-                        if (SUB > 1 && RC == 4) acc[e] += dpp<DPP_ROR4>(0.0f, acc[e]);
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < NB; c++)
-                        for (int n = NP - 1; n >= 0; n--)
-                            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][c].half(), q_of(m, c, n), acc, 0, 0, 0);
-                }
-                for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e] * unscale[m];
-            }
             if (a.softcap > 0.0f)
-                for (int i = 0; i < RUN; i++) s[i] = cap * tanh_of(s[i]);
+                for (int i = 0; i < RUN; i++) s[m][i] = cap * tanh_of(s[m][i]);
             if (edge)
                 for (int i = 0; i < RUN; i++)
-                    if (kv + i > pos[m] || (int64_t)kv + i <= (int64_t)pos[m] - a.window) s[i] = -INFINITY;
-            float top = s[0];
-            for (int i = 1; i < RUN; i++) top = fmaxf(top, s[i]);
+                    if (kv + i > pos[m] || (int64_t)kv + i <= (int64_t)pos[m] - a.window) s[m][i] = -INFINITY;
+            float top = s[m][0];
+            for (int i = 1; i < RUN; i++) top = fmaxf(top, s[m][i]);
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
             const float nm = fmaxf(mx[m], top);
@@ -480,8 +515,8 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
             mx[m] = nm;
             float l = 0.0f;
             for (int i = 0; i < RUN; i++) {
-                s[i] = __builtin_amdgcn_exp2f(s[i] - nm);
-                l += s[i];
+                s[m][i] = __builtin_amdgcn_exp2f(s[m][i] - nm);
+                l += s[m][i];
             }
             sum[m] = sum[m] * down + l;
             if (__any(down != 1.0f))  // the maximum seldom grows after the first steps
@@ -489,7 +524,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
 
             if (!QUANT) {
                 float w[8];
-                for (int i = 0; i < 8; i++) w[i] = s[i] * vunit;
+                for (int i = 0; i < 8; i++) w[i] = s[m][i] * vunit;
                 h8 wf[NP];
                 split8<NP>(w, wf);
 #pragma unroll
@@ -499,7 +534,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
                     for (int n = NP - 1; n >= 0; n--) o[m][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.v, wf[n], o[m][d], 0, 0, 0);
                 }
             } else {
-                for (int i = 0; i < RUN; i++) s[i] *= vunit;
+                for (int i = 0; i < RUN; i++) s[m][i] *= vunit;
 #pragma unroll
                 for (int p = 0; p < BPS; p++) {
                     h8 wf[JN][NP];
@@ -508,7 +543,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
                         for (int i = 0; i < 8; i++) {
                             union { uint32_t u; h2 h; } d;
                             d.u = vs[p][j][i >> 1];
-                            w[i] = fmaf((float)(i & 1 ? d.h.y : d.h.x), s[8 * j + i], 0.0f);
+                            w[i] = fmaf((float)(i & 1 ? d.h.y : d.h.x), s[m][8 * j + i], 0.0f);
                         }
                         split8<NP>(w, wf[j]);
                     }
@@ -524,6 +559,10 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
                             }
                 }
             }
+        }
+        if (AHEAD) {
+            load_v(next);
+            pages_at(next + 4 * STEP < it.k1 ? next + 4 * STEP : next);
         }
     }
 
