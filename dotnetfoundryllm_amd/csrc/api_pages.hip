@@ -196,14 +196,16 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
             return fail(FLLM_E_ARG, "the batch is too large");
         }
         b->plan.n_seqs = 0;  // empty until everything is on its way
-        // sequences, items, tables: parts of 16, 64 and 4 bytes
-        constexpr int N = kAttnClasses + 2;
+        // sequences, items, images, tables: parts of 16, 64, 32 and 4 bytes
+        constexpr int N = kAttnClasses + 3;
         const void* from[N] = {pl.seqs.data()};
         uint64_t size[N] = {(pl.seqs.size() * sizeof(SeqPlan) + 63) / 64 * 64}, at[N + 1] = {0};
         for (int i = 0; i < kAttnClasses; i++) {
             from[1 + i] = b->attn.items[i].data();
             size[1 + i] = b->attn.items[i].size() * sizeof(AttnItem);
         }
+        from[N - 2] = b->attn.image_items.data();
+        size[N - 2] = b->attn.image_items.size() * sizeof(ImageItem);
         from[N - 1] = pl.tables.data();
         size[N - 1] = pl.tables.size() * sizeof(int32_t);
         for (int i = 0; i < N; i++) at[i + 1] = at[i] + size[i];
@@ -231,6 +233,9 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
             b->work.n[i] = (int)b->attn.items[i].size();
         }
         b->work.part_rows = b->attn.part_rows;
+        b->work.image_items = (const ImageItem*)(b->dev + at[N - 2]);
+        b->work.n_image_items = (int)b->attn.image_items.size();
+        b->work.n_images = b->attn.images;
         return FLLM_OK;
     });
 }
@@ -377,11 +382,16 @@ extern "C" int32_t fllm_pages_attention(fllm_batch* b, int32_t layer, const fllm
     std::lock_guard<std::mutex> lock(p->ctx->ws.mu);
     AttnWork w = b->work;
     const uint64_t rows = (uint64_t)w.part_rows * (uint64_t)p->d.n_kv_heads;
-    hipError_t e = workspace_room(p->ctx, rows * (uint64_t)(p->d.head_dim + 2) * sizeof(float), rows);
+    const uint64_t part = (rows * (uint64_t)(p->d.head_dim + 2) * sizeof(float) + 255) / 256 * 256;
+    const uint64_t images = (uint64_t)w.n_images * (uint64_t)p->d.n_kv_heads;
+    const uint64_t image = images * attend_image_bytes(p->d.head_dim, rq.type == FLLM_TYPE_F32 || ro.type == FLLM_TYPE_F32);
+    hipError_t e = workspace_room(p->ctx, part + image + images * 4 * sizeof(float), rows);
     if (e != hipSuccess)
         return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "attention workspace: %s", hipGetErrorString(e));
     w.part = (float*)p->ctx->ws.part;
     w.cnt = p->ctx->ws.cnt;
+    w.images = p->ctx->ws.part + part;
+    w.image_units = (float*)(p->ctx->ws.part + part + image);
     HIP_TRY(launch_pages_attention(pages_view(p, layer), b->view, w, rq, ro, scale, softcap, p->ctx->stream));
     return FLLM_OK;
 }

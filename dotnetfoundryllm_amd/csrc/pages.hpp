@@ -43,7 +43,18 @@ struct AttnWork {
     float* part;
     unsigned* cnt;
     int64_t part_rows;
+    // steps that are turned into images first: room for images * nkv * 64 keys of K and V (attend_image_bytes) and for
+    // 4 floats each
+    const ImageItem* image_items;
+    int n_image_items;
+    int64_t n_images;
+    void* images;
+    float* image_units;
 };
+// bytes of the images of one kv head's 64 keys; wide: F32 rows of q or out
+inline uint64_t attend_image_bytes(int hd, bool wide) {
+    return (uint64_t)(hd <= 64 ? 64 : hd <= 128 ? 128 : 256) * kKeyStep * 2 * 2 * (wide ? 2 : 1);
+}
 hipError_t launch_pages_attention(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q,
                                   const RowsView& out, float scale, float softcap, hipStream_t st);
 

@@ -48,6 +48,13 @@ union H8 {
     uint32_t u[4];
 };
 
+// The scale of the scores in two parts: its sign, which goes into q, and its magnitude, never zero (a masked score is
+// -inf, times zero it would be a NaN): a scale of zero makes q zero.
+__device__ __forceinline__ float scale_sign(float s) { return s < 0.0f ? -1.0f : s > 0.0f ? 1.0f : 0.0f; }
+__device__ __forceinline__ float scale_size(float s, int e, float softcap) {
+    return fmaxf(ldexpf(s == 0.0f ? 1.0f : fabsf(s), -e) * (softcap > 0.0f ? 1.0f / softcap : kLog2e), 1e-37f);
+}
+
 // 4 bytes, each code + 128 or nibble, as fp16 integers: 0x6400 | byte is 1024 + byte exactly
 template <int OFF>
 __device__ __forceinline__ void bytes_to_half(uint32_t w, uint32_t* out) {
@@ -121,18 +128,43 @@ __device__ __forceinline__ H8 codes8(uint32_t a, uint32_t b, int half) {
 }
 
 // x as fp16 halves: one rounded to nearest, or a high and a low one (both cut, together 21 to 22 bits)
+// Mixed-precision multiply-adds on half SEL of a word: a b of two halves, a b of a half and a float, x - a.
+template <int SEL>
+__device__ __forceinline__ float mix_mul(uint32_t a, uint32_t b) {
+    float r;
+    if (SEL) asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel:[1,1,0] op_sel_hi:[1,1,0]" : "=v"(r) : "v"(a), "v"(b));
+    else asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel_hi:[1,1,0]" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+template <int SEL>
+__device__ __forceinline__ float mix_scale(uint32_t a, float b) {
+    float r;
+    if (SEL) asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(a), "v"(b));
+    else asm("v_fma_mix_f32 %0, %1, %2, 0 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+template <int SEL>
+__device__ __forceinline__ float mix_rest(uint32_t a, float x) {
+    float r;
+    if (SEL) asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(a), "v"(x));
+    else asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(a), "v"(x));
+    return r;
+}
+
+// x and y as a high and a low half each
+__device__ __forceinline__ void split2(float x, float y, h2* hi, h2* lo) {
+    union { __fp16 __attribute__((ext_vector_type(2))) c; h2 h; uint32_t u; } a, b;
+    a.c = __builtin_amdgcn_cvt_pkrtz(x, y);
+    b.c = __builtin_amdgcn_cvt_pkrtz(mix_rest<0>(a.u, x), mix_rest<1>(a.u, y));
+    *hi = a.h;
+    *lo = b.h;
+}
+
 template <int NP>
 __device__ __forceinline__ void split4(const f4 x, h2 out[NP][2]) {
     for (int i = 0; i < 2; i++) {
-        if (NP == 1) {
-            out[0][i] = h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
-        } else {
-            union { __fp16 __attribute__((ext_vector_type(2))) c; h2 h; } a, b;
-            a.c = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-            b.c = __builtin_amdgcn_cvt_pkrtz(fmaf((float)a.h.x, -1.0f, x[2 * i]), fmaf((float)a.h.y, -1.0f, x[2 * i + 1]));
-            out[0][i] = a.h;
-            out[NP - 1][i] = b.h;
-        }
+        if (NP == 1) out[0][i] = h2{(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+        else split2(x[2 * i], x[2 * i + 1], &out[0][i], &out[NP - 1][i]);
     }
 }
 template <int NP>
@@ -147,13 +179,31 @@ __device__ __forceinline__ void split8(const float x[8], h8 out[NP]) {
     }
 }
 
-// tanh to 1e-7: a series near zero, where the quotient would cancel
-__device__ __forceinline__ float tanh_of(float x) {
-    const float y = x * x;
-    const float p = x * fmaf(y, fmaf(y, fmaf(y, fmaf(y, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-    const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
-    const float q = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
-    return fabsf(x) < 0.25f ? p : q;
+// cap tanh(us s) of a lane's N scores. Near zero the quotient (1 - t) / (1 + t), t = exp(-2 |x|), cancels: below 1/10
+// a series to x^5 is exact to 6e-8, and where a wave's scores are all that small it is all that runs.
+template <int N, typename V>
+__device__ __forceinline__ void softcap_n(V& s, float us, float cap) {
+    float top = 0.0f;
+    for (int i = 0; i < N; i++) {
+        s[i] *= us;
+        top = fmaxf(top, fabsf(s[i]));
+    }
+    const bool far = __any(top >= 0.1f);
+    for (int i = 0; i < N; i++) {
+        const float x = s[i], y = x * x;
+        const float p = x * fmaf(y, fmaf(y, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
+        s[i] = cap * p;
+        if (far) {
+            const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
+            const float q = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+            const uint32_t big = fabsf(x) < 0.1f ? 0u : 0xFFFFFFFFu;  // selected by bits: no branch per score
+            s[i] = cap * __uint_as_float((__float_as_uint(q) & big) | (__float_as_uint(p) & ~big));
+        }
+    }
+}
+template <typename V>
+__device__ __forceinline__ void softcap16(V& s, float us, float cap) {
+    softcap_n<16>(s, us, cap);
 }
 
 __device__ __forceinline__ f4 load_row4(const RowsView& r, int64_t i) {
@@ -193,6 +243,8 @@ struct AttnArgsP {
     float scale, softcap;
     float *part_o, *part_ml;
     unsigned* cnt;
+    void* images;         // SRC_IMAGE
+    float* image_units;
 };
 
 // Counts this workgroup's partial rows, whose stores were all issued before, as there; true for the workgroup that
@@ -368,16 +420,16 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
         const int e = row_exponent(top);
 #pragma unroll
         for (int i = 0; i < HDP / 64; i++) {
-            const f4 y = x[i] * ldexpf(1.0f, e);
+            const f4 y = x[i] * ldexpf(scale_sign(a.scale), e);
             h2 h[NP][2];
             split4<NP>(y, h);
             for (int n = 0; n < NP; n++) *(u2*)&sm.q[n][r][4 * l16 + 64 * i] = u2{bits(h[n][0]), bits(h[n][1])};
         }
-        if (l16 == 0) s_scale[r] = ldexpf(a.scale, -e) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+        if (l16 == 0) s_scale[r] = scale_size(a.scale, e, a.softcap);
     }
     __syncthreads();
     // this lane's query of each row tile: its position (-1 where there is no row), what undoes its scaling
-    int pos[TM];
+    int pos[TM], low[TM];  // and the first position that it sees
     float unscale[TM];
     h8 qr[QLDS ? 1 : TM][QLDS ? 1 : NB][NP];
     const auto q_frag = [&](int m, int c, int n) {
@@ -396,6 +448,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
     for (int m = 0; m < TM; m++) {
         const int r = 16 * m + cq;
         pos[m] = r < it.nrows ? pos0 + (it.row0 + r) / a.group : -1;
+        low[m] = (int)max((int64_t)pos[m] - a.window + 1, (int64_t)INT_MIN);
         unscale[m] = s_scale[r];
         if (!QLDS) {
 #pragma unroll
@@ -404,8 +457,6 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
         }
     }
     const auto q_of = [&](int m, int c, int n) { return QLDS ? q_frag(m, c, n) : qr[QLDS ? 0 : m][QLDS ? 0 : c][n]; };
-    const float cap = a.softcap * kLog2e;
-
     f4 o[TM][ND];
     float mx[TM], sum[TM];
     int vexp = -30;  // quantised: o is in units of 2^(vexp - 14), vexp at least the exponent of any scale so far (2^-24 and up, or zeros)
@@ -461,7 +512,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
                         for (int n = NP - 1; n >= 0; n--)
                             acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][c].half(), q_of(m, c, n), acc, 0, 0, 0);
                 }
-                for (int e = 0; e < 4; e++) s[m][4 * t + e] = acc[e] * unscale[m];
+                for (int e = 0; e < 4; e++) s[m][4 * t + e] = acc[e];
             }
         if (AHEAD) load_k(next);
 
@@ -501,21 +552,23 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
 
 #pragma unroll
         for (int m = 0; m < TM; m++) {
-            if (a.softcap > 0.0f)
-                for (int i = 0; i < RUN; i++) s[m][i] = cap * tanh_of(s[m][i]);
+            float us = unscale[m];
+            if (a.softcap > 0.0f) {
+                softcap_n<RUN>(s[m], us, a.softcap * kLog2e);
+                us = 1.0f;
+            }
             if (edge)
-                for (int i = 0; i < RUN; i++)
-                    if (kv + i > pos[m] || (int64_t)kv + i <= (int64_t)pos[m] - a.window) s[m][i] = -INFINITY;
+                for (int i = 0; i < RUN; i++) s[m][i] = kv + i > pos[m] || kv + i < low[m] ? -INFINITY : s[m][i];
             float top = s[m][0];
             for (int i = 1; i < RUN; i++) top = fmaxf(top, s[m][i]);
             top = fmaxf(top, __shfl_xor(top, 16));
             top = fmaxf(top, __shfl_xor(top, 32));
-            const float nm = fmaxf(mx[m], top);
+            const float nm = fmaxf(mx[m], top * us);
             const float down = __builtin_amdgcn_exp2f(mx[m] - nm);
             mx[m] = nm;
             float l = 0.0f;
             for (int i = 0; i < RUN; i++) {
-                s[m][i] = __builtin_amdgcn_exp2f(s[m][i] - nm);
+                s[m][i] = __builtin_amdgcn_exp2f(fmaf(s[m][i], us, -nm));
                 l += s[m][i];
             }
             sum[m] = sum[m] * down + l;
@@ -541,9 +594,8 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
                     for (int j = 0; j < JN; j++) {
                         float w[8];
                         for (int i = 0; i < 8; i++) {
-                            union { uint32_t u; h2 h; } d;
-                            d.u = vs[p][j][i >> 1];
-                            w[i] = fmaf((float)(i & 1 ? d.h.y : d.h.x), s[m][8 * j + i], 0.0f);
+                            const uint32_t d = vs[p][j][i >> 1];
+                            w[i] = i & 1 ? mix_scale<1>(d, s[m][8 * j + i]) : mix_scale<0>(d, s[m][8 * j + i]);
                         }
                         split8<NP>(w, wf[j]);
                     }
@@ -616,65 +668,222 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
 }
 
 // ---- many rows -----------------------------------------------------------------------------
+// k_attend_many: tiles of up to 128 rows (prompt chunks), bound by the matrix products. Four waves of 32 rows share
+// steps of keys whose K and V lie in LDS as halves: one plane where a half holds a value exactly (F16 cache) or the rows
+// are 16-bit ones (NP = 1: code times scale, rounded), two planes that hold code times scale exactly (NP = 2); quantised
+// values are multiplied by the power of two that brings their step's largest scale to 2^8. S^T is 32 keys by 32
+// queries a tile: a lane holds 16 keys of its query, so a row's maximum is one exchange between two lanes.
+// Where the halves come from (SRC):
+//   SRC_PAGES   an F16 cache's pages, straight to LDS (16 bytes a lane; the LDS image is made by which address a
+//               lane loads), two steps deep: the next step arrives while one is multiplied
+//   SRC_IMAGE   LDS images that k_pages_image made of a quantised cache's pages before, once for all tiles of a
+//               sequence, likewise
+//   SRC_CODES   a quantised cache's codes, turned into halves by every workgroup: for sequences of few tiles, where
+//               writing and reading images costs more than the turning
 typedef float f16v __attribute__((ext_vector_type(16)));
+enum { SRC_PAGES, SRC_IMAGE, SRC_CODES };
 
 constexpr int kManyRows = kAttnTile[kAttnClasses - 1], kManySplit = kAttnSplit[kAttnClasses - 1];
 
 // LDS planes of a step: K [keys][HDP], V [HDP][keys], halves in chunks of 8. Chunk c of a row lies at
 // c ^ swizzle(row), so that the 16 rows that a quarter of a wave reads cover the banks once.
+template <int HDP> __device__ __forceinline__ int k_swizzle(int key) { return HDP == 64 ? key >> 1 & 7 : key & 15; }
+template <int STEP> __device__ __forceinline__ int v_swizzle(int d) { return STEP == 64 ? d >> 1 & 7 : d >> 2 & 3; }
 template <int HDP>
 __device__ __forceinline__ int k_chunk(int key, int c) {
-    return key * (HDP / 8) + (c ^ (HDP == 64 ? key >> 1 & 7 : key & 15));
+    return key * (HDP / 8) + (c ^ k_swizzle<HDP>(key));
 }
 template <int STEP>
 __device__ __forceinline__ int v_chunk(int d, int c) {
-    return STEP == 64 ? d * 8 + (c ^ (d >> 1 & 7)) : d * 4 + (c ^ (d >> 2 & 3));
+    return d * (STEP / 8) + (c ^ v_swizzle<STEP>(d));
 }
 
-// codes times scales (one per element, times 2^s), as halves in planes `gap` chunks apart
+// 8 codes times their scales d (two halves a word, `step` words on for each two codes) times unit, as halves: in one
+// plane rounded, or in two exactly, `gap` chunks apart.
 template <int KP>
-__device__ __forceinline__ void scaled_out(const H8& c, const uint32_t* d, int step, float unit, u4* to, int gap) {
+__device__ __forceinline__ void scaled_out(const H8& c, const uint32_t* d, int step, h2 unit, u4* to, int gap) {
     H8 hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         union { uint32_t u; h2 h; } s;
         s.u = d[i * step];
+        s.h = s.h * unit;
         if (KP == 1) {
-            const h2 t = s.h * h2{(_Float16)unit, (_Float16)unit};
-            hi.p[i] = c.p[i] * t;
+            hi.p[i] = c.p[i] * s.h;
         } else {
-            const float x = fmaf((float)c.p[i].x, (float)s.h.x * unit, 0.0f), y = fmaf((float)c.p[i].y, (float)s.h.y * unit, 0.0f);
-            union { __fp16 __attribute__((ext_vector_type(2))) c; h2 h; } a, b;
-            a.c = __builtin_amdgcn_cvt_pkrtz(x, y);
-            b.c = __builtin_amdgcn_cvt_pkrtz(fmaf((float)a.h.x, -1.0f, x), fmaf((float)a.h.y, -1.0f, y));
-            hi.p[i] = a.h;
-            lo.p[i] = b.h;
+            const float x = mix_mul<0>(c.u[i], s.u), y = mix_mul<1>(c.u[i], s.u);
+            split2(x, y, &hi.p[i], &lo.p[i]);
         }
     }
     to[0] = u4{hi.u[0], hi.u[1], hi.u[2], hi.u[3]};
     if (KP == 2) to[gap] = u4{lo.u[0], lo.u[1], lo.u[2], lo.u[3]};
 }
 
-// keys a step: 64, or 32 where q, o and the codes on their way leave too few registers
+// keys a step: 64, or 32 where q, o and the codes on their way leave too few registers or the planes too little LDS
 constexpr int many_step(int hdp, int np) { return hdp > 128 || (hdp == 128 && np == 2) ? 32 : 64; }
 
+// the workgroup's LDS writes (and with DIRECT its loads into LDS) are done, and every wave is here; loads into
+// registers stay on their way
+template <bool DIRECT>
+__device__ __forceinline__ void lds_barrier() {
+    if (DIRECT) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void to_lds(const void* from, u4* to) {  // lane l's 16 bytes to to[l]
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+}
+
+// A step's codes of a quantised cache, from the pages into registers and as halves into planes.
+template <int TYPE, int HDP, int STEP, int KP>
+struct Codes {
+    static constexpr int NB = HDP / 32, PIECES = STEP / 16, CH = STEP * HDP / 8;
+    static constexpr int KU = (STEP * NB + 255) / 256;          // (key, block) units a thread
+    static constexpr int VROWS = TYPE == FLLM_TYPE_Q4_0 ? HDP / 2 : HDP;
+    static constexpr int VU = (VROWS * PIECES + 255) / 256;     // (row, 16 keys) units a thread
+    static constexpr int KW = TYPE == FLLM_TYPE_Q8_0 ? 2 : 1;   // 16-byte words of a K unit
+    u4 kr[KU][KW], vr[VU], vd[VU][2], ks, vs;  // codes, V's scales, a wave's view of all scales
+    uint32_t kd[KU];                           // K's scale of the unit
+    int pk, pv[VU], ps;                        // pages of the next step
+    float kunit;                               // what K's values are multiplied by
+    int vexp;                                  // V's are multiplied by 2^min(8 - vexp, 15)
+
+    __device__ __forceinline__ void pages_at(const int* table, int last_block, int lp, int k0) {
+        const auto page_of = [&](int key) { return table[min(key >> lp, last_block)]; };
+        pk = page_of(k0 + (int)threadIdx.x % STEP);
+        for (int i = 0; i < VU; i++) pv[i] = page_of(k0 + 16 * (((int)threadIdx.x + 256 * i) / VROWS & (PIECES - 1)));
+        ps = page_of(k0 + 8 * ((int)threadIdx.x & (STEP / 8 - 1)));
+    }
+    __device__ __forceinline__ void load(const PagesView& pg, int kvh, int k0) {
+        constexpr int KB = TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;
+        const int tid = threadIdx.x, lane = tid & 63, nb = pg.hd >> 5, P = 1 << pg.page_log2;
+        const auto cell = [&](int page) { return ((uint64_t)(uint32_t)page * pg.nkv + kvh) * pg.cell; };
+        const int key = k0 + tid % STEP;
+        const uint8_t* kc = pg.k + cell(pk);
+#pragma unroll
+        for (int i = 0; i < KU; i++) {
+            const int blk = tid / STEP + 256 / STEP * i, at = (blk < nb ? blk : 0) * P + (key & (P - 1));
+            for (int w = 0; w < KW; w++) kr[i][w] = *(const u4*)(kc + (uint32_t)(at * KB + 16 * w));
+            kd[i] = *(const uint16_t*)(kc + pg.scale_off + (uint32_t)(2 * at));
+        }
+#pragma unroll
+        for (int i = 0; i < VU; i++) {
+            const int u = tid + 256 * i, row = u % VROWS, key16 = k0 + 16 * (u / VROWS & (PIECES - 1));
+            const int rows = TYPE == FLLM_TYPE_Q4_0 ? pg.hd / 2 : pg.hd, blk = TYPE == FLLM_TYPE_Q4_0 ? row >> 4 : row >> 5;
+            const uint8_t* vc = pg.v + cell(pv[i]);
+            vr[i] = *(const u4*)(vc + (uint32_t)((row < rows ? row : 0) * P + (key16 & (P - 1))));
+            const uint8_t* sc = vc + pg.scale_off + (uint32_t)(2 * ((blk < nb ? blk : 0) * P + (key16 & (P - 1))));
+            vd[i][0] = *(const u4*)sc;
+            vd[i][1] = *(const u4*)(sc + 16);
+        }
+        const int blk = lane / (STEP / 8), at = 2 * ((blk < nb ? blk : 0) * P + ((k0 + 8 * (lane & (STEP / 8 - 1))) & (P - 1)));
+        ks = *(const u4*)(pg.k + cell(ps) + pg.scale_off + (uint32_t)at);
+        vs = *(const u4*)(pg.v + cell(ps) + pg.scale_off + (uint32_t)at);
+    }
+    // kunit and vexp from the step's largest scales among the keys [lo, hi) that the sequence has; V scales of zero for
+    // the others, which may be anything
+    __device__ __forceinline__ void look(int k0, int64_t lo, int64_t hi) {
+        const int tid = threadIdx.x, lane = tid & 63;
+        us2 tk = {0, 0}, tv = {0, 0};
+        const bool outside = k0 < lo || k0 + STEP > hi;
+        for (int i = 0; i < 4; i++) {
+            union { uint32_t u; us2 h; } x, y;  // magnitudes compare as integers
+            x.u = ks[i] & 0x7FFF7FFFu;
+            y.u = vs[i] & 0x7FFF7FFFu;
+            if (outside) {
+                const int64_t key = k0 + 8 * (lane & (STEP / 8 - 1)) + 2 * i;
+                const uint32_t keep = (key >= lo && key < hi ? 0xFFFFu : 0u) | (key + 1 >= lo && key + 1 < hi ? 0xFFFF0000u : 0u);
+                x.u &= keep;
+                y.u &= keep;
+            }
+            tk = __builtin_elementwise_max(tk, x.h);
+            tv = __builtin_elementwise_max(tv, y.h);
+        }
+        if (outside)
+            for (int i = 0; i < VU; i++)
+                for (int j = 0; j < 16; j++) {
+                    const int64_t key = k0 + 16 * ((tid + 256 * i) / VROWS & (PIECES - 1)) + j;
+                    vd[i][j >> 3][(j & 7) >> 1] &= key >= lo && key < hi ? 0xFFFFFFFFu : j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+                }
+        const int ek = ((int)wave_max((float)max((int)tk.x, (int)tk.y)) >> 10) - 14;  // every scale < 2^ek
+        kunit = ldexpf(1.0f, min(8 - ek, 15));
+        vexp = ((int)wave_max((float)max((int)tv.x, (int)tv.y)) >> 10) - 14;
+    }
+    // the codes in registers as halves: K's planes at k, V's at v; V's values for the exponent e >= vexp
+    __device__ __forceinline__ void stage(u4* k, u4* v, int e) const {
+        const int tid = threadIdx.x;
+        const h2 ku = h2{(_Float16)kunit, (_Float16)kunit};
+        const _Float16 vf = (_Float16)ldexpf(1.0f, min(8 - e, 15));
+        const h2 vu = h2{vf, vf};
+#pragma unroll
+        for (int i = 0; i < KU; i++) {
+            const int key = tid % STEP, blk = tid / STEP + 256 / STEP * i;
+            if (STEP * NB % 256 && blk >= NB) continue;
+            const uint32_t d = kd[i] | kd[i] << 16;
+            for (int c = 0; c < 4; c++) {
+                const u4& w = kr[i][TYPE == FLLM_TYPE_Q8_0 ? c >> 1 & (KW - 1) : 0];
+                scaled_out<KP>(codes8<TYPE>(w[2 * (c & 1)], w[2 * (c & 1) + 1], TYPE == FLLM_TYPE_Q8_0 ? 0 : c >> 1), &d, 0, ku,
+                               k + k_chunk<HDP>(key, 4 * blk + c), CH);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < VU; i++) {
+            const int u = tid + 256 * i, row = u % VROWS, piece = u / VROWS;
+            if (VROWS * PIECES % 256 && piece >= PIECES) continue;
+            for (int c = 0; c < 2; c++) {
+                const uint32_t d[4] = {vd[i][c].x, vd[i][c].y, vd[i][c].z, vd[i][c].w};
+                const int at = TYPE == FLLM_TYPE_Q4_0 ? (row >> 4) * 32 + (row & 15) : row;
+                for (int n = 0; n < (TYPE == FLLM_TYPE_Q4_0 ? 2 : 1); n++)
+                    scaled_out<KP>(codes8<TYPE>(vr[i][2 * c], vr[i][2 * c + 1], n), d, 1, vu, v + v_chunk<STEP>(at + 16 * n, 2 * piece + c), CH);
+            }
+        }
+    }
+};
+
+// Images of a quantised cache's steps: [step][kv head] of the planes K, V as they lie in LDS, and of (1 / kunit, vexp).
 template <int TYPE, int HDP, int NP>
+__global__ __launch_bounds__(256) void k_pages_image(AttnArgsP a, const ImageItem* items) {
+    constexpr int STEP = many_step(HDP, NP);
+    using C = Codes<TYPE, HDP, STEP, NP>;
+    __shared__ u4 planes[2][NP * C::CH];
+    const int kvh = blockIdx.x % a.pg.nkv;
+    const ImageItem it = items[blockIdx.x / a.pg.nkv];
+    const int* table = a.tables + it.table;
+    const int last_block = (it.len - 1) >> a.pg.page_log2;
+    C c;
+    c.pages_at(table, last_block, a.pg.page_log2, it.k0);
+    c.load(a.pg, kvh, it.k0);
+    for (int i = 0; i < it.n * (kKeyStep / STEP); i++) {
+        const int k0 = it.k0 + i * STEP;
+        c.look(k0, it.lo, it.len);
+        if (i) lds_barrier<false>();  // the image before is copied
+        c.stage(planes[0], planes[1], c.vexp);
+        const int64_t at = ((int64_t)it.image * (kKeyStep / STEP) + i) * a.pg.nkv + kvh;
+        if (threadIdx.x == 0) {
+            a.image_units[2 * at] = 1.0f / c.kunit;
+            a.image_units[2 * at + 1] = (float)c.vexp;
+        }
+        c.pages_at(table, last_block, a.pg.page_log2, k0 + STEP);
+        c.load(a.pg, kvh, k0 + STEP);
+        lds_barrier<false>();
+        u4* to = (u4*)a.images + at * (2 * NP * C::CH);
+        const u4* from = planes[0];
+        for (int u = threadIdx.x; u < 2 * NP * C::CH; u += 256) to[u] = from[u];
+    }
+}
+
+template <int TYPE, int HDP, int NP, int SRC>
 __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgsP a) {
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
-    constexpr int NB = HDP / 32, KS = HDP / 16;
+    constexpr int KS = HDP / 16, ND = HDP / 32;
     constexpr int KP = QUANT ? NP : 1;                       // planes of K and V
     constexpr int STEP = many_step(HDP, NP), T = STEP / 32;  // keys a step, tiles of 32
-    constexpr int PIECES = STEP / 16;
-    constexpr int KCH = STEP * HDP / 8, VCH = KCH;           // chunks of 8 halves a plane
-    constexpr int KU = (STEP * NB + 255) / 256;              // (key, block) units a thread
-    constexpr int VROWS = TYPE == FLLM_TYPE_Q4_0 ? HDP / 2 : HDP;
-    constexpr int VU = (VROWS * PIECES + 255) / 256;              // (row, 16 keys) units a thread
-    constexpr int KW = TYPE == FLLM_TYPE_F16 ? 4 : TYPE == FLLM_TYPE_Q8_0 ? 2 : 1;  // 16-byte words of a K unit
-    constexpr int VW = TYPE == FLLM_TYPE_F16 ? 2 : 1;                               // of a V unit
+    constexpr int CH = STEP * HDP / 8;                       // chunks of 8 halves a plane
+    constexpr int DL = CH / 256;                             // loads of a plane a thread
+    constexpr bool DIRECT = SRC != SRC_CODES;
     __shared__ union {
-        struct {
-            u4 k[KP * KCH], v[KP * VCH];
-        } t;
+        u4 t[DIRECT ? 2 : 1][2][KP * CH];  // [step parity][K, V]
         float w[kManySplit * kManyRows];
     } sm;
     __shared__ int s_last;
@@ -685,12 +894,57 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
     const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
     const int* table = a.tables + it.table;
     const int last_block = (it.len - 1) >> lp;
+    const int64_t tile_lo = (int64_t)it.pos0 + it.row0 / a.group + 1 - a.window;  // the first key that any row sees
+
+    // ---- the steps on their way; pages of a step are looked up a step before its loads
+    Codes<QUANT ? TYPE : (int)FLLM_TYPE_Q8_0, HDP, STEP, KP> codes;  // SRC_CODES
+    int pk[DL], pv;                                                  // SRC_PAGES
+    float ik = 1.0f, ik_next = 1.0f;                                 // quantised: 1 / kunit of this step and the next
+    int ev = 0, ev_next = 0;                                         // and vexp
+    const auto pages_at = [&](int k0) {
+        if (SRC == SRC_CODES) codes.pages_at(table, last_block, lp, k0);
+        if (SRC == SRC_PAGES) {
+            for (int i = 0; i < DL; i++) pk[i] = table[min((k0 + (tid + 256 * i) / (HDP / 8)) >> lp, last_block)];
+            // the chunk that this thread's slots hold is the same in each: 256 slots are a multiple of 16 rows
+            pv = table[min((k0 + 8 * ((tid % (STEP / 8)) ^ v_swizzle<STEP>(tid / (STEP / 8)))) >> lp, last_block)];
+        }
+    };
+    const auto load = [&](int k0, int buf) {
+        if (SRC == SRC_CODES) codes.load(a.pg, kvh, k0);
+        if (SRC == SRC_IMAGE) {
+            k0 = min(k0, (it.k1 - 1) / STEP * STEP);  // past the item's end: its last step again
+            const int64_t at = ((int64_t)it.image * (kKeyStep / STEP) + k0 / STEP) * a.pg.nkv + kvh;
+            const u4* p = (const u4*)a.images + at * (2 * KP * CH) + tid;
+#pragma unroll
+            for (int i = 0; i < 2 * KP * DL; i++) to_lds(p + 256 * i, &sm.t[buf][0][256 * i + 64 * wave]);
+            ik_next = a.image_units[2 * at];
+            ev_next = (int)a.image_units[2 * at + 1];
+        }
+        if (SRC == SRC_PAGES) {  // slot by slot of the LDS image
+            const auto cell = [&](int page) { return ((uint64_t)(uint32_t)page * a.pg.nkv + kvh) * a.pg.cell; };
+#pragma unroll
+            for (int i = 0; i < DL; i++) {
+                const int slot = tid + 256 * i, key = slot / (HDP / 8), c = (slot % (HDP / 8)) ^ k_swizzle<HDP>(key);
+                to_lds(a.pg.k + cell(pk[i]) + (uint32_t)((((c >> 2) < nb ? c >> 2 : 0) * P + ((k0 + key) & (P - 1))) * 64 + (c & 3) * 16),
+                       &sm.t[buf][0][256 * i + 64 * wave]);
+            }
+            const uint8_t* vc = a.pg.v + cell(pv);
+#pragma unroll
+            for (int i = 0; i < DL; i++) {
+                const int slot = tid + 256 * i, d = slot / (STEP / 8), c = (slot % (STEP / 8)) ^ v_swizzle<STEP>(d);
+                to_lds(vc + (uint32_t)((d < hd ? d : 0) * P + ((k0 + 8 * c) & (P - 1))) * 2, &sm.t[buf][1][256 * i + 64 * wave]);
+            }
+        }
+    };
+    pages_at(it.k0);
+    load(it.k0, 0);
+    pages_at(it.k0 + STEP);
 
     // this lane's query
     const int r = 32 * wave + col;
     const bool live = r < it.nrows;
     const int qrow = it.row0 + (live ? r : 0), qtok = qrow / a.group, head = kvh * a.group + qrow % a.group;
-    const int pos = live ? it.pos0 + qtok : -1;
+    const int pos = live ? it.pos0 + qtok : -1, low = (int)max((int64_t)pos - a.window + 1, (int64_t)INT_MIN);
     float unscale;
     h8 q[KS][NP];
     {
@@ -726,210 +980,127 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
             }
         top = fmaxf(top, __shfl_xor(top, 32));
         const int e = row_exponent(top);
-        const float up = ldexpf(1.0f, e);
+        const float up = ldexpf(scale_sign(a.scale), e);
 #pragma unroll
         for (int k = 0; k < KS; k++) {
             for (int i = 0; i < 8; i++) x[k][i] *= up;
             split8<NP>(x[k], q[k]);
         }
-        unscale = ldexpf(a.scale, -e) * (a.softcap > 0.0f ? 1.0f / a.softcap : kLog2e);
+        unscale = scale_size(a.scale, e, a.softcap);
     }
-    const float cap = a.softcap * kLog2e;
 
-    f16v o[HDP / 32];
-    for (int d = 0; d < HDP / 32; d++)
+    f16v o[ND];
+    for (int d = 0; d < ND; d++)
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float mx = kNoScore, sum = 0.0f;
-    int vexp = -30;
-    // keys that every row of the wave, any row of it and any row of the tile sees
+    // keys that every row of the wave sees: [all_lo, all_hi)
     const int w0 = it.row0 + min(32 * wave, it.nrows - 1), w1 = it.row0 + min(32 * wave + 31, it.nrows - 1);
     const int64_t all_hi = it.pos0 + w0 / a.group + 1, all_lo = (int64_t)it.pos0 + w1 / a.group - a.window + 1;
-    const int64_t any_hi = 32 * wave < it.nrows ? it.pos0 + w1 / a.group + 1 : 0, any_lo = all_hi - a.window;
-    const int64_t tile_lo = (int64_t)it.pos0 + it.row0 / a.group + 1 - a.window;
 
-    // ---- a step's codes and scales on their way to LDS
-    u4 kr[KU][KW], vr[VU][VW], ks, vs;
-    uint32_t kd[KU];             // K: the unit's scale
-    u4 vd[QUANT ? VU : 1][2];    // V: 16 keys' scales
-    int pk, pv[VU], ps;          // pages of the next step
-    const auto pages_at = [&](int k0) {
-        pk = table[min((k0 + (tid % STEP)) >> lp, last_block)];
-        for (int i = 0; i < VU; i++) pv[i] = table[min((k0 + 16 * ((tid + 256 * i) / VROWS & (PIECES - 1))) >> lp, last_block)];
-        if (QUANT) ps = table[min((k0 + 8 * (lane & (STEP / 8 - 1))) >> lp, last_block)];
-    };
-    const auto cell = [&](int page) { return ((uint64_t)(uint32_t)page * a.pg.nkv + kvh) * a.pg.cell; };
-    const auto load = [&](int k0) {
-        constexpr int KB = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;
-        const int key = k0 + (tid % STEP);
-        const uint8_t* kc = a.pg.k + cell(pk);
-#pragma unroll
-        for (int i = 0; i < KU; i++) {
-            const int blk = tid / STEP + 256 / STEP * i, at = (blk < nb ? blk : 0) * P + (key & (P - 1));
-            for (int w = 0; w < KW; w++) kr[i][w] = *(const u4*)(kc + (uint32_t)(at * KB + 16 * w));
-            if (QUANT) kd[i] = *(const uint16_t*)(kc + a.pg.scale_off + (uint32_t)(2 * at));
-        }
-#pragma unroll
-        for (int i = 0; i < VU; i++) {
-            const int u = tid + 256 * i, row = u % VROWS, key16 = k0 + 16 * (u / VROWS & (PIECES - 1));
-            const int rows = TYPE == FLLM_TYPE_Q4_0 ? hd / 2 : hd;
-            const uint8_t* vc = a.pg.v + cell(pv[i]);
-            const int at = (row < rows ? row : 0) * P + (key16 & (P - 1));
-            for (int w = 0; w < VW; w++) vr[i][w] = *(const u4*)(vc + (uint32_t)(at * (TYPE == FLLM_TYPE_F16 ? 2 : 1) + 16 * w));
-            if (QUANT) {
-                const int blk = TYPE == FLLM_TYPE_Q4_0 ? row >> 4 : row >> 5;
-                const uint8_t* sc = vc + a.pg.scale_off + (uint32_t)(2 * ((blk < nb ? blk : 0) * P + (key16 & (P - 1))));
-                vd[i][0] = *(const u4*)sc;
-                vd[i][1] = *(const u4*)(sc + 16);
+    int buf = 0, vexp = -30;  // quantised: o is in units of 2^-min(8 - vexp, 15), vexp the largest so far
+    for (int k0 = it.k0; k0 < it.k1; k0 += STEP, buf ^= DIRECT) {
+        // pages and codes past the item's end are those of its sequence's last page: loaded, never used
+        if (SRC == SRC_CODES) {
+            codes.look(k0, tile_lo, it.len);
+            ik = __builtin_amdgcn_rcpf(codes.kunit);  // a power of two: exact
+            ev = max(codes.vexp, vexp);
+            if (k0 != it.k0) lds_barrier<false>();  // the step before is read
+            codes.stage(sm.t[0][0], sm.t[0][1], ev);
+            lds_barrier<false>();
+        } else {
+            ik = ik_next;
+            ev = ev_next;
+            lds_barrier<true>();
+            if (SRC == SRC_PAGES && (k0 < tile_lo || k0 + STEP > it.len)) {
+                // zeros for what lies outside the sequence, which may be anything
+                uint16_t* v = (uint16_t*)sm.t[buf][1];
+                for (int u = tid; u < HDP * STEP; u += 256) {
+                    const int d = u / STEP, j = u % STEP;
+                    if (k0 + j < tile_lo || k0 + j >= it.len) v[v_chunk<STEP>(d, j >> 3) * 8 + (j & 7)] = 0;
+                }
+                lds_barrier<false>();
             }
         }
+        load(k0 + STEP, buf ^ 1);
+        pages_at(k0 + 2 * STEP);
+        float wunit = NP == 2 ? 16384.0f : 1.0f;  // weights times this: 2^14 leaves the low halves room
         if (QUANT) {
-            const int blk = lane / (STEP / 8), at = 2 * ((blk < nb ? blk : 0) * P + ((k0 + 8 * (lane & (STEP / 8 - 1))) & (P - 1)));
-            ks = *(const u4*)(a.pg.k + cell(ps) + a.pg.scale_off + (uint32_t)at);
-            vs = *(const u4*)(a.pg.v + cell(ps) + a.pg.scale_off + (uint32_t)at);
-        }
-    };
-    // s with largest scale * 2^s * 127 < 2^15, over the keys of the step that the sequence has
-    const auto top_scale = [&](u4 s, int k0) {
-        us2 top = {0, 0};
-        for (int i = 0; i < 4; i++) {
-            union { uint32_t u; us2 h; } c;
-            c.u = s[i] & 0x7FFF7FFFu;
-            const int64_t key = k0 + 8 * (lane & (STEP / 8 - 1)) + 2 * i;
-            if (key < tile_lo || key >= it.len) c.h.x = 0;
-            if (key + 1 < tile_lo || key + 1 >= it.len) c.h.y = 0;
-            top = __builtin_elementwise_max(top, c.h);
-        }
-        float m = (float)max((int)top.x, (int)top.y);
-        m = wave_max(m);
-        return ((int)m >> 10) - 14;  // every scale < 2^this
-    };
-
-    pages_at(it.k0);
-    load(it.k0);
-    if (it.k0 + STEP < it.k1) pages_at(it.k0 + STEP);
-    for (int k0 = it.k0; k0 < it.k1; k0 += STEP) {
-        float kunit = 1.0f, vunit = 1.0f;  // what the planes' values are multiplied by
-        if (QUANT) {
-            const int ek = __builtin_amdgcn_readfirstlane(top_scale(ks, k0)), ev = __builtin_amdgcn_readfirstlane(top_scale(vs, k0));
-            kunit = ldexpf(1.0f, min(8 - ek, 15));
-            if (ev > vexp) {  // o is in units of the largest V scale so far
-                const float down = ldexpf(1.0f, max(vexp, -7) - max(ev, -7));
-                for (int d = 0; d < HDP / 32; d++) o[d] *= down;
+            if (ev > vexp) {
+                const float fall = ldexpf(1.0f, max(vexp, -7) - max(ev, -7));
+                for (int d = 0; d < ND; d++) o[d] *= fall;
                 vexp = ev;
             }
-            vunit = ldexpf(1.0f, min(8 - vexp, 15));
+            if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
         }
-        if (k0 != it.k0) __syncthreads();  // the step before is read
-#pragma unroll
-        for (int i = 0; i < KU; i++) {
-            const int key = tid % STEP, blk = tid / STEP + 256 / STEP * i;
-            if (STEP * NB % 256 && blk >= NB) continue;
-            if (!QUANT) {
-                for (int w = 0; w < KW; w++) sm.t.k[k_chunk<HDP>(key, 4 * blk + w)] = kr[i][w];
-            } else {
-                const uint32_t d = kd[i] | kd[i] << 16;
-                for (int c = 0; c < 4; c++) {
-                    const H8 x = TYPE == FLLM_TYPE_Q8_0 ? codes8<TYPE>(kr[i][c >> 1 & (KW - 1)][2 * (c & 1)], kr[i][c >> 1 & (KW - 1)][2 * (c & 1) + 1], 0)
-                                                        : codes8<TYPE>(kr[i][0][2 * (c & 1)], kr[i][0][2 * (c & 1) + 1], c >> 1);
-                    scaled_out<KP>(x, &d, 0, kunit, &sm.t.k[k_chunk<HDP>(key, 4 * blk + c)], KCH);
-                }
-            }
-        }
-        const bool outside = k0 < tile_lo || k0 + STEP > it.len;
-#pragma unroll
-        for (int i = 0; i < VU; i++) {
-            const int u = tid + 256 * i, row = u % VROWS, piece = u / VROWS;
-            if (VROWS * PIECES % 256 && piece >= PIECES) continue;
-            if (outside)  // what lies outside the sequence may be anything: zeros instead
-                for (int j = 0; j < 16; j++) {
-                    const int64_t key = k0 + 16 * piece + j;
-                    const uint32_t keep = key >= tile_lo && key < it.len ? 0xFFFFFFFFu : j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-                    if (QUANT) vd[i][j >> 3][(j & 7) >> 1] &= keep;
-                    else vr[i][j >> 3 & (VW - 1)][(j & 7) >> 1] &= keep;
-                }
-            if (!QUANT) {
-                for (int w = 0; w < VW; w++) sm.t.v[v_chunk<STEP>(row, 2 * piece + w)] = vr[i][w];
-            } else {
-                for (int c = 0; c < 2; c++) {
-                    const uint32_t d[4] = {vd[i][c].x, vd[i][c].y, vd[i][c].z, vd[i][c].w};
-                    if (TYPE == FLLM_TYPE_Q8_0) {
-                        scaled_out<KP>(codes8<TYPE>(vr[i][0][2 * c], vr[i][0][2 * c + 1], 0), d, 1, vunit, &sm.t.v[v_chunk<STEP>(row, 2 * piece + c)], VCH);
-                    } else {
-                        const int at = (row >> 4) * 32 + (row & 15);
-                        for (int n = 0; n < 2; n++)
-                            scaled_out<KP>(codes8<TYPE>(vr[i][0][2 * c], vr[i][0][2 * c + 1], n), d, 1, vunit, &sm.t.v[v_chunk<STEP>(at + 16 * n, 2 * piece + c)], VCH);
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        if (k0 + STEP < it.k1) {
-            load(k0 + STEP);
-            if (k0 + 2 * STEP < it.k1) pages_at(k0 + 2 * STEP);
-        }
-        if (k0 >= any_hi || k0 + STEP <= any_lo) continue;  // no row of this wave sees the step
+        const u4 *kt = sm.t[buf][0], *vt = sm.t[buf][1];
 
         // S^T = K Q^T: row rho of a 32-key tile is the key with bits 2 and 3 of rho swapped, so that a lane's 8
         // registers 8 s .. are the consecutive keys 16 s + 8 h ..: the second product's operand
         f16v s[T];
         const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
 #pragma unroll
-        for (int t = 0; t < T; t++) {
+        for (int t = 0; t < T; t++)
             for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int t = 0; t < T; t++) {
                 union { u4 u; h8 h; } kf[KP];
-                for (int p = 0; p < KP; p++) kf[p].u = sm.t.k[p * KCH + k_chunk<HDP>(32 * t + krow, 2 * k + h)];
+                for (int p = 0; p < KP; p++) kf[p].u = kt[p * CH + k_chunk<HDP>(32 * t + krow, 2 * k + h)];
                 if (KP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[KP - 1].h, q[k][0], s[t], 0, 0, 0);
                 if (NP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0].h, q[k][NP - 1], s[t], 0, 0, 0);
                 s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0].h, q[k][0], s[t], 0, 0, 0);
             }
+        float us = unscale;
+        if (QUANT) us *= ik;
+        if (a.softcap > 0.0f) {
+#pragma unroll
+            for (int t = 0; t < T; t++) softcap16(s[t], us, a.softcap * kLog2e);
+            us = 1.0f;
         }
-        const float us = unscale / kunit;
-        const bool edge = k0 < all_lo || k0 + STEP > all_hi;
-        float top = kNoScore;
+        if (k0 < all_lo || k0 + STEP > all_hi)
+#pragma unroll
+            for (int t = 0; t < T; t++)
+                for (int i = 0; i < 16; i++) {
+                    const int key = k0 + 32 * t + 16 * (i >> 3) + 8 * h + (i & 7);
+                    s[t][i] = key > pos || key < low ? -INFINITY : s[t][i];
+                }
+        float top = s[0][0];
 #pragma unroll
         for (int t = 0; t < T; t++)
-            for (int i = 0; i < 16; i++) {
-                s[t][i] *= us;
-                if (a.softcap > 0.0f) s[t][i] = cap * tanh_of(s[t][i]);
-                if (edge) {
-                    const int key = k0 + 32 * t + 16 * (i >> 3) + 8 * h + (i & 7);
-                    if (key > pos || (int64_t)key <= (int64_t)pos - a.window) s[t][i] = -INFINITY;
-                }
-                top = fmaxf(top, s[t][i]);
-            }
+            for (int i = t ? 0 : 1; i < 16; i++) top = fmaxf(top, s[t][i]);
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float nm = fmaxf(mx, top), down = __builtin_amdgcn_exp2f(mx - nm);
+        const float nm = fmaxf(mx, top * us), down = __builtin_amdgcn_exp2f(mx - nm);
         mx = nm;
         float l = 0.0f;
 #pragma unroll
         for (int t = 0; t < T; t++)
             for (int i = 0; i < 16; i++) {
-                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - nm);
+                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], us, -nm));
                 l += s[t][i];
             }
         sum = sum * down + l;
-        if (__any(down != 1.0f))
-            for (int d = 0; d < HDP / 32; d++) o[d] *= down;
+        if (__any(down != 1.0f))  // the maximum seldom grows after the first steps
+            for (int d = 0; d < ND; d++) o[d] *= down;
 
         // O^T += V^T P^T
 #pragma unroll
         for (int k = 0; k < 2 * T; k++) {
             float w[8];
-            for (int i = 0; i < 8; i++) w[i] = s[k >> 1][8 * (k & 1) + i] * (NP == 2 ? 16384.0f : 1.0f);
+            for (int i = 0; i < 8; i++) w[i] = s[k >> 1][8 * (k & 1) + i] * wunit;
             h8 wf[NP];
             split8<NP>(w, wf);
 #pragma unroll
-            for (int d = 0; d < HDP / 32; d++) {
+            for (int d = 0; d < ND; d++) {
                 union { u4 u; h8 h; } vf[KP];
-                for (int p = 0; p < KP; p++) vf[p].u = sm.t.v[p * VCH + v_chunk<STEP>(32 * d + col, 2 * k + h)];
+                for (int p = 0; p < KP; p++) vf[p].u = vt[p * CH + v_chunk<STEP>(32 * d + col, 2 * k + h)];
                 if (KP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[KP - 1].h, wf[0], o[d], 0, 0, 0);
                 if (NP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0].h, wf[NP - 1], o[d], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0].h, wf[0], o[d], 0, 0, 0);
             }
         }
     }
+    if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads into LDS that nobody reads
 
     // results: o in units of 2^-(its scaling)
     sum += __shfl_xor(sum, 32);
@@ -965,22 +1136,36 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
 inline AttnArgsP attend_args(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q, const RowsView& out,
                              float scale, float softcap) {
     return AttnArgsP{pg, b.tables, nullptr, b.n_heads / pg.nkv, b.window, q, out, scale, softcap,
-                     w.part, w.part + w.part_rows * pg.nkv * pg.hd, w.cnt};
+                     w.part, w.part + w.part_rows * pg.nkv * pg.hd, w.cnt, w.images, w.image_units};
 }
 
 template <int TYPE, int HDP, int NP>
 hipError_t launch_items(AttnArgsP a, const AttnWork& w, hipStream_t st) {
+    constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
+    const auto grid = [&](int c) { return dim3((unsigned)w.n[c] * (unsigned)a.pg.nkv); };
     // the long-running tiles first
     for (int c = kAttnClasses - 1; c >= 0; c--) {
         if (w.n[c] == 0) continue;
         a.items = w.items[c];
-        const dim3 grid((unsigned)w.n[c] * (unsigned)a.pg.nkv);
-        constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
-        if (c == 0) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, QUANT ? 4 : 16>), grid, dim3(256), 0, st, a);
-        else if (c == 1) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, QUANT ? 8 : 16>), grid, dim3(256), 0, st, a);
-        else if (c == 2) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, 16>), grid, dim3(256), 0, st, a);
-        else if (c == 3) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2, 16>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP>), grid, dim3(256), 0, st, a);
+        if (c == kAttnImage) {
+            if constexpr (QUANT) {
+                hipLaunchKernelGGL((k_pages_image<TYPE, HDP, NP>), dim3((unsigned)w.n_image_items * (unsigned)a.pg.nkv), dim3(256), 0, st, a, w.image_items);
+                const hipError_t e = hipGetLastError();
+                if (e != hipSuccess) return e;
+                hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, SRC_IMAGE>), grid(c), dim3(256), 0, st, a);
+            }
+        } else if (c == kAttnMany) {
+            hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, QUANT ? SRC_CODES : SRC_PAGES>), grid(c), dim3(256), 0, st, a);
+        } else if (c == 3) {
+            if constexpr (HDP <= 128) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2, 16>), grid(c), dim3(256), 0, st, a);
+        } else if (c == 2) {
+            hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, 16>), grid(c), dim3(256), 0, st, a);
+        } else {
+            if constexpr (QUANT) {
+                if (c == 1) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, 8>), grid(c), dim3(256), 0, st, a);
+                else hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, 4>), grid(c), dim3(256), 0, st, a);
+            }
+        }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -172,20 +172,32 @@ inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, 
 struct AttnItem {
     int seq, row0, nrows, k0, k1, part, split, nsplit;
     int tok0, pos0, len, table;  // of the sequence: its first new row and that row's position, its length, its table's start
-    int pad[4];
+    int image;  // of a quantised cache's key step 0, counted in steps of kKeyStep (may be negative)
+    int pad[3];
+};
+// Key steps of a sequence that are turned into images: n from position k0 on, the first being image `image`; positions
+// outside [lo, len) count as nothing.
+struct ImageItem {
+    int table, len, lo, k0, n, image, pad[2];
 };
 constexpr int kKeyStep = 64;
-constexpr int kAttnClasses = 5;
-constexpr int kAttnTile[kAttnClasses] = {4, 8, 16, 32, 128};       // rows of a tile
-constexpr int kAttnSplit[kAttnClasses] = {128, 128, 128, 128, 32};  // most items of one
+// Classes of tiles: their rows, and the most items of one. The last class is that of sequences of many rows whose
+// keys and values are turned into images first.
+constexpr int kAttnClasses = 6, kAttnMany = 4, kAttnImage = 5;
+constexpr int kAttnTile[kAttnClasses] = {4, 8, 16, 32, 128, 128};
+constexpr int kAttnSplit[kAttnClasses] = {128, 128, 128, 128, 32, 32};
+constexpr int kImageTiles = 4;  // tiles from which images pay
+constexpr int kImageRun = 4;    // key steps of an image item
 
 struct AttnPlan {
     std::vector<AttnItem> items[kAttnClasses];  // tiles of up to kAttnTile[c] rows
     int64_t part_rows = 0;           // partial rows per kv head
+    std::vector<ImageItem> image_items;
+    int64_t images = 0;              // key steps that they make, per kv head
 };
 
 // Items of the tiles of class c of sequence i, each of at most `steps` steps of keys where the splits allow it.
-inline void attn_items(const SeqPlan& s, int i, int table, int group, int window, int c, int64_t steps,
+inline void attn_items(const SeqPlan& s, int i, int table, int image, int group, int window, int c, int64_t steps,
                        std::vector<AttnItem>* out, int64_t* part_rows) {
     const int64_t rows = (int64_t)s.n_new * group;
     const int tile = kAttnTile[c];
@@ -200,7 +212,7 @@ inline void attn_items(const SeqPlan& s, int i, int table, int group, int window
         const int used = (g1 - g0 + per - 1) / per;
         for (int k = 0; k < used; k++)
             out->push_back({i, (int)r, n, (g0 + k * per) * kKeyStep, std::min((g0 + (k + 1) * per) * kKeyStep, last + 1),
-                            (int)*part_rows, k, used, s.row0, pos0, s.len, table, {0, 0, 0, 0}});
+                            (int)*part_rows, k, used, s.row0, pos0, s.len, table, image, {0, 0, 0}});
         if (used > 1) *part_rows += (int64_t)used * n;
     }
 }
@@ -225,24 +237,26 @@ inline void attn_count(const SeqPlan& s, int group, int window, int c, int64_t s
 // The items of a batch on a device of n_cu CUs. False where they or their partial rows are too many.
 inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, bool quant, int window, int n_cu, AttnPlan* p) {
     const int group = n_heads / n_kv;
-    p->part_rows = 0;
-    constexpr int kMany = kAttnClasses - 1;
+    p->part_rows = p->images = 0;
+    p->image_items.clear();
     // the smallest tile that holds the sequence's rows; an F16 cache has no use for the two smallest (pages_attend.hpp)
     const auto class_of = [&](const SeqPlan& s) {
+        const int64_t rows = (int64_t)s.n_new * group;
         int c = quant ? 0 : 2;
-        while (c < kMany && (int64_t)s.n_new * group > kAttnTile[c]) c++;
-        return c;
+        while (c < kAttnMany && rows > kAttnTile[c]) c++;
+        if (c == 3 && head_dim > 128) c = 2;  // wide heads leave no registers for two tiles of 16: one after the other
+        return quant && rows > (kImageTiles - 1) * kAttnTile[kAttnMany] ? kAttnImage : c;
     };
     // two workgroups are resident on a CU, one of heads wider than 128
     const int64_t slots = (head_dim > 128 ? 1 : 2) * (int64_t)n_cu;
-    // Few rows: the shortest items whose workgroups all start at once (a key step for each of the four waves at
+    // Few rows: the shortest items whose workgroups all start at once (two key steps at
     // least), so that the longest one is as short as it can be.
-    int64_t few = 4, hi = kPagesMaxLength / kKeyStep + 1;
+    int64_t few = 2, hi = kPagesMaxLength / kKeyStep + 1;
     while (few < hi) {
         const int64_t mid = (few + hi) / 2;
         AttnCount n;
         for (const SeqPlan& s : b.seqs)
-            if (class_of(s) < kMany) attn_count(s, group, window, class_of(s), mid, &n);
+            if (class_of(s) < kAttnMany) attn_count(s, group, window, class_of(s), mid, &n);
         if (n.items * n_kv <= slots) hi = mid;
         else few = mid + 1;
     }
@@ -250,7 +264,7 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, b
     // about half a longest item after the mean; a part of a tile costs about 3 steps more (its partial rows).
     const auto ends = [&](int64_t steps, AttnCount* n) {
         for (const SeqPlan& s : b.seqs)
-            if (class_of(s) == kMany) attn_count(s, group, window, kMany, steps, n);
+            if (class_of(s) >= kAttnMany) attn_count(s, group, window, kAttnMany, steps, n);
         return n->items * n_kv <= slots ? (double)n->longest
                                         : (double)(n->steps + 3 * n->items) * n_kv / (double)slots + 0.5 * (double)n->longest;
     };
@@ -267,7 +281,17 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, b
     for (int i = 0; i < b.n_seqs; i++) {
         const SeqPlan& s = b.seqs[(size_t)i];
         const int c = class_of(s);
-        if (s.n_new) attn_items(s, i, i * b.tab_w, group, window, c, c == kMany ? many : few, &p->items[c], &p->part_rows);
+        int64_t image = 0;
+        if (s.n_new && c == kAttnImage) {
+            const int64_t low = std::max<int64_t>(0, (int64_t)s.len - s.n_new - window + 1);
+            const int g0 = (int)(low / kKeyStep), g1 = (s.len - 1) / kKeyStep + 1;
+            image = p->images - g0;
+            for (int g = g0; g < g1; g += kImageRun)
+                p->image_items.push_back({i * b.tab_w, s.len, (int)low, g * kKeyStep, std::min(kImageRun, g1 - g), (int)(image + g), {0, 0}});
+            p->images += g1 - g0;
+            if (p->images > INT32_MAX / 4 / n_kv) return false;
+        }
+        if (s.n_new) attn_items(s, i, i * b.tab_w, (int)image, group, window, c, c >= kAttnMany ? many : few, &p->items[c], &p->part_rows);
         if (p->part_rows > INT32_MAX / n_kv) return false;
     }
     for (auto& v : p->items) {

@@ -20,6 +20,11 @@ extern "C" int64_t plan_items(int32_t c, AttnItem* out) {
     if (out && !g_attn.items[c].empty()) memcpy(out, g_attn.items[c].data(), g_attn.items[c].size() * sizeof(AttnItem));
     return (int64_t)g_attn.items[c].size();
 }
+extern "C" int64_t plan_images(ImageItem* out, int64_t* total) {
+    if (out && !g_attn.image_items.empty()) memcpy(out, g_attn.image_items.data(), g_attn.image_items.size() * sizeof(ImageItem));
+    *total = g_attn.images;
+    return (int64_t)g_attn.image_items.size();
+}
 extern "C" int64_t plan_part_rows() { return g_attn.part_rows; }
 extern "C" void plan_sizes(int32_t* out) {
     const int32_t v[] = {g_plan.n_seqs, g_plan.n_rows, g_plan.n_pos, g_plan.tab_w, g_plan.new_blocks, g_plan.all_blocks,

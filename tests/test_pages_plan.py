@@ -12,7 +12,7 @@ import dotnetfoundryllm_amd._native as N
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 NO_WINDOW = 0x7FFFFFFF
-TILE, SPLIT = (4, 8, 16, 32, 128), (128, 128, 128, 128, 32)  # rows of the item classes, most items of a tile
+TILE, SPLIT = (4, 8, 16, 32, 128, 128), (128, 128, 128, 128, 32, 32)  # rows of the item classes, most items of a tile
 STEP = 64
 
 
@@ -22,7 +22,7 @@ def lib(tmp_path_factory):
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-shared", "-fPIC", "-o", out,
                     os.path.join(HERE, "pages_plan_shim.cpp")], check=True)
     so = C.CDLL(out)
-    so.plan_items.restype = so.plan_part_rows.restype = C.c_int64
+    so.plan_items.restype = so.plan_part_rows.restype = so.plan_images.restype = C.c_int64
     so.plan_error.restype = C.c_char_p
     return so
 
@@ -90,7 +90,7 @@ def check(so, new, length, heads, kv, window):
     parts = set()  # partial rows in use
     limit, tab_w = so.plan_part_rows(), sizes(so)["tab_w"]
     for c, list_ in enumerate(items(so)):
-        for seq, row0, nrows, k0, k1, part, split, nsplit, tok0, pos0, ln, table in list_[:, :12].tolist():
+        for seq, row0, nrows, k0, k1, part, split, nsplit, tok0, pos0, ln, table in list_[:, :12].tolist():  # noqa: E741
             assert 0 <= seq < len(new) and 0 <= row0 and 1 <= nrows <= TILE[c] and row0 + nrows <= new[seq] * group
             assert 0 <= k0 < k1 <= length[seq] and k0 % STEP == 0 and 0 <= split < nsplit <= SPLIT[c]
             assert k1 % STEP == 0 or split == nsplit - 1
@@ -102,6 +102,24 @@ def check(so, new, length, heads, kv, window):
                 assert rows[-1] < limit and not parts.intersection(rows)
                 parts.update(rows)
     assert len(parts) == limit
+    # images: every key step of the last class's items has one, made once, in order, for its own sequence
+    total = C.c_int64()
+    n = so.plan_images(None, C.byref(total))
+    a = np.zeros((n, 8), np.int32)
+    so.plan_images(a.ctypes.data_as(C.c_void_p), C.byref(total))
+    made = {}
+    for tab, ln, lo, k0, n, image, _, _ in a.tolist():
+        assert n >= 1 and k0 % STEP == 0 and k0 + n * STEP < ln + STEP and 0 <= lo < ln
+        for k in range(n):
+            assert 0 <= image + k < total.value and image + k not in made
+            made[image + k] = (tab, k0 + k * STEP, lo)
+    assert len(made) == total.value
+    for row in items(so)[-1].tolist():
+        seq, row0, k0, k1, image = row[0], row[1], row[3], row[4], row[12]
+        for k in range(k0 // STEP, -(-k1 // STEP)):
+            tab, at, lo = made[image + k]
+            assert (tab, at) == (seq * tab_w, k * STEP)
+            assert lo <= max(0, length[seq] - new[seq] + row0 // group - window + 1)
     for i, (n, ln) in enumerate(zip(new, length)):
         for r in range(n * group):
             got = sorted(seen.pop((i, r)))
