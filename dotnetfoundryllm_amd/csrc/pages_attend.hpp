@@ -188,17 +188,20 @@ __device__ __forceinline__ void softcap_n(V& s, float us, float cap) {
         s[i] *= us;
         top = fmaxf(top, fabsf(s[i]));
     }
-    const bool far = __any(top >= 0.1f);
+    if (!__any(top >= 0.1f)) {
+        for (int i = 0; i < N; i++) {
+            const float y = s[i] * s[i];
+            s[i] *= cap * fmaf(y, fmaf(y, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
+        }
+        return;
+    }
     for (int i = 0; i < N; i++) {
         const float x = s[i], y = x * x;
         const float p = x * fmaf(y, fmaf(y, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
-        s[i] = cap * p;
-        if (far) {
-            const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
-            const float q = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
-            const uint32_t big = fabsf(x) < 0.1f ? 0u : 0xFFFFFFFFu;  // selected by bits: no branch per score
-            s[i] = cap * __uint_as_float((__float_as_uint(q) & big) | (__float_as_uint(p) & ~big));
-        }
+        const float t = __builtin_amdgcn_exp2f(-2.0f * kLog2e * fabsf(x));
+        const float q = copysignf((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t), x);
+        const uint32_t big = fabsf(x) < 0.1f ? 0u : 0xFFFFFFFFu;  // selected by bits: no branch per score
+        s[i] = cap * __uint_as_float((__float_as_uint(q) & big) | (__float_as_uint(p) & ~big));
     }
 }
 template <typename V>
@@ -882,10 +885,10 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
     constexpr int CH = STEP * HDP / 8;                       // chunks of 8 halves a plane
     constexpr int DL = CH / 256;                             // loads of a plane a thread
     constexpr bool DIRECT = SRC != SRC_CODES;
-    __shared__ union {
-        u4 t[DIRECT ? 2 : 1][2][KP * CH];  // [step parity][K, V]
-        float w[kManySplit * kManyRows];
-    } sm;
+    // K, V of a step and of the next one: two objects, so that the compiler sees that reads of the one need not wait for
+    // loads into the other
+    constexpr int WCH = kManySplit * kManyRows / 4;  // the weights of joined parts, in the first one
+    __shared__ u4 lds0[2 * KP * CH > WCH ? 2 * KP * CH : WCH], lds1[DIRECT ? 2 * KP * CH : 1];
     __shared__ int s_last;
 
     const int kvh = blockIdx.x % a.pg.nkv;
@@ -909,14 +912,14 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
             pv = table[min((k0 + 8 * ((tid % (STEP / 8)) ^ v_swizzle<STEP>(tid / (STEP / 8)))) >> lp, last_block)];
         }
     };
-    const auto load = [&](int k0, int buf) {
+    const auto load = [&](int k0, u4* to) {
         if (SRC == SRC_CODES) codes.load(a.pg, kvh, k0);
         if (SRC == SRC_IMAGE) {
             k0 = min(k0, (it.k1 - 1) / STEP * STEP);  // past the item's end: its last step again
             const int64_t at = ((int64_t)it.image * (kKeyStep / STEP) + k0 / STEP) * a.pg.nkv + kvh;
             const u4* p = (const u4*)a.images + at * (2 * KP * CH) + tid;
 #pragma unroll
-            for (int i = 0; i < 2 * KP * DL; i++) to_lds(p + 256 * i, &sm.t[buf][0][256 * i + 64 * wave]);
+            for (int i = 0; i < 2 * KP * DL; i++) to_lds(p + 256 * i, to + 256 * i + 64 * wave);
             ik_next = a.image_units[2 * at];
             ev_next = (int)a.image_units[2 * at + 1];
         }
@@ -926,18 +929,18 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
             for (int i = 0; i < DL; i++) {
                 const int slot = tid + 256 * i, key = slot / (HDP / 8), c = (slot % (HDP / 8)) ^ k_swizzle<HDP>(key);
                 to_lds(a.pg.k + cell(pk[i]) + (uint32_t)((((c >> 2) < nb ? c >> 2 : 0) * P + ((k0 + key) & (P - 1))) * 64 + (c & 3) * 16),
-                       &sm.t[buf][0][256 * i + 64 * wave]);
+                       to + 256 * i + 64 * wave);
             }
             const uint8_t* vc = a.pg.v + cell(pv);
 #pragma unroll
             for (int i = 0; i < DL; i++) {
                 const int slot = tid + 256 * i, d = slot / (STEP / 8), c = (slot % (STEP / 8)) ^ v_swizzle<STEP>(d);
-                to_lds(vc + (uint32_t)((d < hd ? d : 0) * P + ((k0 + 8 * c) & (P - 1))) * 2, &sm.t[buf][1][256 * i + 64 * wave]);
+                to_lds(vc + (uint32_t)((d < hd ? d : 0) * P + ((k0 + 8 * c) & (P - 1))) * 2, to + KP * CH + 256 * i + 64 * wave);
             }
         }
     };
     pages_at(it.k0);
-    load(it.k0, 0);
+    load(it.k0, lds0);
     pages_at(it.k0 + STEP);
 
     // this lane's query
@@ -997,15 +1000,16 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
     const int w0 = it.row0 + min(32 * wave, it.nrows - 1), w1 = it.row0 + min(32 * wave + 31, it.nrows - 1);
     const int64_t all_hi = it.pos0 + w0 / a.group + 1, all_lo = (int64_t)it.pos0 + w1 / a.group - a.window + 1;
 
-    int buf = 0, vexp = -30;  // quantised: o is in units of 2^-min(8 - vexp, 15), vexp the largest so far
-    for (int k0 = it.k0; k0 < it.k1; k0 += STEP, buf ^= DIRECT) {
+    int vexp = -30;  // quantised: o is in units of 2^-min(8 - vexp, 15), vexp the largest so far
+    constexpr float wbits = NP == 2 ? 256.0f : 1.0f;  // weights (up to 2^6) times this: leaves the low halves room
+    const auto step = [&](u4* cur, u4* nxt, int k0) {
         // pages and codes past the item's end are those of its sequence's last page: loaded, never used
         if (SRC == SRC_CODES) {
             codes.look(k0, tile_lo, it.len);
             ik = __builtin_amdgcn_rcpf(codes.kunit);  // a power of two: exact
             ev = max(codes.vexp, vexp);
             if (k0 != it.k0) lds_barrier<false>();  // the step before is read
-            codes.stage(sm.t[0][0], sm.t[0][1], ev);
+            codes.stage(cur, cur + KP * CH, ev);
             lds_barrier<false>();
         } else {
             ik = ik_next;
@@ -1013,7 +1017,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
             lds_barrier<true>();
             if (SRC == SRC_PAGES && (k0 < tile_lo || k0 + STEP > it.len)) {
                 // zeros for what lies outside the sequence, which may be anything
-                uint16_t* v = (uint16_t*)sm.t[buf][1];
+                uint16_t* v = (uint16_t*)(cur + KP * CH);
                 for (int u = tid; u < HDP * STEP; u += 256) {
                     const int d = u / STEP, j = u % STEP;
                     if (k0 + j < tile_lo || k0 + j >= it.len) v[v_chunk<STEP>(d, j >> 3) * 8 + (j & 7)] = 0;
@@ -1021,18 +1025,9 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
                 lds_barrier<false>();
             }
         }
-        load(k0 + STEP, buf ^ 1);
+        load(k0 + STEP, nxt);
         pages_at(k0 + 2 * STEP);
-        float wunit = NP == 2 ? 16384.0f : 1.0f;  // weights times this: 2^14 leaves the low halves room
-        if (QUANT) {
-            if (ev > vexp) {
-                const float fall = ldexpf(1.0f, max(vexp, -7) - max(ev, -7));
-                for (int d = 0; d < ND; d++) o[d] *= fall;
-                vexp = ev;
-            }
-            if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
-        }
-        const u4 *kt = sm.t[buf][0], *vt = sm.t[buf][1];
+        const u4 *kt = cur, *vt = cur + KP * CH;
 
         // S^T = K Q^T: row rho of a 32-key tile is the key with bits 2 and 3 of rho swapped, so that a lane's 8
         // registers 8 s .. are the consecutive keys 16 s + 8 h ..: the second product's operand
@@ -1069,19 +1064,33 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
 #pragma unroll
         for (int t = 0; t < T; t++)
             for (int i = t ? 0 : 1; i < 16; i++) top = fmaxf(top, s[t][i]);
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float nm = fmaxf(mx, top * us), down = __builtin_amdgcn_exp2f(mx - nm);
-        mx = nm;
+        top = fmaxf(top, __shfl_xor(top, 32)) * us;
+        // The weights' reference follows the maximum once one is 2^6 above it: o is seldom multiplied.
+        if (__any(top > mx + 6.0f) || (QUANT && ev > vexp)) {
+            const float nm = fmaxf(mx, top);
+            float down = __builtin_amdgcn_exp2f(mx - nm);
+            mx = nm;
+            sum *= down;
+            if (QUANT && ev > vexp) {
+                down *= ldexpf(1.0f, max(vexp, -7) - max(ev, -7));
+                vexp = ev;
+            }
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= down;
+        }
+        if constexpr (HDP > 128)  // kept in accumulation registers, or every step would copy them
+#pragma unroll
+            for (int d = 0; d < ND; d++) asm volatile("" : "+a"(o[d]));
+        float wunit = wbits;
+        if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
         float l = 0.0f;
 #pragma unroll
         for (int t = 0; t < T; t++)
             for (int i = 0; i < 16; i++) {
-                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], us, -nm));
+                s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], us, -mx));
                 l += s[t][i];
             }
-        sum = sum * down + l;
-        if (__any(down != 1.0f))  // the maximum seldom grows after the first steps
-            for (int d = 0; d < ND; d++) o[d] *= down;
+        sum += l;
 
         // O^T += V^T P^T
 #pragma unroll
@@ -1099,12 +1108,19 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0].h, wf[0], o[d], 0, 0, 0);
             }
         }
+    };
+    for (int k0 = it.k0;;) {
+        step(lds0, DIRECT ? lds1 : lds0, k0);
+        if ((k0 += STEP) >= it.k1) break;
+        if (!DIRECT) continue;
+        step(lds1, lds0, k0);
+        if ((k0 += STEP) >= it.k1) break;
     }
     if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads into LDS that nobody reads
 
     // results: o in units of 2^-(its scaling)
     sum += __shfl_xor(sum, 32);
-    const float unit = ldexpf(1.0f, (QUANT ? -min(8 - vexp, 15) : 0) - (NP == 2 ? 14 : 0));
+    const float unit = ldexpf(1.0f, (QUANT ? -min(8 - vexp, 15) : 0) - (NP == 2 ? 8 : 0));
     if (it.nsplit == 1) {
         const float inv = unit / sum;
         const int64_t at = (int64_t)(it.tok0 + qtok) * a.out.ld + (int64_t)head * hd;
@@ -1130,7 +1146,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
         if (h == 0) __builtin_amdgcn_raw_buffer_store_b64(f2{mx, sum}, rml, pr * 8, 0, CPOL_SC1);
     }
     if (!last_of_tile(a.cnt + part0, it.nsplit, &s_last)) return;
-    join_parts<kManySplit>(a, it, kvh, ro, rml, sm.w);
+    join_parts<kManySplit>(a, it, kvh, ro, rml, (float*)lds0);
 }
 
 inline AttnArgsP attend_args(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q, const RowsView& out,
