@@ -180,15 +180,15 @@ __device__ __forceinline__ void split8(const float x[8], h8 out[NP]) {
 }
 
 // cap tanh(us s) of a lane's N scores. Near zero the quotient (1 - t) / (1 + t), t = exp(-2 |x|), cancels: below 1/10
-// a series to x^5 is exact to 6e-8, and where a wave's scores are all that small it is all that runs.
-template <int N, typename V>
+// a series to x^5 is exact to 6e-8, and where a wave's scores are all that small it is all that runs (SERIES).
+template <int N, bool SERIES, typename V>
 __device__ __forceinline__ void softcap_n(V& s, float us, float cap) {
     float top = 0.0f;
     for (int i = 0; i < N; i++) {
         s[i] *= us;
         top = fmaxf(top, fabsf(s[i]));
     }
-    if (!__any(top >= 0.1f)) {
+    if (SERIES && !__any(top >= 0.1f)) {
         for (int i = 0; i < N; i++) {
             const float y = s[i] * s[i];
             s[i] *= cap * fmaf(y, fmaf(y, 2.0f / 15.0f, -1.0f / 3.0f), 1.0f);
@@ -206,7 +206,7 @@ __device__ __forceinline__ void softcap_n(V& s, float us, float cap) {
 }
 template <typename V>
 __device__ __forceinline__ void softcap16(V& s, float us, float cap) {
-    softcap_n<16>(s, us, cap);
+    softcap_n<16, true>(s, us, cap);
 }
 
 __device__ __forceinline__ f4 load_row4(const RowsView& r, int64_t i) {
@@ -557,7 +557,7 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
         for (int m = 0; m < TM; m++) {
             float us = unscale[m];
             if (a.softcap > 0.0f) {
-                softcap_n<RUN>(s[m], us, a.softcap * kLog2e);
+                softcap_n<RUN, false>(s[m], us, a.softcap * kLog2e);
                 us = 1.0f;
             }
             if (edge)
