@@ -263,13 +263,13 @@ __device__ __forceinline__ bool last_of_tile(unsigned* cnt, int n, int* s_last) 
 }
 
 // Joins a tile's partial rows [split][row] (ro: head_dim floats, rml: max and sum) into out. w: MAXS floats a row.
-template <int MAXS>
+template <int MAXS, int NT = 256>
 __device__ __forceinline__ void join_parts(const AttnArgsP& a, const AttnItem& it, int kvh, __amdgpu_buffer_rsrc_t ro,
                                            __amdgpu_buffer_rsrc_t rml, float* w) {
     constexpr int N = (MAXS + 63) / 64;
     const int lane = threadIdx.x & 63, hd = a.pg.hd;
     // weights of the parts, a wave per row: exp2(m - max) / sum
-    for (int row = threadIdx.x >> 6; row < it.nrows; row += 4) {
+    for (int row = threadIdx.x >> 6; row < it.nrows; row += NT / 64) {
         float m1[N], l1[N], top = kNoScore, l = 0.0f;
         for (int i = 0; i < N; i++) {
             const int k = lane + 64 * i;
@@ -288,7 +288,7 @@ __device__ __forceinline__ void join_parts(const AttnArgsP& a, const AttnItem& i
             if (lane + 64 * i < MAXS) w[row * MAXS + lane + 64 * i] = lane + 64 * i < it.nsplit ? m1[i] * inv : 0.0f;
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < it.nrows * (hd / 4); u += 256) {
+    for (int u = threadIdx.x; u < it.nrows * (hd / 4); u += NT) {
         const int row = u / (hd / 4), d = u % (hd / 4) * 4;
         f4 acc = {0.f, 0.f, 0.f, 0.f};
         for (int k0 = 0; k0 < it.nsplit; k0 += 16) {  // 16 loads on their way; those past the end read zeros
@@ -690,7 +690,9 @@ constexpr int kManyRows = kAttnTile[kAttnClasses - 1], kManySplit = kAttnSplit[k
 
 // LDS planes of a step: K [keys][HDP], V [HDP][keys], halves in chunks of 8. Chunk c of a row lies at
 // c ^ swizzle(row), so that the 16 rows that a quarter of a wave reads cover the banks once.
-template <int HDP> __device__ __forceinline__ int k_swizzle(int key) { return HDP == 64 ? key >> 1 & 7 : key & 15; }
+template <int HDP> __device__ __forceinline__ int k_swizzle(int key) {
+    return HDP == 64 ? key >> 1 & 7 : HDP == 128 ? key & 15 : (key & 3) | (key >> 1 & 12);  // 256: k_attend_wide's rows
+}
 template <int STEP> __device__ __forceinline__ int v_swizzle(int d) { return STEP == 64 ? d >> 1 & 7 : d >> 2 & 3; }
 template <int HDP>
 __device__ __forceinline__ int k_chunk(int key, int c) {
@@ -739,12 +741,12 @@ __device__ __forceinline__ void to_lds(const void* from, u4* to) {  // lane l's 
 }
 
 // A step's codes of a quantised cache, from the pages into registers and as halves into planes.
-template <int TYPE, int HDP, int STEP, int KP>
+template <int TYPE, int HDP, int STEP, int KP, int NT = 256>
 struct Codes {
     static constexpr int NB = HDP / 32, PIECES = STEP / 16, CH = STEP * HDP / 8;
-    static constexpr int KU = (STEP * NB + 255) / 256;          // (key, block) units a thread
+    static constexpr int KU = (STEP * NB + NT - 1) / NT;        // (key, block) units a thread
     static constexpr int VROWS = TYPE == FLLM_TYPE_Q4_0 ? HDP / 2 : HDP;
-    static constexpr int VU = (VROWS * PIECES + 255) / 256;     // (row, 16 keys) units a thread
+    static constexpr int VU = (VROWS * PIECES + NT - 1) / NT;  // (row, 16 keys) units a thread
     static constexpr int KW = TYPE == FLLM_TYPE_Q8_0 ? 2 : 1;   // 16-byte words of a K unit
     u4 kr[KU][KW], vr[VU], vd[VU][2], ks, vs;  // codes, V's scales, a wave's view of all scales
     uint32_t kd[KU];                           // K's scale of the unit
@@ -755,7 +757,7 @@ struct Codes {
     __device__ __forceinline__ void pages_at(const int* table, int last_block, int lp, int k0) {
         const auto page_of = [&](int key) { return table[min(key >> lp, last_block)]; };
         pk = page_of(k0 + (int)threadIdx.x % STEP);
-        for (int i = 0; i < VU; i++) pv[i] = page_of(k0 + 16 * (((int)threadIdx.x + 256 * i) / VROWS & (PIECES - 1)));
+        for (int i = 0; i < VU; i++) pv[i] = page_of(k0 + 16 * (((int)threadIdx.x + NT * i) / VROWS & (PIECES - 1)));
         ps = page_of(k0 + 8 * ((int)threadIdx.x & (STEP / 8 - 1)));
     }
     __device__ __forceinline__ void load(const PagesView& pg, int kvh, int k0) {
@@ -766,13 +768,13 @@ struct Codes {
         const uint8_t* kc = pg.k + cell(pk);
 #pragma unroll
         for (int i = 0; i < KU; i++) {
-            const int blk = tid / STEP + 256 / STEP * i, at = (blk < nb ? blk : 0) * P + (key & (P - 1));
+            const int blk = tid / STEP + NT / STEP * i, at = (blk < nb ? blk : 0) * P + (key & (P - 1));
             for (int w = 0; w < KW; w++) kr[i][w] = *(const u4*)(kc + (uint32_t)(at * KB + 16 * w));
             kd[i] = *(const uint16_t*)(kc + pg.scale_off + (uint32_t)(2 * at));
         }
 #pragma unroll
         for (int i = 0; i < VU; i++) {
-            const int u = tid + 256 * i, row = u % VROWS, key16 = k0 + 16 * (u / VROWS & (PIECES - 1));
+            const int u = tid + NT * i, row = u % VROWS, key16 = k0 + 16 * (u / VROWS & (PIECES - 1));
             const int rows = TYPE == FLLM_TYPE_Q4_0 ? pg.hd / 2 : pg.hd, blk = TYPE == FLLM_TYPE_Q4_0 ? row >> 4 : row >> 5;
             const uint8_t* vc = pg.v + cell(pv[i]);
             vr[i] = *(const u4*)(vc + (uint32_t)((row < rows ? row : 0) * P + (key16 & (P - 1))));
@@ -806,7 +808,7 @@ struct Codes {
         if (outside)
             for (int i = 0; i < VU; i++)
                 for (int j = 0; j < 16; j++) {
-                    const int64_t key = k0 + 16 * ((tid + 256 * i) / VROWS & (PIECES - 1)) + j;
+                    const int64_t key = k0 + 16 * ((tid + NT * i) / VROWS & (PIECES - 1)) + j;
                     vd[i][j >> 3][(j & 7) >> 1] &= key >= lo && key < hi ? 0xFFFFFFFFu : j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
                 }
         const int ek = ((int)wave_max((float)max((int)tk.x, (int)tk.y)) >> 10) - 14;  // every scale < 2^ek
@@ -821,8 +823,8 @@ struct Codes {
         const h2 vu = h2{vf, vf};
 #pragma unroll
         for (int i = 0; i < KU; i++) {
-            const int key = tid % STEP, blk = tid / STEP + 256 / STEP * i;
-            if (STEP * NB % 256 && blk >= NB) continue;
+            const int key = tid % STEP, blk = tid / STEP + NT / STEP * i;
+            if (STEP * NB % NT && blk >= NB) continue;
             const uint32_t d = kd[i] | kd[i] << 16;
             for (int c = 0; c < 4; c++) {
                 const u4& w = kr[i][TYPE == FLLM_TYPE_Q8_0 ? c >> 1 & (KW - 1) : 0];
@@ -832,8 +834,8 @@ struct Codes {
         }
 #pragma unroll
         for (int i = 0; i < VU; i++) {
-            const int u = tid + 256 * i, row = u % VROWS, piece = u / VROWS;
-            if (VROWS * PIECES % 256 && piece >= PIECES) continue;
+            const int u = tid + NT * i, row = u % VROWS, piece = u / VROWS;
+            if (VROWS * PIECES % NT && piece >= PIECES) continue;
             for (int c = 0; c < 2; c++) {
                 const uint32_t d[4] = {vd[i][c].x, vd[i][c].y, vd[i][c].z, vd[i][c].w};
                 const int at = TYPE == FLLM_TYPE_Q4_0 ? (row >> 4) * 32 + (row & 15) : row;
@@ -877,7 +879,7 @@ __global__ __launch_bounds__(256) void k_pages_image(AttnArgsP a, const ImageIte
 }
 
 template <int TYPE, int HDP, int NP, int SRC>
-__global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgsP a) {
+__global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
     constexpr int KS = HDP / 16, ND = HDP / 32;
     constexpr int KP = QUANT ? NP : 1;                       // planes of K and V
@@ -1078,9 +1080,6 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
 #pragma unroll
             for (int d = 0; d < ND; d++) o[d] *= down;
         }
-        if constexpr (HDP > 128)  // kept in accumulation registers, or every step would copy them
-#pragma unroll
-            for (int d = 0; d < ND; d++) asm volatile("" : "+a"(o[d]));
         float wunit = wbits;
         if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
         float l = 0.0f;
@@ -1149,6 +1148,268 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_many(AttnArgs
     join_parts<kManySplit>(a, it, kvh, ro, rml, (float*)lds0);
 }
 
+// k_attend_wide: the same for heads wider than 128, whose q and o would take all of a 32-row wave's registers: eight
+// waves of 16 rows on the 16x16x32 products, two to a SIMD, so that one multiplies while the other reads. S^T tiles and
+// operands are k_attend_few's: a lane holds the keys 8 g .. + 8 of a step of 32.
+template <int TYPE, int NP, int SRC>
+__global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
+    constexpr int HDP = 256, NT = 512;
+    constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
+    constexpr int NB = HDP / 32, ND = HDP / 16;
+    constexpr int KP = QUANT ? NP : 1;                       // planes of K and V
+    constexpr int STEP = many_step(HDP, NP);                 // keys a step
+    static_assert(STEP == 32, "two tiles of 16 keys");
+    constexpr int CH = STEP * HDP / 8;                       // chunks of 8 halves a plane
+    constexpr int DL = CH / NT;                              // loads of a plane a thread
+    constexpr bool DIRECT = SRC != SRC_CODES;
+    // K, V of a step and of the next one: two objects, so that the compiler sees that reads of the one need not wait for
+    // loads into the other
+    constexpr int WCH = kManySplit * kManyRows / 4;  // the weights of joined parts, in the first one
+    __shared__ u4 lds0[2 * KP * CH > WCH ? 2 * KP * CH : WCH], lds1[DIRECT ? 2 * KP * CH : 1];
+    __shared__ int s_last;
+
+    const int kvh = blockIdx.x % a.pg.nkv;
+    const AttnItem it = a.items[blockIdx.x / a.pg.nkv];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
+    const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
+    const int* table = a.tables + it.table;
+    const int last_block = (it.len - 1) >> lp;
+    const int64_t tile_lo = (int64_t)it.pos0 + it.row0 / a.group + 1 - a.window;  // the first key that any row sees
+
+    // ---- the steps on their way; pages of a step are looked up a step before its loads
+    Codes<QUANT ? TYPE : (int)FLLM_TYPE_Q8_0, HDP, STEP, KP, NT> codes;  // SRC_CODES
+    int pk[DL], pv;                                                  // SRC_PAGES
+    float ik = 1.0f, ik_next = 1.0f;                                 // quantised: 1 / kunit of this step and the next
+    int ev = 0, ev_next = 0;                                         // and vexp
+    const auto pages_at = [&](int k0) {
+        if (SRC == SRC_CODES) codes.pages_at(table, last_block, lp, k0);
+        if (SRC == SRC_PAGES) {
+            for (int i = 0; i < DL; i++) pk[i] = table[min((k0 + (tid + NT * i) / (HDP / 8)) >> lp, last_block)];
+            // the chunk that this thread's slots hold is the same in each: NT slots are a multiple of 16 rows
+            pv = table[min((k0 + 8 * ((tid % (STEP / 8)) ^ v_swizzle<STEP>(tid / (STEP / 8)))) >> lp, last_block)];
+        }
+    };
+    const auto load = [&](int k0, u4* to) {
+        if (SRC == SRC_CODES) codes.load(a.pg, kvh, k0);
+        if (SRC == SRC_IMAGE) {
+            k0 = min(k0, (it.k1 - 1) / STEP * STEP);  // past the item's end: its last step again
+            const int64_t at = ((int64_t)it.image * (kKeyStep / STEP) + k0 / STEP) * a.pg.nkv + kvh;
+            const u4* p = (const u4*)a.images + at * (2 * KP * CH) + tid;
+#pragma unroll
+            for (int i = 0; i < 2 * KP * DL; i++) to_lds(p + NT * i, to + NT * i + 64 * wave);
+            ik_next = a.image_units[2 * at];
+            ev_next = (int)a.image_units[2 * at + 1];
+        }
+        if (SRC == SRC_PAGES) {  // slot by slot of the LDS image
+            const auto cell = [&](int page) { return ((uint64_t)(uint32_t)page * a.pg.nkv + kvh) * a.pg.cell; };
+#pragma unroll
+            for (int i = 0; i < DL; i++) {
+                const int slot = tid + NT * i, key = slot / (HDP / 8), c = (slot % (HDP / 8)) ^ k_swizzle<HDP>(key);
+                to_lds(a.pg.k + cell(pk[i]) + (uint32_t)((((c >> 2) < nb ? c >> 2 : 0) * P + ((k0 + key) & (P - 1))) * 64 + (c & 3) * 16),
+                       to + NT * i + 64 * wave);
+            }
+            const uint8_t* vc = a.pg.v + cell(pv);
+#pragma unroll
+            for (int i = 0; i < DL; i++) {
+                const int slot = tid + NT * i, d = slot / (STEP / 8), c = (slot % (STEP / 8)) ^ v_swizzle<STEP>(d);
+                to_lds(vc + (uint32_t)((d < hd ? d : 0) * P + ((k0 + 8 * c) & (P - 1))) * 2, to + KP * CH + NT * i + 64 * wave);
+            }
+        }
+    };
+    pages_at(it.k0);
+    load(it.k0, lds0);
+    pages_at(it.k0 + STEP);
+
+    // this lane's query
+    const int r = 16 * wave + col;
+    const bool live = r < it.nrows;
+    const int qrow = it.row0 + (live ? r : 0), qtok = qrow / a.group, head = kvh * a.group + qrow % a.group;
+    const int pos = live ? it.pos0 + qtok : -1, low = (int)max((int64_t)pos - a.window + 1, (int64_t)INT_MIN);
+    float unscale;
+    h8 q[NB][NP];
+    {
+        const int64_t at = (int64_t)(it.tok0 + qtok) * a.q.ld + (int64_t)head * hd;
+        float x[NB][8], top = 0.0f;
+        if (a.q.type == FLLM_TYPE_F32) {
+#pragma unroll
+            for (int c = 0; c < NB; c++) {
+                const int d = 32 * c + 8 * g;
+                const float* p = (const float*)a.q.p + at + (d < hd ? d : 0);
+                const f4 u = *(const f4*)p, v = *(const f4*)(p + 4);
+                for (int i = 0; i < 4; i++) x[c][i] = u[i], x[c][4 + i] = v[i];
+            }
+        } else {
+            const bool f16 = a.q.type == FLLM_TYPE_F16;
+#pragma unroll
+            for (int c = 0; c < NB; c++) {
+                const int d = 32 * c + 8 * g;
+                const u4 u = *(const u4*)(a.q.p + 2 * (at + (d < hd ? d : 0)));
+                for (int i = 0; i < 4; i++) {
+                    union { uint32_t u; h2 h; } w;
+                    w.u = u[i];
+                    x[c][2 * i] = f16 ? (float)w.h.x : __uint_as_float(u[i] << 16);
+                    x[c][2 * i + 1] = f16 ? (float)w.h.y : __uint_as_float(u[i] & 0xFFFF0000u);
+                }
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < NB; c++)
+            for (int i = 0; i < 8; i++) {
+                if (!live || 32 * c + 8 * g >= hd) x[c][i] = 0.0f;
+                top = fmaxf(top, fabsf(x[c][i]));
+            }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const int e = row_exponent(top);
+        const float up = ldexpf(scale_sign(a.scale), e);
+#pragma unroll
+        for (int c = 0; c < NB; c++) {
+            for (int i = 0; i < 8; i++) x[c][i] *= up;
+            split8<NP>(x[c], q[c]);
+        }
+        unscale = scale_size(a.scale, e, a.softcap);
+    }
+
+    f4 o[ND];
+    for (int d = 0; d < ND; d++) o[d] = f4{0.f, 0.f, 0.f, 0.f};
+    float mx = kNoScore, sum = 0.0f;
+    // keys that every row of the wave sees: [all_lo, all_hi)
+    const int w0 = it.row0 + min(16 * wave, it.nrows - 1), w1 = it.row0 + min(16 * wave + 15, it.nrows - 1);
+    const int64_t all_hi = it.pos0 + w0 / a.group + 1, all_lo = (int64_t)it.pos0 + w1 / a.group - a.window + 1;
+
+    int vexp = -30;  // quantised: o is in units of 2^-min(8 - vexp, 15), vexp the largest so far
+    constexpr float wbits = NP == 2 ? 256.0f : 1.0f;  // weights (up to 2^6) times this: leaves the low halves room
+    const auto step = [&](u4* cur, u4* nxt, int k0) {
+        // pages and codes past the item's end are those of its sequence's last page: loaded, never used
+        if (SRC == SRC_CODES) {
+            codes.look(k0, tile_lo, it.len);
+            ik = __builtin_amdgcn_rcpf(codes.kunit);  // a power of two: exact
+            ev = max(codes.vexp, vexp);
+            if (k0 != it.k0) lds_barrier<false>();  // the step before is read
+            codes.stage(cur, cur + KP * CH, ev);
+            lds_barrier<false>();
+        } else {
+            ik = ik_next;
+            ev = ev_next;
+            lds_barrier<true>();
+            if (SRC == SRC_PAGES && (k0 < tile_lo || k0 + STEP > it.len)) {
+                // zeros for what lies outside the sequence, which may be anything
+                uint16_t* v = (uint16_t*)(cur + KP * CH);
+                for (int u = tid; u < HDP * STEP; u += NT) {
+                    const int d = u / STEP, j = u % STEP;
+                    if (k0 + j < tile_lo || k0 + j >= it.len) v[v_chunk<STEP>(d, j >> 3) * 8 + (j & 7)] = 0;
+                }
+                lds_barrier<false>();
+            }
+        }
+        load(k0 + STEP, nxt);
+        pages_at(k0 + 2 * STEP);
+        const u4 *kt = cur, *vt = cur + KP * CH;
+
+        // S^T = K Q^T: row rho of tile t is key 8 (rho >> 2) + 4 t + (rho & 3); high and low products apart, so that there
+        // are four chains of them
+        f4 hi[2], lo[2];
+#pragma unroll
+        for (int t = 0; t < 2; t++) hi[t] = lo[t] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NB; c++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                union { u4 u; h8 h; } kf[KP];
+                for (int p = 0; p < KP; p++) kf[p].u = kt[p * CH + k_chunk<HDP>(8 * (col >> 2) + 4 * t + (col & 3), 4 * c + g)];
+                hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0].h, q[c][0], hi[t], 0, 0, 0);
+                if (NP == 2) lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0].h, q[c][NP - 1], lo[t], 0, 0, 0);
+                if (KP == 2) lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[KP - 1].h, q[c][0], lo[t], 0, 0, 0);
+            }
+        float s[8];
+        for (int i = 0; i < 8; i++) s[i] = NP == 2 ? hi[i >> 2][i & 3] + lo[i >> 2][i & 3] : hi[i >> 2][i & 3];
+        float us = unscale;
+        if (QUANT) us *= ik;
+        if (a.softcap > 0.0f) {
+            softcap_n<8, true>(s, us, a.softcap * kLog2e);
+            us = 1.0f;
+        }
+        if (k0 < all_lo || k0 + STEP > all_hi)
+            for (int i = 0; i < 8; i++) {
+                const int key = k0 + 8 * g + i;
+                s[i] = key > pos || key < low ? -INFINITY : s[i];
+            }
+        float top = s[0];
+        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32)) * us;
+        // The weights' reference follows the maximum once one is 2^6 above it: o is seldom multiplied.
+        if (__any(top > mx + 6.0f) || (QUANT && ev > vexp)) {
+            const float nm = fmaxf(mx, top);
+            float down = __builtin_amdgcn_exp2f(mx - nm);
+            mx = nm;
+            sum *= down;
+            if (QUANT && ev > vexp) {
+                down *= ldexpf(1.0f, max(vexp, -7) - max(ev, -7));
+                vexp = ev;
+            }
+#pragma unroll
+            for (int d = 0; d < ND; d++) o[d] *= down;
+        }
+        float wunit = wbits;
+        if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
+        float w[8], l = 0.0f;
+        for (int i = 0; i < 8; i++) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], us, -mx));
+            l += s[i];
+            w[i] = s[i] * wunit;
+        }
+        sum += l;
+        h8 wf[NP];
+        split8<NP>(w, wf);
+
+        // O^T += V^T P^T
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            union { u4 u; h8 h; } vf[KP];
+            for (int p = 0; p < KP; p++) vf[p].u = vt[p * CH + v_chunk<STEP>(16 * d + col, g)];
+            if (KP == 2) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[KP - 1].h, wf[0], o[d], 0, 0, 0);
+            if (NP == 2) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[0].h, wf[NP - 1], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[0].h, wf[0], o[d], 0, 0, 0);
+        }
+    };
+    for (int k0 = it.k0;;) {
+        step(lds0, DIRECT ? lds1 : lds0, k0);
+        if ((k0 += STEP) >= it.k1) break;
+        if (!DIRECT) continue;
+        step(lds1, lds0, k0);
+        if ((k0 += STEP) >= it.k1) break;
+    }
+    if (DIRECT) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // loads into LDS that nobody reads
+
+    // results: o in units of 2^-(its scaling)
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    const float unit = ldexpf(1.0f, (QUANT ? -min(8 - vexp, 15) : 0) - (NP == 2 ? 8 : 0));
+    if (it.nsplit == 1) {
+        const float inv = unit / sum;
+        const int64_t at = (int64_t)(it.tok0 + qtok) * a.out.ld + (int64_t)head * hd;
+        if (live)
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                if (16 * d < hd) store_row4(a.out, at + 16 * d + 4 * g, o[d] * inv);
+        return;
+    }
+    const int64_t part0 = (int64_t)it.part * a.pg.nkv + (int64_t)kvh * it.nsplit * it.nrows;
+    const uint32_t n_part = (uint32_t)(it.nsplit * it.nrows);
+    const __amdgpu_buffer_rsrc_t ro = wt_rsrc(a.part_o + part0 * hd, n_part * hd * 4);
+    const __amdgpu_buffer_rsrc_t rml = wt_rsrc(a.part_ml + 2 * part0, n_part * 8);
+    if (live) {
+        const uint32_t pr = (uint32_t)(it.split * it.nrows + r);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            if (16 * d < hd) __builtin_amdgcn_raw_buffer_store_b128(o[d] * unit, ro, (pr * hd + 16 * d + 4 * g) * 4, 0, CPOL_SC1);
+        if (g == 0) __builtin_amdgcn_raw_buffer_store_b64(f2{mx, sum}, rml, pr * 8, 0, CPOL_SC1);
+    }
+    if (!last_of_tile(a.cnt + part0, it.nsplit, &s_last)) return;
+    join_parts<kManySplit, NT>(a, it, kvh, ro, rml, (float*)lds0);
+}
+
 inline AttnArgsP attend_args(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q, const RowsView& out,
                              float scale, float softcap) {
     return AttnArgsP{pg, b.tables, nullptr, b.n_heads / pg.nkv, b.window, q, out, scale, softcap,
@@ -1168,10 +1429,12 @@ hipError_t launch_items(AttnArgsP a, const AttnWork& w, hipStream_t st) {
                 hipLaunchKernelGGL((k_pages_image<TYPE, HDP, NP>), dim3((unsigned)w.n_image_items * (unsigned)a.pg.nkv), dim3(256), 0, st, a, w.image_items);
                 const hipError_t e = hipGetLastError();
                 if (e != hipSuccess) return e;
-                hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, SRC_IMAGE>), grid(c), dim3(256), 0, st, a);
+                if constexpr (HDP > 128) hipLaunchKernelGGL((k_attend_wide<TYPE, NP, SRC_IMAGE>), grid(c), dim3(512), 0, st, a);
+                else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, SRC_IMAGE>), grid(c), dim3(256), 0, st, a);
             }
         } else if (c == kAttnMany) {
-            hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, QUANT ? SRC_CODES : SRC_PAGES>), grid(c), dim3(256), 0, st, a);
+            if constexpr (HDP > 128) hipLaunchKernelGGL((k_attend_wide<TYPE, NP, QUANT ? SRC_CODES : SRC_PAGES>), grid(c), dim3(512), 0, st, a);
+            else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, QUANT ? SRC_CODES : SRC_PAGES>), grid(c), dim3(256), 0, st, a);
         } else if (c == 3) {
             if constexpr (HDP <= 128) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2, 16>), grid(c), dim3(256), 0, st, a);
         } else if (c == 2) {
