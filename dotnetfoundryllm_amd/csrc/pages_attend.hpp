@@ -22,6 +22,8 @@
 // attn_body.hpp, so no second launch).
 #pragma once
 
+#include <type_traits>
+
 #include "attn_body.hpp"
 #include "pages.hpp"
 #include "pages_plan.hpp"
@@ -167,6 +169,15 @@ __device__ __forceinline__ void split4(const f4 x, h2 out[NP][2]) {
         else split2(x[2 * i], x[2 * i + 1], &out[0][i], &out[NP - 1][i]);
     }
 }
+// x + the sum of 8 halves: what the product with V weighs with, where the weights are rounded to one half
+__device__ __forceinline__ float add_halves(h8 w, float x) {
+    H8 h;
+    h.v = w;
+    const h2 one = {(_Float16)1.0f, (_Float16)1.0f};
+    for (int i = 0; i < 4; i++) x = __builtin_amdgcn_fdot2(h.p[i], one, x, false);
+    return x;
+}
+
 template <int NP>
 __device__ __forceinline__ void split8(const float x[8], h8 out[NP]) {
     h2 a[NP][2], b[NP][2];
@@ -315,7 +326,7 @@ __device__ __forceinline__ void join_parts(const AttnArgsP& a, const AttnItem& i
 // multiplied by its own blocks' scales, and of each product with V only the columns whose group the block belongs
 // to are kept. A lane then loads and applies BPS scales a key in place of NB.
 template <int TYPE, int HDP, int NP, int TM, int RC>
-__global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ? 1 : 2, HDP > 128 ? 1 : 2))) void k_attend_few(AttnArgsP a) {
     constexpr int NB = HDP / 32, ND = HDP / 16;      // blocks of 32 elements, tiles of 16
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
     // runs of 32 keys a step: 16 bytes of V a lane, 8 where registers are short
@@ -679,12 +690,13 @@ __global__ __launch_bounds__(256, HDP > 128 ? 1 : 2) void k_attend_few(AttnArgsP
 // Where the halves come from (SRC):
 //   SRC_PAGES   an F16 cache's pages, straight to LDS (16 bytes a lane; the LDS image is made by which address a
 //               lane loads), two steps deep: the next step arrives while one is multiplied
+//   SRC_PARTS   the same from pages shorter than a step: every lane looks up its own
 //   SRC_IMAGE   LDS images that k_pages_image made of a quantised cache's pages before, once for all tiles of a
 //               sequence, likewise
 //   SRC_CODES   a quantised cache's codes, turned into halves by every workgroup: for sequences of few tiles, where
 //               writing and reading images costs more than the turning
 typedef float f16v __attribute__((ext_vector_type(16)));
-enum { SRC_PAGES, SRC_IMAGE, SRC_CODES };
+enum { SRC_PAGES, SRC_PARTS, SRC_IMAGE, SRC_CODES };
 
 constexpr int kManyRows = kAttnTile[kAttnClasses - 1], kManySplit = kAttnSplit[kAttnClasses - 1];
 
@@ -757,6 +769,7 @@ struct Codes {
     __device__ __forceinline__ void pages_at(const int* table, int last_block, int lp, int k0) {
         const auto page_of = [&](int key) { return table[min(key >> lp, last_block)]; };
         pk = page_of(k0 + (int)threadIdx.x % STEP);
+#pragma unroll
         for (int i = 0; i < VU; i++) pv[i] = page_of(k0 + 16 * (((int)threadIdx.x + NT * i) / VROWS & (PIECES - 1)));
         ps = page_of(k0 + 8 * ((int)threadIdx.x & (STEP / 8 - 1)));
     }
@@ -846,6 +859,79 @@ struct Codes {
     }
 };
 
+// A step of an F16 cache's pages to LDS, slot by slot of the LDS image. Where a page holds whole steps (WHOLE) the page
+// is the same for all threads; a thread's offsets within the cells never change.
+template <int HDP, int STEP, int NT, bool WHOLE>
+struct PageLoads {
+    static constexpr int CH = STEP * HDP / 8, DL = CH / NT;  // chunks of a plane, loads of one a thread
+    uint32_t ko[DL], vo[DL];  // offsets of this thread's slots of K and V in their cells, for position 0 of the step
+    int pk[WHOLE ? 1 : DL], pv;  // pages of the next step
+
+    __device__ __forceinline__ void start(const PagesView& pg) {
+        const int tid = threadIdx.x, P = 1 << pg.page_log2, nb = pg.hd >> 5;
+#pragma unroll
+        for (int i = 0; i < DL; i++) {
+            const int slot = tid + NT * i, key = slot / (HDP / 8), c = (slot % (HDP / 8)) ^ k_swizzle<HDP>(key);
+            ko[i] = (uint32_t)((((c >> 2) < nb ? c >> 2 : 0) * P + (key & (P - 1))) * 64 + (c & 3) * 16);
+            const int d = slot / (STEP / 8), b = (slot % (STEP / 8)) ^ v_swizzle<STEP>(d);
+            vo[i] = (uint32_t)(((d < pg.hd ? d : 0) * P + (8 * b & (P - 1))) * 2);
+        }
+    }
+    __device__ __forceinline__ void pages_at(const int* table, int last_block, int lp, int k0) {
+        const int tid = threadIdx.x;
+        if constexpr (WHOLE) {  // the constant address space: a scalar load also beside stores and barriers
+            pk[0] = ((const __attribute__((address_space(4))) int*)table)[__builtin_amdgcn_readfirstlane(min(k0 >> lp, last_block))];
+        } else {
+#pragma unroll
+            for (int i = 0; i < DL; i++) pk[i] = table[min((k0 + (tid + NT * i) / (HDP / 8)) >> lp, last_block)];
+            // the chunk that this thread's slots of V hold is the same in each: NT slots are a multiple of 16 rows
+            pv = table[min((k0 + 8 * ((tid % (STEP / 8)) ^ v_swizzle<STEP>(tid / (STEP / 8)))) >> lp, last_block)];
+        }
+    }
+    __device__ __forceinline__ void load(const PagesView& pg, int kvh, int k0, u4* k, u4* v) const {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        const auto cell = [&](int p) { return ((uint64_t)(uint32_t)p * pg.nkv + kvh) * pg.cell; };
+        if constexpr (WHOLE) {
+            const int at = k0 & ((1 << pg.page_log2) - 1);
+            const uint64_t c = cell(pk[0]);
+            const uint8_t *kp = pg.k + c + at * 64, *vp = pg.v + c + at * 2;
+#pragma unroll
+            for (int i = 0; i < DL; i++) to_lds(kp + ko[i], k + NT * i + 64 * wave);
+#pragma unroll
+            for (int i = 0; i < DL; i++) to_lds(vp + vo[i], v + NT * i + 64 * wave);
+        } else {
+#pragma unroll
+            for (int i = 0; i < DL; i++) to_lds(pg.k + cell(pk[i]) + ko[i], k + NT * i + 64 * wave);
+            const uint8_t* vp = pg.v + cell(pv);
+#pragma unroll
+            for (int i = 0; i < DL; i++) to_lds(vp + vo[i], v + NT * i + 64 * wave);
+        }
+    }
+};
+
+// V of a step in LDS: zeros at the positions outside [lo, hi).
+template <int HDP, int STEP, int NT>
+__device__ __forceinline__ void zero_outside(u4* v, int k0, int64_t lo, int64_t hi) {
+#pragma unroll 1
+    for (int u = threadIdx.x; u < HDP * STEP / 8; u += NT) {
+        const int d = u / (STEP / 8), c = u % (STEP / 8);
+        u4 x = v[v_chunk<STEP>(d, c)];
+        for (int j = 0; j < 8; j++) {
+            const int64_t key = k0 + 8 * c + j;
+            if (key < lo || key >= hi) x[j >> 1] &= j & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+        v[v_chunk<STEP>(d, c)] = x;
+    }
+}
+
+// An image to LDS.
+template <int CHUNKS, int NT>
+__device__ __forceinline__ void image_to_lds(const u4* image, u4* to) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < CHUNKS / NT; i++) to_lds((const uint8_t*)(image + NT * i) + (uint32_t)threadIdx.x * 16, to + NT * i + 64 * wave);
+}
+
 // Images of a quantised cache's steps: [step][kv head] of the planes K, V as they lie in LDS, and of (1 / kunit, vexp).
 template <int TYPE, int HDP, int NP>
 __global__ __launch_bounds__(256) void k_pages_image(AttnArgsP a, const ImageItem* items) {
@@ -879,13 +965,12 @@ __global__ __launch_bounds__(256) void k_pages_image(AttnArgsP a, const ImageIte
 }
 
 template <int TYPE, int HDP, int NP, int SRC>
-__global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_many(AttnArgsP a) {
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
     constexpr int KS = HDP / 16, ND = HDP / 32;
     constexpr int KP = QUANT ? NP : 1;                       // planes of K and V
     constexpr int STEP = many_step(HDP, NP), T = STEP / 32;  // keys a step, tiles of 32
     constexpr int CH = STEP * HDP / 8;                       // chunks of 8 halves a plane
-    constexpr int DL = CH / 256;                             // loads of a plane a thread
     constexpr bool DIRECT = SRC != SRC_CODES;
     // K, V of a step and of the next one: two objects, so that the compiler sees that reads of the one need not wait for
     // loads into the other
@@ -896,51 +981,32 @@ __global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
     const int kvh = blockIdx.x % a.pg.nkv;
     const AttnItem it = a.items[blockIdx.x / a.pg.nkv];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 31, h = lane >> 5;
-    const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
+    const int hd = a.pg.hd, lp = a.pg.page_log2;
     const int* table = a.tables + it.table;
     const int last_block = (it.len - 1) >> lp;
     const int64_t tile_lo = (int64_t)it.pos0 + it.row0 / a.group + 1 - a.window;  // the first key that any row sees
 
     // ---- the steps on their way; pages of a step are looked up a step before its loads
     Codes<QUANT ? TYPE : (int)FLLM_TYPE_Q8_0, HDP, STEP, KP> codes;  // SRC_CODES
-    int pk[DL], pv;                                                  // SRC_PAGES
+    PageLoads<HDP, STEP, 256, SRC == SRC_PAGES> direct;              // SRC_PAGES, SRC_PARTS
     float ik = 1.0f, ik_next = 1.0f;                                 // quantised: 1 / kunit of this step and the next
     int ev = 0, ev_next = 0;                                         // and vexp
     const auto pages_at = [&](int k0) {
         if (SRC == SRC_CODES) codes.pages_at(table, last_block, lp, k0);
-        if (SRC == SRC_PAGES) {
-            for (int i = 0; i < DL; i++) pk[i] = table[min((k0 + (tid + 256 * i) / (HDP / 8)) >> lp, last_block)];
-            // the chunk that this thread's slots hold is the same in each: 256 slots are a multiple of 16 rows
-            pv = table[min((k0 + 8 * ((tid % (STEP / 8)) ^ v_swizzle<STEP>(tid / (STEP / 8)))) >> lp, last_block)];
-        }
+        if (SRC <= SRC_PARTS) direct.pages_at(table, last_block, lp, k0);
     };
     const auto load = [&](int k0, u4* to) {
         if (SRC == SRC_CODES) codes.load(a.pg, kvh, k0);
         if (SRC == SRC_IMAGE) {
             k0 = min(k0, (it.k1 - 1) / STEP * STEP);  // past the item's end: its last step again
             const int64_t at = ((int64_t)it.image * (kKeyStep / STEP) + k0 / STEP) * a.pg.nkv + kvh;
-            const u4* p = (const u4*)a.images + at * (2 * KP * CH) + tid;
-#pragma unroll
-            for (int i = 0; i < 2 * KP * DL; i++) to_lds(p + 256 * i, to + 256 * i + 64 * wave);
+            image_to_lds<2 * KP * CH, 256>((const u4*)a.images + at * (2 * KP * CH), to);
             ik_next = a.image_units[2 * at];
             ev_next = (int)a.image_units[2 * at + 1];
         }
-        if (SRC == SRC_PAGES) {  // slot by slot of the LDS image
-            const auto cell = [&](int page) { return ((uint64_t)(uint32_t)page * a.pg.nkv + kvh) * a.pg.cell; };
-#pragma unroll
-            for (int i = 0; i < DL; i++) {
-                const int slot = tid + 256 * i, key = slot / (HDP / 8), c = (slot % (HDP / 8)) ^ k_swizzle<HDP>(key);
-                to_lds(a.pg.k + cell(pk[i]) + (uint32_t)((((c >> 2) < nb ? c >> 2 : 0) * P + ((k0 + key) & (P - 1))) * 64 + (c & 3) * 16),
-                       to + 256 * i + 64 * wave);
-            }
-            const uint8_t* vc = a.pg.v + cell(pv);
-#pragma unroll
-            for (int i = 0; i < DL; i++) {
-                const int slot = tid + 256 * i, d = slot / (STEP / 8), c = (slot % (STEP / 8)) ^ v_swizzle<STEP>(d);
-                to_lds(vc + (uint32_t)((d < hd ? d : 0) * P + ((k0 + 8 * c) & (P - 1))) * 2, to + KP * CH + 256 * i + 64 * wave);
-            }
-        }
+        if (SRC <= SRC_PARTS) direct.load(a.pg, kvh, k0, to, to + KP * CH);
     };
+    if (SRC <= SRC_PARTS) direct.start(a.pg);
     pages_at(it.k0);
     load(it.k0, lds0);
     pages_at(it.k0 + STEP);
@@ -1004,6 +1070,11 @@ __global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
 
     int vexp = -30;  // quantised: o is in units of 2^-min(8 - vexp, 15), vexp the largest so far
     constexpr float wbits = NP == 2 ? 256.0f : 1.0f;  // weights (up to 2^6) times this: leaves the low halves room
+    constexpr bool HALF_SUM = NP == 1 && SRC != SRC_IMAGE;  // an image's weights carry its units, and may vanish in them
+    // This lane's operands in a plane: K row krow of a tile, V row col, the chunk 2 k + h of each; chunk bits of k are
+    // apart from the row's, so that they are one exclusive or away.
+    const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
+    const int k_at0 = k_chunk<HDP>(krow, h) * 16, v_at0 = v_chunk<STEP>(col, h) * 16;
     const auto step = [&](u4* cur, u4* nxt, int k0) {
         // pages and codes past the item's end are those of its sequence's last page: loaded, never used
         if (SRC == SRC_CODES) {
@@ -1017,37 +1088,43 @@ __global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
             ik = ik_next;
             ev = ev_next;
             lds_barrier<true>();
-            if (SRC == SRC_PAGES && (k0 < tile_lo || k0 + STEP > it.len)) {
+            if (SRC <= SRC_PARTS && (k0 < tile_lo || k0 + STEP > it.len)) {
                 // zeros for what lies outside the sequence, which may be anything
-                uint16_t* v = (uint16_t*)(cur + KP * CH);
-                for (int u = tid; u < HDP * STEP; u += 256) {
-                    const int d = u / STEP, j = u % STEP;
-                    if (k0 + j < tile_lo || k0 + j >= it.len) v[v_chunk<STEP>(d, j >> 3) * 8 + (j & 7)] = 0;
-                }
+                zero_outside<HDP, STEP, 256>(cur + KP * CH, k0, tile_lo, it.len);
                 lds_barrier<false>();
             }
         }
         load(k0 + STEP, nxt);
         pages_at(k0 + 2 * STEP);
         const u4 *kt = cur, *vt = cur + KP * CH;
+        int k_at = k_at0, v_at = v_at0;
+        asm volatile("" : "+v"(k_at), "+v"(v_at));  // or each address would be kept in a register across the steps
 
         // S^T = K Q^T: row rho of a 32-key tile is the key with bits 2 and 3 of rho swapped, so that a lane's 8
         // registers 8 s .. are the consecutive keys 16 s + 8 h ..: the second product's operand
         f16v s[T];
-        const int krow = (col & 19) | (col & 4) << 1 | (col & 8) >> 1;
 #pragma unroll
         for (int t = 0; t < T; t++)
             for (int i = 0; i < 16; i++) s[t][i] = 0.0f;
+        union { u4 u; h8 h; } kf[2][T][KP];  // operands of this product and the next
+        const auto k_load = [&](int k) {
 #pragma unroll
-        for (int k = 0; k < KS; k++)
+            for (int t = 0; t < T; t++)
+                for (int p = 0; p < KP; p++)
+                    kf[k & 1][t][p].u = *(const u4*)((const uint8_t*)(kt + p * CH + 32 * t * (HDP / 8)) + (k_at ^ 32 * k));
+        };
+        k_load(0);
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            if (k + 1 < KS) k_load(k + 1);
+            __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead of this product
 #pragma unroll
             for (int t = 0; t < T; t++) {
-                union { u4 u; h8 h; } kf[KP];
-                for (int p = 0; p < KP; p++) kf[p].u = kt[p * CH + k_chunk<HDP>(32 * t + krow, 2 * k + h)];
-                if (KP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[KP - 1].h, q[k][0], s[t], 0, 0, 0);
-                if (NP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0].h, q[k][NP - 1], s[t], 0, 0, 0);
-                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[0].h, q[k][0], s[t], 0, 0, 0);
+                if (KP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k & 1][t][KP - 1].h, q[k][0], s[t], 0, 0, 0);
+                if (NP == 2) s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k & 1][t][0].h, q[k][NP - 1], s[t], 0, 0, 0);
+                s[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k & 1][t][0].h, q[k][0], s[t], 0, 0, 0);
             }
+        }
         float us = unscale;
         if (QUANT) us *= ik;
         if (a.softcap > 0.0f) {
@@ -1055,12 +1132,13 @@ __global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
             for (int t = 0; t < T; t++) softcap16(s[t], us, a.softcap * kLog2e);
             us = 1.0f;
         }
+        const int hide_hi = pos - k0 - 8 * h, hide_lo = low - k0 - 8 * h;
         if (k0 < all_lo || k0 + STEP > all_hi)
 #pragma unroll
             for (int t = 0; t < T; t++)
                 for (int i = 0; i < 16; i++) {
-                    const int key = k0 + 32 * t + 16 * (i >> 3) + 8 * h + (i & 7);
-                    s[t][i] = key > pos || key < low ? -INFINITY : s[t][i];
+                    const int key = 32 * t + 16 * (i >> 3) + (i & 7);
+                    s[t][i] = key > hide_hi || key < hide_lo ? -INFINITY : s[t][i];
                 }
         float top = s[0][0];
 #pragma unroll
@@ -1082,14 +1160,12 @@ __global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
         }
         float wunit = wbits;
         if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
-        float l = 0.0f;
 #pragma unroll
         for (int t = 0; t < T; t++)
             for (int i = 0; i < 16; i++) {
                 s[t][i] = __builtin_amdgcn_exp2f(fmaf(s[t][i], us, -mx));
-                l += s[t][i];
+                if (!HALF_SUM) sum += s[t][i];
             }
-        sum += l;
 
         // O^T += V^T P^T
 #pragma unroll
@@ -1098,10 +1174,11 @@ __global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
             for (int i = 0; i < 8; i++) w[i] = s[k >> 1][8 * (k & 1) + i] * wunit;
             h8 wf[NP];
             split8<NP>(w, wf);
+            if (HALF_SUM) sum = add_halves(wf[0], sum);
 #pragma unroll
             for (int d = 0; d < ND; d++) {
                 union { u4 u; h8 h; } vf[KP];
-                for (int p = 0; p < KP; p++) vf[p].u = vt[p * CH + v_chunk<STEP>(32 * d + col, 2 * k + h)];
+                for (int p = 0; p < KP; p++) vf[p].u = *(const u4*)((const uint8_t*)(vt + p * CH + 32 * d * (STEP / 8)) + (v_at ^ 32 * k));
                 if (KP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[KP - 1].h, wf[0], o[d], 0, 0, 0);
                 if (NP == 2) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0].h, wf[NP - 1], o[d], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[0].h, wf[0], o[d], 0, 0, 0);
@@ -1152,7 +1229,7 @@ __global__ __launch_bounds__(256, 2) void k_attend_many(AttnArgsP a) {
 // waves of 16 rows on the 16x16x32 products, two to a SIMD, so that one multiplies while the other reads. S^T tiles and
 // operands are k_attend_few's: a lane holds the keys 8 g .. + 8 of a step of 32.
 template <int TYPE, int NP, int SRC>
-__global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attend_wide(AttnArgsP a) {
     constexpr int HDP = 256, NT = 512;
     constexpr bool QUANT = TYPE != FLLM_TYPE_F16;
     constexpr int NB = HDP / 32, ND = HDP / 16;
@@ -1160,7 +1237,6 @@ __global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
     constexpr int STEP = many_step(HDP, NP);                 // keys a step
     static_assert(STEP == 32, "two tiles of 16 keys");
     constexpr int CH = STEP * HDP / 8;                       // chunks of 8 halves a plane
-    constexpr int DL = CH / NT;                              // loads of a plane a thread
     constexpr bool DIRECT = SRC != SRC_CODES;
     // K, V of a step and of the next one: two objects, so that the compiler sees that reads of the one need not wait for
     // loads into the other
@@ -1171,51 +1247,32 @@ __global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
     const int kvh = blockIdx.x % a.pg.nkv;
     const AttnItem it = a.items[blockIdx.x / a.pg.nkv];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, col = lane & 15, g = lane >> 4;
-    const int hd = a.pg.hd, nb = hd >> 5, lp = a.pg.page_log2, P = 1 << lp;
+    const int hd = a.pg.hd, lp = a.pg.page_log2;
     const int* table = a.tables + it.table;
     const int last_block = (it.len - 1) >> lp;
     const int64_t tile_lo = (int64_t)it.pos0 + it.row0 / a.group + 1 - a.window;  // the first key that any row sees
 
     // ---- the steps on their way; pages of a step are looked up a step before its loads
     Codes<QUANT ? TYPE : (int)FLLM_TYPE_Q8_0, HDP, STEP, KP, NT> codes;  // SRC_CODES
-    int pk[DL], pv;                                                  // SRC_PAGES
+    PageLoads<HDP, STEP, NT, SRC == SRC_PAGES> direct;               // SRC_PAGES, SRC_PARTS
     float ik = 1.0f, ik_next = 1.0f;                                 // quantised: 1 / kunit of this step and the next
     int ev = 0, ev_next = 0;                                         // and vexp
     const auto pages_at = [&](int k0) {
         if (SRC == SRC_CODES) codes.pages_at(table, last_block, lp, k0);
-        if (SRC == SRC_PAGES) {
-            for (int i = 0; i < DL; i++) pk[i] = table[min((k0 + (tid + NT * i) / (HDP / 8)) >> lp, last_block)];
-            // the chunk that this thread's slots hold is the same in each: NT slots are a multiple of 16 rows
-            pv = table[min((k0 + 8 * ((tid % (STEP / 8)) ^ v_swizzle<STEP>(tid / (STEP / 8)))) >> lp, last_block)];
-        }
+        if (SRC <= SRC_PARTS) direct.pages_at(table, last_block, lp, k0);
     };
     const auto load = [&](int k0, u4* to) {
         if (SRC == SRC_CODES) codes.load(a.pg, kvh, k0);
         if (SRC == SRC_IMAGE) {
             k0 = min(k0, (it.k1 - 1) / STEP * STEP);  // past the item's end: its last step again
             const int64_t at = ((int64_t)it.image * (kKeyStep / STEP) + k0 / STEP) * a.pg.nkv + kvh;
-            const u4* p = (const u4*)a.images + at * (2 * KP * CH) + tid;
-#pragma unroll
-            for (int i = 0; i < 2 * KP * DL; i++) to_lds(p + NT * i, to + NT * i + 64 * wave);
+            image_to_lds<2 * KP * CH, NT>((const u4*)a.images + at * (2 * KP * CH), to);
             ik_next = a.image_units[2 * at];
             ev_next = (int)a.image_units[2 * at + 1];
         }
-        if (SRC == SRC_PAGES) {  // slot by slot of the LDS image
-            const auto cell = [&](int page) { return ((uint64_t)(uint32_t)page * a.pg.nkv + kvh) * a.pg.cell; };
-#pragma unroll
-            for (int i = 0; i < DL; i++) {
-                const int slot = tid + NT * i, key = slot / (HDP / 8), c = (slot % (HDP / 8)) ^ k_swizzle<HDP>(key);
-                to_lds(a.pg.k + cell(pk[i]) + (uint32_t)((((c >> 2) < nb ? c >> 2 : 0) * P + ((k0 + key) & (P - 1))) * 64 + (c & 3) * 16),
-                       to + NT * i + 64 * wave);
-            }
-            const uint8_t* vc = a.pg.v + cell(pv);
-#pragma unroll
-            for (int i = 0; i < DL; i++) {
-                const int slot = tid + NT * i, d = slot / (STEP / 8), c = (slot % (STEP / 8)) ^ v_swizzle<STEP>(d);
-                to_lds(vc + (uint32_t)((d < hd ? d : 0) * P + ((k0 + 8 * c) & (P - 1))) * 2, to + KP * CH + NT * i + 64 * wave);
-            }
-        }
+        if (SRC <= SRC_PARTS) direct.load(a.pg, kvh, k0, to, to + KP * CH);
     };
+    if (SRC <= SRC_PARTS) direct.start(a.pg);
     pages_at(it.k0);
     load(it.k0, lds0);
     pages_at(it.k0 + STEP);
@@ -1279,6 +1336,8 @@ __global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
 
     int vexp = -30;  // quantised: o is in units of 2^-min(8 - vexp, 15), vexp the largest so far
     constexpr float wbits = NP == 2 ? 256.0f : 1.0f;  // weights (up to 2^6) times this: leaves the low halves room
+    // this lane's operands in a plane: K row 8 (col >> 2) + (col & 3) of tile 0, the chunk 4 c + g; V row col, the chunk g
+    const int k_at0 = k_chunk<HDP>(8 * (col >> 2) + (col & 3), g) * 16, v_at0 = v_chunk<STEP>(col, g) * 16;
     const auto step = [&](u4* cur, u4* nxt, int k0) {
         // pages and codes past the item's end are those of its sequence's last page: loaded, never used
         if (SRC == SRC_CODES) {
@@ -1292,35 +1351,42 @@ __global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
             ik = ik_next;
             ev = ev_next;
             lds_barrier<true>();
-            if (SRC == SRC_PAGES && (k0 < tile_lo || k0 + STEP > it.len)) {
+            if (SRC <= SRC_PARTS && (k0 < tile_lo || k0 + STEP > it.len)) {
                 // zeros for what lies outside the sequence, which may be anything
-                uint16_t* v = (uint16_t*)(cur + KP * CH);
-                for (int u = tid; u < HDP * STEP; u += NT) {
-                    const int d = u / STEP, j = u % STEP;
-                    if (k0 + j < tile_lo || k0 + j >= it.len) v[v_chunk<STEP>(d, j >> 3) * 8 + (j & 7)] = 0;
-                }
+                zero_outside<HDP, STEP, NT>(cur + KP * CH, k0, tile_lo, it.len);
                 lds_barrier<false>();
             }
         }
         load(k0 + STEP, nxt);
         pages_at(k0 + 2 * STEP);
         const u4 *kt = cur, *vt = cur + KP * CH;
+        int k_at = k_at0, v_at = v_at0;
+        asm volatile("" : "+v"(k_at), "+v"(v_at));  // or each address would be kept in a register across the steps
 
         // S^T = K Q^T: row rho of tile t is key 8 (rho >> 2) + 4 t + (rho & 3); high and low products apart, so that there
         // are four chains of them
         f4 hi[2], lo[2];
 #pragma unroll
         for (int t = 0; t < 2; t++) hi[t] = lo[t] = f4{0.f, 0.f, 0.f, 0.f};
+        union { u4 u; h8 h; } kf[2][2][KP];  // operands of this product and the next
+        const auto k_load = [&](int c) {
 #pragma unroll
-        for (int c = 0; c < NB; c++)
+            for (int t = 0; t < 2; t++)
+                for (int p = 0; p < KP; p++)
+                    kf[c & 1][t][p].u = *(const u4*)((const uint8_t*)(kt + p * CH + 4 * t * (HDP / 8)) + (k_at ^ 64 * c));
+        };
+        k_load(0);
+#pragma unroll
+        for (int c = 0; c < NB; c++) {
+            if (c + 1 < NB) k_load(c + 1);
+            __builtin_amdgcn_sched_barrier(0);  // the reads stay ahead of this product
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                union { u4 u; h8 h; } kf[KP];
-                for (int p = 0; p < KP; p++) kf[p].u = kt[p * CH + k_chunk<HDP>(8 * (col >> 2) + 4 * t + (col & 3), 4 * c + g)];
-                hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0].h, q[c][0], hi[t], 0, 0, 0);
-                if (NP == 2) lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[0].h, q[c][NP - 1], lo[t], 0, 0, 0);
-                if (KP == 2) lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[KP - 1].h, q[c][0], lo[t], 0, 0, 0);
+                hi[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c & 1][t][0].h, q[c][0], hi[t], 0, 0, 0);
+                if (NP == 2) lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c & 1][t][0].h, q[c][NP - 1], lo[t], 0, 0, 0);
+                if (KP == 2) lo[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[c & 1][t][KP - 1].h, q[c][0], lo[t], 0, 0, 0);
             }
+        }
         float s[8];
         for (int i = 0; i < 8; i++) s[i] = NP == 2 ? hi[i >> 2][i & 3] + lo[i >> 2][i & 3] : hi[i >> 2][i & 3];
         float us = unscale;
@@ -1329,10 +1395,10 @@ __global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
             softcap_n<8, true>(s, us, a.softcap * kLog2e);
             us = 1.0f;
         }
+        const int hide_hi = pos - k0 - 8 * g, hide_lo = low - k0 - 8 * g;
         if (k0 < all_lo || k0 + STEP > all_hi)
             for (int i = 0; i < 8; i++) {
-                const int key = k0 + 8 * g + i;
-                s[i] = key > pos || key < low ? -INFINITY : s[i];
+                s[i] = i > hide_hi || i < hide_lo ? -INFINITY : s[i];
             }
         float top = s[0];
         for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
@@ -1367,7 +1433,7 @@ __global__ __launch_bounds__(512, 2) void k_attend_wide(AttnArgsP a) {
 #pragma unroll
         for (int d = 0; d < ND; d++) {
             union { u4 u; h8 h; } vf[KP];
-            for (int p = 0; p < KP; p++) vf[p].u = vt[p * CH + v_chunk<STEP>(16 * d + col, g)];
+            for (int p = 0; p < KP; p++) vf[p].u = *(const u4*)((const uint8_t*)(vt + p * CH + 16 * d * (STEP / 8)) + v_at);
             if (KP == 2) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[KP - 1].h, wf[0], o[d], 0, 0, 0);
             if (NP == 2) o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[0].h, wf[NP - 1], o[d], 0, 0, 0);
             o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[0].h, wf[0], o[d], 0, 0, 0);
@@ -1433,8 +1499,15 @@ hipError_t launch_items(AttnArgsP a, const AttnWork& w, hipStream_t st) {
                 else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, SRC_IMAGE>), grid(c), dim3(256), 0, st, a);
             }
         } else if (c == kAttnMany) {
-            if constexpr (HDP > 128) hipLaunchKernelGGL((k_attend_wide<TYPE, NP, QUANT ? SRC_CODES : SRC_PAGES>), grid(c), dim3(512), 0, st, a);
-            else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, QUANT ? SRC_CODES : SRC_PAGES>), grid(c), dim3(256), 0, st, a);
+            const bool whole = 1 << a.pg.page_log2 >= many_step(HDP, NP);
+            const auto go = [&](auto src) {
+                constexpr int SRC = decltype(src)::value;
+                if constexpr (HDP > 128) hipLaunchKernelGGL((k_attend_wide<TYPE, NP, SRC>), grid(c), dim3(512), 0, st, a);
+                else hipLaunchKernelGGL((k_attend_many<TYPE, HDP, NP, SRC>), grid(c), dim3(256), 0, st, a);
+            };
+            if constexpr (QUANT) go(std::integral_constant<int, SRC_CODES>());
+            else if (whole) go(std::integral_constant<int, SRC_PAGES>());
+            else go(std::integral_constant<int, SRC_PARTS>());
         } else if (c == 3) {
             if constexpr (HDP <= 128) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2, 16>), grid(c), dim3(256), 0, st, a);
         } else if (c == 2) {
