@@ -444,12 +444,12 @@ extern "C" int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d) {
     v.u_sample = (const float*)d->u_sample->ptr;
     v.out_tokens = (int*)d->out_tokens->ptr;
     v.out_counts = (int*)d->out_counts->ptr;
-    int seg = 0;
-    const int n_seg = draft_segments(v.n_seqs, v.vocab, ctx->n_cu, &seg);
+    int seg = 0, runs = 1;
+    const int n_seg = draft_segments(v.n_seqs, v.vocab, ctx->n_cu, &seg, &runs);
     std::lock_guard<std::mutex> lock(ctx->ws.mu);
     hipError_t e = workspace_room(ctx, (uint64_t)n * (uint64_t)n_seg * 16, (uint64_t)n);
     if (e != hipSuccess)
         return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "draft workspace: %s", hipGetErrorString(e));
-    HIP_TRY(launch_draft_verify(v, seg, n_seg, (double*)ctx->ws.part, ctx->ws.cnt, ctx->stream));
+    HIP_TRY(launch_draft_verify(v, seg, n_seg, runs, (double*)ctx->ws.part, ctx->ws.cnt, ctx->stream));
     return FLLM_OK;
 }

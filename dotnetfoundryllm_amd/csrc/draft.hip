@@ -40,6 +40,7 @@ struct Ids16 {
                 p[k] = *(const f4a*)(w.t + i);
                 if (w.d) q[k] = *(const f4a*)(w.d + i);
             } else {
+#pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (i + e < hi) {
                         p[k][e] = w.t[i + e];
@@ -91,7 +92,7 @@ __device__ __forceinline__ void scan256(const double v[N], double before[N], dou
     }
 }
 
-__global__ __launch_bounds__(256) void k_draft_verify(DraftView d, int seg, int n_seg, double* part, unsigned* cnt) {
+__global__ __launch_bounds__(256) void k_draft_verify(DraftView d, int seg, int n_seg, int runs, double* part, unsigned* cnt) {
     __shared__ double s_wave[4][4], s_want;
     __shared__ int s_seg, s_last, s_found, s_pos, s_id;
     const int s = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
@@ -124,26 +125,34 @@ __global__ __launch_bounds__(256) void k_draft_verify(DraftView d, int seg, int 
     w.d = d.draft && w.rest ? d.draft + ((int64_t)s * d.n_draft + c) * d.draft_ld : nullptr;
     w.point = !d.draft && w.rest ? d.tokens[(int64_t)s * d.n_draft + c] : -1;
 
-    // this segment's sums: of the weights, and of the target's alone
-    const int lo = blockIdx.x * seg, hi = min(lo + seg, d.vocab);
-    Ids16 x;
-    x.load(w, lo, hi);
-    double sums[2] = {0.0, 0.0}, before2[2];
-#pragma unroll
-    for (int k = 0; k < 4; k++)
-        for (int e = 0; e < 4; e++) {
-            sums[0] += w.of(x.p[k][e], x.q[k][e], lo + 1024 * k + 4 * tid + e);
-            sums[1] += counted((double)x.p[k][e]);
-        }
-    scan256<2>(sums, before2, sums, s_wave);
+    // these segments' sums: of the weights, and of the target's alone
+    const int seg0 = blockIdx.x * runs, seg1 = min(seg0 + runs, n_seg);
     const __amdgpu_buffer_rsrc_t rp = wt_rsrc(part + (int64_t)s * n_seg * 2, (uint32_t)n_seg * 16);
+    Ids16 x;
+    x.load(w, seg0 * seg, min(seg0 * seg + seg, d.vocab));
+    for (int g = seg0; g < seg1; g++) {
+        Ids16 next;
+        const int lo = g * seg, ahead = (g + 1 < seg1 ? g + 1 : g) * seg;
+        next.load(w, ahead, g + 1 < seg1 ? min(ahead + seg, d.vocab) : ahead);
+        double sums[2] = {0.0, 0.0}, before2[2];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            for (int e = 0; e < 4; e++) {
+                sums[0] += w.of(x.p[k][e], x.q[k][e], lo + 1024 * k + 4 * tid + e);
+                sums[1] += counted((double)x.p[k][e]);
+            }
+        scan256<2>(sums, before2, sums, s_wave);
+        if (tid == 0) {
+            union { double v[2]; u4 u; } both;
+            both.v[0] = sums[0];
+            both.v[1] = sums[1];
+            __builtin_amdgcn_raw_buffer_store_b128(both.u, rp, (uint32_t)g * 16, 0, CPOL_SC1);
+        }
+        x = next;
+    }
     if (tid == 0) {
-        union { double v[2]; u4 u; } both;
-        both.v[0] = sums[0];
-        both.v[1] = sums[1];
-        __builtin_amdgcn_raw_buffer_store_b128(both.u, rp, (uint32_t)blockIdx.x * 16, 0, CPOL_SC1);
         wt_complete();
-        s_last = __hip_atomic_fetch_add(cnt + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(n_seg - 1);
+        s_last = __hip_atomic_fetch_add(cnt + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
         if (s_last) st_wt_u(cnt + s, 0u);
     }
     __syncthreads();
@@ -212,17 +221,23 @@ __global__ __launch_bounds__(256) void k_draft_verify(DraftView d, int seg, int 
 
 }  // namespace
 
-// Segments of a row: as many as give every CU a few workgroups over all sequences, of 1024 ids (4 a thread) at least
-// and 4096 (16 a thread) at most; up to 256 of them (a thread each in the last workgroup).
-int draft_segments(int n_seqs, int vocab, int n_cu, int* seg) {
+// Segments of a row: of 1024 ids (4 a thread) at least and 4096 (16 a thread) at most, shorter ones while they leave
+// every CU no more than a few workgroups over all sequences; up to 256 of them (a thread each in the last workgroup).
+// A workgroup takes `runs` of them in a row, the next one's loads under way while one is summed, so that two
+// workgroups a CU remain: each begins with the same three dependent loads. 64 x 152064: 1 run 37.5 us, 2: 29.7,
+// 3: 27.4, 4: 26.9, 6: 26.4, 10: 29.8; 1 x 128256 (126 segments): 1 run 16.5 us, 2: 16.9, 4: 19.8.
+int draft_segments(int n_seqs, int vocab, int n_cu, int* seg, int* runs) {
     int k = (int)((int64_t)n_seqs * vocab / ((int64_t)4 * n_cu * 1024)) + 1;
     k = k > 4 ? 4 : k;
     while (k < 4 && (vocab + 1024 * k - 1) / (1024 * k) > 256) k++;
     *seg = 1024 * k;
-    return (vocab + *seg - 1) / *seg;
+    const int n_seg = (vocab + *seg - 1) / *seg;
+    const int64_t r = (int64_t)n_seqs * n_seg / (2 * n_cu);
+    *runs = r < 1 ? 1 : r < n_seg ? (int)r : n_seg;
+    return n_seg;
 }
 
-hipError_t launch_draft_verify(const DraftView& d, int seg, int n_seg, double* part, unsigned* cnt, hipStream_t st) {
+hipError_t launch_draft_verify(const DraftView& d, int seg, int n_seg, int runs, double* part, unsigned* cnt, hipStream_t st) {
     for (int s0 = 0; s0 < d.n_seqs; s0 += 65535) {  // the grid's second dimension ends at 65535
         DraftView v = d;
         v.n_seqs = d.n_seqs - s0 < 65535 ? d.n_seqs - s0 : 65535;
@@ -235,7 +250,7 @@ hipError_t launch_draft_verify(const DraftView& d, int seg, int n_seg, double* p
         v.u_sample += s0;
         v.out_tokens += s0 * n1;
         v.out_counts += s0;
-        hipLaunchKernelGGL(k_draft_verify, dim3(n_seg, v.n_seqs), dim3(256), 0, st, v, seg, n_seg, part + (int64_t)s0 * n_seg * 2, cnt + s0);
+        hipLaunchKernelGGL(k_draft_verify, dim3((n_seg + runs - 1) / runs, v.n_seqs), dim3(256), 0, st, v, seg, n_seg, runs, part + (int64_t)s0 * n_seg * 2, cnt + s0);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

@@ -78,9 +78,9 @@ struct DraftView {
 };
 // A row's segments of *seg ids each, a workgroup per sequence and segment; vocab up to kDraftVocab.
 constexpr int kDraftVocab = 1 << 20;
-int draft_segments(int n_seqs, int vocab, int n_cu, int* seg);
+int draft_segments(int n_seqs, int vocab, int n_cu, int* seg, int* runs);
 // part: 2 doubles per sequence and segment; cnt: a zero per sequence, left as one
-hipError_t launch_draft_verify(const DraftView& d, int seg, int n_seg, double* part, unsigned* cnt, hipStream_t st);
+hipError_t launch_draft_verify(const DraftView& d, int seg, int n_seg, int runs, double* part, unsigned* cnt, hipStream_t st);
 
 // ---- elements ---------------------------------------------------------------------------
 __device__ __forceinline__ float row_elem(const RowsView& r, int64_t i) {
