@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <vector>
@@ -234,6 +235,20 @@ inline void attn_count(const SeqPlan& s, int group, int window, int c, int64_t s
     }
 }
 
+// Key steps an item of few rows should have at least: one that is cut into n parts ends when its workgroup has read
+// S / n steps and the one that joins them n partial results, both as fast as one CU can; S steps of rows r and e bytes an
+// element balance at sqrt(S r / (16 e)). One sequence, 4 rows, Q8_0, in us with 2, 4 and 8 steps an item: 518 positions
+// 8.8, 9.4, 11.3; 2048: 9.5, 9.7, 11.8; 4096: 12.3, 10.5, 12.0; 8192: 14.2, 14.2, 13.1. 4 sequences of 2000, 20
+// rows, F16: 20.8, 19.2, 20.3; 7 rows, Q8_0: 10.5, 11.4, 14.4, so that fewer than 4 are left alone. Longer sequences
+// fill all CUs with 8 steps and more.
+inline int64_t join_steps(const SeqPlan& s, int group, int window, int c, bool quant) {
+    AttnCount n;
+    attn_count(s, group, window, c, 1, &n);
+    const int64_t rows = std::min<int64_t>((int64_t)s.n_new * group, kAttnTile[c]), tiles = ((int64_t)s.n_new * group + kAttnTile[c] - 1) / kAttnTile[c];
+    const double best = std::sqrt((double)(n.steps / tiles * rows) / (quant ? 16.0 : 32.0));
+    return best < 4.0 ? 0 : std::min<int64_t>(8, 2 * (int64_t)(best / 2 + 0.5));
+}
+
 // The items of a batch on a device of n_cu CUs. False where they or their partial rows are too many.
 inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, bool quant, int window, int n_cu, AttnPlan* p) {
     const int group = n_heads / n_kv;
@@ -291,7 +306,9 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, b
             p->images += g1 - g0;
             if (p->images > INT32_MAX / 4 / n_kv) return false;
         }
-        if (s.n_new) attn_items(s, i, i * b.tab_w, (int)image, group, window, c, c >= kAttnMany ? many : few, &p->items[c], &p->part_rows);
+        if (s.n_new)
+            attn_items(s, i, i * b.tab_w, (int)image, group, window, c, c >= kAttnMany ? many : std::max(few, join_steps(s, group, window, c, quant)),
+                       &p->items[c], &p->part_rows);
         if (p->part_rows > INT32_MAX / n_kv) return false;
     }
     for (auto& v : p->items) {
