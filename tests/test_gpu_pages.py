@@ -12,6 +12,7 @@ or 2^-8: 5 x 2^-11 and 2^-8 + 4 x 2^-11. No single element is off by more than 4
 """
 import ctypes as C
 import math
+import threading
 
 import numpy as np
 import pytest
@@ -531,3 +532,266 @@ def test_wrapped_buffers(ctx):
     for b in (w, whole, x, y):
         b.close()
     assert hip.hipFree(base) == 0
+
+
+# ---- longer, wider, larger ------------------------------------------------------------------------
+def check(got, want, act, more=1.0):
+    tol = more * {"f32": 2.0 ** -18, "f16": 5 * 2.0 ** -11, "bf16": 2.0 ** -8 + 4 * 2.0 ** -11}[act]
+    off = got.reshape(want.shape) - want
+    assert np.linalg.norm(off) <= tol * np.linalg.norm(want)
+    assert np.abs(off).max() <= 40 * tol * np.abs(want).max()
+
+
+def attention_of(s, k, v, heads, act="f32", window=F.NO_WINDOW, scale=None, softcap=0.0, batch=None, new=None, length=None, q=None):
+    """One call's rows and what they should be, a sequence each."""
+    new, length = new or s.new, length or s.length
+    b = batch or s.batch(heads, window, new, length)
+    n, hd, scale = sum(new), s.hd, 1.0 / math.sqrt(s.hd) if scale is None else scale
+    q = s.rng.standard_normal((n, heads * hd)) if q is None else q
+    q = from_bits(to_bits(q, act), act)
+    out = s.put(np.zeros((n, heads * hd)), act)
+    b.attention(s.layer, s.put(q, act), out, scale, softcap)
+    s.ctx.sync()
+    got, at = s.get(out, act), np.cumsum([0] + new)
+    for i, (lo, hi) in enumerate(zip(at, at[1:])):
+        if hi > lo:
+            yield got[lo:hi], attend(q[lo:hi].reshape(-1, heads, hd), k[i], v[i], heads // s.kv, length[i] - new[i], window, scale, softcap)
+
+
+@pytest.mark.parametrize("cache", TYPES)
+@pytest.mark.parametrize("kv,heads,hd,page,new,length,window,softcap", [
+    (1, 4, 256, 64, [111, 3], [500, 90], None, 0.0),      # wide heads, many rows beside few
+    (2, 6, 192, 16, [150], [163], 40, 20.0),              # tiles whose window leaves parts of their steps
+    (1, 8, 64, 32, [130, 120], [1000, 120], None, 0.0),   # pages shorter than a step, two sequences
+    (1, 4, 128, 128, [97], [9000], None, 0.0),            # few tiles over long keys: cut and joined
+    (1, 2, 256, 128, [65], [6000], None, 0.0),
+    (1, 1, 128, 64, [1], [70000], None, 0.0),             # one row over very many keys
+    (1, 16, 32, 16, [1, 1], [20000, 31], 19990, 0.0),
+    (1, 32, 128, 64, [2], [4000], None, 0.0),
+])
+def test_attention_over_longer_ranges(make, cache, kv, heads, hd, page, new, length, window, softcap):
+    for act in ("f32", "bf16"):
+        s = make(cache, kv, hd, page, new, length, seed=hd, garbage=0x7F)
+        for got, want in attention_of(s, *s.fill(), heads, act, window or F.NO_WINDOW, None, softcap):
+            check(got, want, act)
+
+
+@pytest.mark.parametrize("cache", TYPES)
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+@pytest.mark.parametrize("new,length", [([1, 3], [300, 40]), ([140], [150])])
+def test_attention_of_other_magnitudes(make, cache, act, new, length):
+    """Scores' scales of any sign and zero, values near the ends of half precision, rows of q of any size. The tolerances
+    are relative to the outputs; scores stay of size 1."""
+    for scale, of_k, of_v, of_q in ((-0.125, 1, 1, 1), (0.0, 1, 1, 1), (0.125, 1, 2.0 ** -18, 1), (0.125, 1, 10000, 1),
+                                    (0.125 * 2.0 ** 12, 2.0 ** -12, 1, 1), (0.125 * 2.0 ** -90, 1, 1, 2.0 ** 90),
+                                    (0.125 * 2.0 ** 90, 1, 1, 2.0 ** -90)):
+        s = make(cache, 2, 64, 32, new, length, seed=5)
+        k, v = s.fill(of_k, of_v)
+        q = s.rng.standard_normal((sum(new), 6 * 64)) * of_q
+        q[0, :64] = 0.0
+        for softcap in (0.0, 2.0):
+            for got, want in attention_of(s, k, v, 6, act, scale=scale, softcap=softcap, q=q):
+                check(got, want, act)
+
+
+@pytest.mark.parametrize("cache", TYPES)
+def test_attention_with_pages_given_back(make, cache):
+    """A page before the window may go to another sequence, whose rows then stand in it."""
+    s = make(cache, 2, 64, 32, [2, 40], [300, 250], seed=3)
+    k, v = s.fill()
+    s.tables[0, :5] = -1  # 300 - 2 - 100 + 1 = 199: keys from page 6 on
+    s.tables[1, :3] = -1  # 250 - 40 - 100 + 1 = 111
+    for got, want in attention_of(s, k, v, 8, window=100):
+        check(got, want, "f32")
+
+
+@pytest.mark.parametrize("cache", TYPES)
+def test_attention_over_a_shared_prefix(make, cache):
+    s = make(cache, 2, 64, 16, [3, 3, 70], [70, 75, 134], seed=4)
+    s.tables[1:, :4] = s.tables[0, :4]
+    w = 128
+    x = [s.rng.standard_normal((64 + 6 + 11 + 70, w)).astype(np.float32) for _ in (0, 1)]
+    b = s.batch(2, new=[0, 0, 0], length=[64, 64, 64])
+    b.set([64], [64], s.tables[:1])  # a page that is written belongs to one sequence
+    b.append(1, *(s.put(a[:64], "f32") for a in x))
+    b.set([6, 11, 70], [70, 75, 134], s.tables)
+    b.append(1, *(s.put(a[64:], "f32") for a in x))
+    part = [[np.concatenate([a[:64], a[lo:hi]]) for lo, hi in ((64, 70), (70, 81), (81, 151))] for a in x]
+    k, v = ([stored(a, cache).reshape(-1, 2, 64) for a in p] for p in part)
+    for got, want in attention_of(s, k, v, 4):
+        check(got, want, "f32")
+
+
+@pytest.mark.parametrize("cache,act", [("f16", "f32"), ("q8_0", "bf16"), ("q4_0", "f32")])
+def test_the_same_call_gives_the_same_bits(make, cache, act):
+    s = make(cache, 2, 128, 64, [1, 5, 100], [3000, 700, 400], seed=6)
+    s.fill()
+    b, n = s.batch(8), 106
+    q = s.put(s.rng.standard_normal((n, 1024)), act)
+    outs = [s.put(np.zeros((n, 1024)), act) for _ in range(6)]
+    for o in outs:
+        b.attention(1, q, o, 0.1)
+    s.ctx.sync()
+    for o in outs[1:]:
+        assert np.array_equal(s.get(outs[0], act), s.get(o, act))
+
+
+def test_pages_beyond_four_gigabytes(ctx):
+    """Cells and rows whose offsets pass 32 bits: pages at the end of a large array, rows far apart."""
+    kv, hd, page, n_pages = 8, 256, 128, 9000
+    for cache in ("f16", "q8_0"):
+        p = F.PagedKvCache(ctx, TYPES[cache], 1, kv, hd, page, n_pages)
+        b = p.batch(kv)
+        b.set([150], [150], [[n_pages - 1, n_pages - 2]])
+        rng = np.random.default_rng(1)
+        x = [rng.standard_normal((150, kv * hd)).astype(np.float32) for _ in (0, 1)]
+        ld = 1 << 24
+        far = F.DeviceBuffer(ctx, 149 * 4 * ld + 4 * kv * hd)  # 10 GB
+        for i, row in enumerate(x[0]):
+            far.write(row, 4 * ld * i)
+        near = F.DeviceBuffer(ctx, x[1].nbytes)
+        near.write(x[1])
+        b.append(0, F.Rows(far, ld), F.Rows(near, kv * hd))
+        far.write(np.zeros(kv * hd, np.float32), 4 * ld * 140)
+        b.read(0, F.Rows(far, ld), F.Rows(near, kv * hd))
+        ctx.sync()
+        k, v = (stored(a.reshape(150, kv, hd), cache) for a in x)
+        assert np.array_equal(far.read(4 * kv * hd, offset=4 * ld * 140), k[140].reshape(-1).astype(np.float32))
+        assert np.array_equal(near.read(x[1].nbytes).reshape(150, kv, hd), v.astype(np.float32))
+        q = rng.standard_normal((150, kv * hd)).astype(np.float32)
+        for i, row in enumerate(q):
+            far.write(row, 4 * ld * i)
+        for new in (150, 2):  # many rows, few rows
+            b.set([new], [150], [[n_pages - 1, n_pages - 2]])
+            b.attention(0, F.Rows(far, ld, F.F32, 4 * ld * (150 - new)), F.Rows(near, kv * hd), 1 / 16)
+            ctx.sync()
+            got = near.read(4 * new * kv * hd).reshape(new, kv, hd).astype(np.float64)
+            check(got, attend(q[150 - new:].reshape(new, kv, hd).astype(np.float64), k, v, 1, 150 - new, F.NO_WINDOW, 1 / 16, 0.0), "f32")
+        for x in (b, p, far, near):
+            x.close()
+
+
+def test_two_threads_on_one_context(make):
+    """Calls of two threads share the context's stream and workspace."""
+    s = make("q8_0", 2, 64, 32, [1, 2, 90], [4000, 300, 260], seed=8)
+    s.fill()
+    sets = [([1, 2, 90], s.batch(8)), ([1, 0, 0], s.batch(8, new=[1, 0, 0])), ([0, 2, 0], s.batch(8, new=[0, 2, 0]))]
+    jobs = []
+    for new, b in sets:
+        q = s.put(s.rng.standard_normal((sum(new), 512)), "f32")
+        outs = [s.put(np.zeros((sum(new), 512)), "f32") for _ in range(12)]
+        b.attention(1, q, outs[0], 0.1)
+        jobs.append((b, q, outs))
+    s.ctx.sync()
+    failed = []
+
+    def work(b, q, outs):
+        try:
+            for o in outs[1:]:
+                b.attention(1, q, o, 0.1)
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    s.ctx.sync()
+    assert not failed
+    for _, _, outs in jobs:
+        first = s.get(outs[0], "f32")
+        assert first.any()
+        for o in outs[1:]:
+            assert np.array_equal(s.get(o, "f32"), first)
+
+
+# ---- together ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("cache", TYPES)
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64)])
+def test_serving_with_drafts(ctx, cache, hd, page):
+    """Three requests through two layers as a server has them: prompts in, then steps of up to three drafted tokens behind
+    the last one, each checked against the target; what was refused is overwritten by the next step. A dense model of the
+    same layers in 64 bits, without pages, drafts or steps, gives the same rows."""
+    kv, heads, vocab, layers, drafts = 2, 6, 301, 2, 3
+    rng = np.random.default_rng(hd)
+    lens, n_pages = [37, 5, 70], 60
+    tables = rng.permutation(n_pages).astype(np.int32)[:3 * 15].reshape(3, 15)
+    w, wq = kv * hd, heads * hd
+    embed = rng.standard_normal((layers, 2, vocab, w)).astype(np.float32)   # a token's k and v in each layer
+    query = rng.standard_normal((layers, vocab, wq)).astype(np.float32)
+    tokens = [list(rng.integers(0, vocab, n)) for n in lens]
+    p = F.PagedKvCache(ctx, TYPES[cache], layers, kv, hd, page, n_pages)
+    b, bufs = p.batch(heads), []
+
+    def put(x):
+        x = np.ascontiguousarray(x)
+        buf = F.DeviceBuffer(ctx, max(x.nbytes, 16))
+        buf.write(x)
+        bufs.append(buf)
+        return buf
+
+    def step(new):
+        """New tokens of each request through both layers: the rows of the last one."""
+        ids = np.concatenate([np.asarray(t, np.int64) for t in new])
+        b.set([len(t) for t in new], [len(t) + len(n) for t, n in zip(tokens, new)], tables)
+        outs = []
+        for layer in range(layers):
+            b.append(layer, F.Rows(put(embed[layer, 0, ids]), w), F.Rows(put(embed[layer, 1, ids]), w))
+            out = put(np.zeros((len(ids), wq), np.float32))
+            b.attention(layer, F.Rows(put(query[layer, ids]), wq), F.Rows(out, wq), 0.1)
+            outs.append(out)
+        ctx.sync()
+        return [o.read(4 * len(ids) * wq).reshape(len(ids), heads, hd).astype(np.float64) for o in outs], [len(t) for t in new]
+
+    def dense(i, layer, ids, pos0):
+        k, v = (stored(embed[layer, j, np.asarray(ids)].reshape(-1, kv, hd), cache) for j in (0, 1))
+        q = query[layer, np.asarray(ids)[pos0:]].reshape(-1, heads, hd).astype(np.float64)
+        return attend(q, k, v, heads // kv, pos0, F.NO_WINDOW, 0.1, 0.0)
+
+    def compare(outs, counts, new):
+        at = np.cumsum([0] + counts)
+        for layer in range(layers):
+            for i in range(3):
+                check(outs[layer][at[i]:at[i + 1]], dense(i, layer, tokens[i] + list(new[i]), len(tokens[i])), "f32")
+
+    prompts, tokens = tokens, [[], [], []]
+    outs, counts = step(prompts)
+    compare(outs, counts, prompts)
+    tokens = [list(t) for t in prompts]
+    soft = lambda x: (np.exp(x) / np.exp(x).sum(-1, keepdims=True)).astype(np.float32)  # noqa: E731
+    lasts = [int(rng.integers(0, vocab)) for _ in range(3)]
+    refused = 0
+    for _ in range(6):
+        n_draft = np.array([drafts, int(rng.integers(0, drafts + 1)), 1])
+        q = soft(3 * rng.standard_normal((3, drafts, vocab)))
+        t = soft(3 * rng.standard_normal((3, drafts + 1, vocab)))
+        t[:, :drafts] = 0.6 * t[:, :drafts] + 0.4 * q
+        drafted = np.array([[rng.choice(vocab, p=r.astype(np.float64) / r.sum(dtype=np.float64)) for r in rows] for rows in q])
+        new = [[lasts[i]] + list(drafted[i, :n_draft[i]]) for i in range(3)]
+        outs, counts = step(new)
+        compare(outs, counts, new)
+        ua, us = rng.random((3, drafts), dtype=np.float32), rng.random(3, dtype=np.float32)
+        ids, kept = put(np.zeros((3, drafts + 1), np.int32)), put(np.zeros(3, np.int32))
+        F.draft_verify(ctx, 3, drafts, vocab, F.Rows(put(t.reshape(-1, vocab)), vocab), put(drafted.astype(np.int32)), put(ua), put(us),
+                       ids, kept, draft=F.Rows(put(q.reshape(-1, vocab)), vocab), counts=put(n_draft.astype(np.int32)))
+        ctx.sync()
+        got = ids.read(48, np.int32).reshape(3, drafts + 1), kept.read(12, np.int32)
+        want = verify(t, q, drafted, n_draft, ua, us)
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+        for i in range(3):
+            c = got[1][i]
+            refused += n_draft[i] - c
+            tokens[i] += new[i][:1 + c]
+            lasts[i] = int(got[0][i, c])
+    assert refused > 0
+    b.set([0, 0, 0], [len(t) for t in tokens], tables)
+    n = sum(len(t) for t in tokens)
+    k, v = put(np.zeros((n, w), np.float32)), put(np.zeros((n, w), np.float32))
+    b.read(1, F.Rows(k, w), F.Rows(v, w))
+    ctx.sync()
+    ids = np.concatenate([np.asarray(t) for t in tokens])
+    for j, x in enumerate((k, v)):
+        assert np.array_equal(x.read(4 * n * w).reshape(n, kv, hd), stored(embed[1, j, ids].reshape(-1, kv, hd), cache).astype(np.float32))
+    for x in bufs + [b, p]:
+        x.close()
