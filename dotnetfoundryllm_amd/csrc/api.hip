@@ -229,6 +229,12 @@ extern "C" int32_t fllm_ctx_destroy(fllm_ctx* ctx) {
     staging_free(ctx->stage);
     if (ctx->ws.part) hipFree(ctx->ws.part);
     if (ctx->ws.cnt) hipFree(ctx->ws.cnt);
+    for (size_t i = 0; i < ctx->spare.n; i++) {
+        const BatchBlock& b = ctx->spare.blocks[i];
+        if (b.dev) hipFree(b.dev);
+        if (b.pin) hipHostFree(b.pin);
+        hipEventDestroy(b.sent);
+    }
     hipStreamDestroy(ctx->stream);
     delete ctx;
     return FLLM_OK;

@@ -28,12 +28,7 @@ struct fllm_batch {
     int n_heads = 0, window = 0;
     BatchPlan plan;
     AttnPlan attn;
-    // the plan's arrays on the device and the pinned block that they are copied from; `sent` says when
-    // the last copy has read it
-    uint8_t *dev = nullptr, *pin = nullptr;
-    uint64_t cap = 0;
-    hipEvent_t sent = nullptr;
-    bool in_flight = false;
+    BatchBlock mem;
     BatchView view{};
     AttnWork work{};
 };
@@ -132,7 +127,12 @@ extern "C" int32_t fllm_batch_create(fllm_pages* p, int32_t n_heads, int32_t win
     HIP_TRY(hipSetDevice(p->ctx->device));
     return guarded([&]() -> int32_t {
         fllm_batch* b = new fllm_batch();
-        hipError_t e = hipEventCreateWithFlags(&b->sent, hipEventDisableTiming);
+        SpareBlocks& spare = p->ctx->spare;
+        {
+            std::lock_guard<std::mutex> lock(spare.mu);
+            if (spare.n) b->mem = spare.blocks[--spare.n];
+        }
+        const hipError_t e = b->mem.sent ? hipSuccess : hipEventCreateWithFlags(&b->mem.sent, hipEventDisableTiming);
         if (e != hipSuccess) {
             delete b;
             return fail(FLLM_E_DEVICE, "hipEventCreate: %s", hipGetErrorString(e));
@@ -148,12 +148,12 @@ extern "C" int32_t fllm_batch_create(fllm_pages* p, int32_t n_heads, int32_t win
 
 // Room for n bytes on the device and in the pinned block. The old memory may still be read by enqueued
 // calls: they are waited for first.
-static hipError_t batch_room(fllm_batch* b, uint64_t n) {
+static hipError_t batch_room(fllm_ctx* ctx, BatchBlock* b, uint64_t n) {
     hipError_t e = hipSuccess;
     if (b->in_flight) e = hipEventSynchronize(b->sent);
     b->in_flight = false;
     if (e != hipSuccess || n <= b->cap) return e;
-    e = hipStreamSynchronize(b->p->ctx->stream);
+    e = hipStreamSynchronize(ctx->stream);
     if (e != hipSuccess) return e;
     if (b->dev) hipFree(b->dev);
     if (b->pin) hipHostFree(b->pin);
@@ -209,17 +209,17 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         from[N - 1] = pl.tables.data();
         size[N - 1] = pl.tables.size() * sizeof(int32_t);
         for (int i = 0; i < N; i++) at[i + 1] = at[i] + size[i];
-        hipError_t e = batch_room(b, at[N]);
+        hipError_t e = batch_room(p->ctx, &b->mem, at[N]);
         if (e != hipSuccess)
             return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "batch memory: %s", hipGetErrorString(e));
         for (int i = 0; i < N; i++)
-            if (size[i]) memcpy(b->pin + at[i], from[i], i ? size[i] : pl.seqs.size() * sizeof(SeqPlan));
-        HIP_TRY(hipMemcpyAsync(b->dev, b->pin, at[N], hipMemcpyHostToDevice, p->ctx->stream));
-        HIP_TRY(hipEventRecord(b->sent, p->ctx->stream));
-        b->in_flight = true;
+            if (size[i]) memcpy(b->mem.pin + at[i], from[i], i ? size[i] : pl.seqs.size() * sizeof(SeqPlan));
+        HIP_TRY(hipMemcpyAsync(b->mem.dev, b->mem.pin, at[N], hipMemcpyHostToDevice, p->ctx->stream));
+        HIP_TRY(hipEventRecord(b->mem.sent, p->ctx->stream));
+        b->mem.in_flight = true;
         b->plan.n_seqs = n_plan_seqs;
-        b->view.seqs = (const int4*)b->dev;
-        b->view.tables = (const int*)(b->dev + at[N - 1]);
+        b->view.seqs = (const int4*)b->mem.dev;
+        b->view.tables = (const int*)(b->mem.dev + at[N - 1]);
         b->view.tab_w = pl.tab_w;
         b->view.n_seqs = n_plan_seqs;
         b->view.new_blocks = pl.new_blocks;
@@ -229,11 +229,11 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         b->view.n_heads = b->n_heads;
         b->view.window = b->window;
         for (int i = 0; i < kAttnClasses; i++) {
-            b->work.items[i] = (const AttnItem*)(b->dev + at[1 + i]);
+            b->work.items[i] = (const AttnItem*)(b->mem.dev + at[1 + i]);
             b->work.n[i] = (int)b->attn.items[i].size();
         }
         b->work.part_rows = b->attn.part_rows;
-        b->work.image_items = (const ImageItem*)(b->dev + at[N - 2]);
+        b->work.image_items = (const ImageItem*)(b->mem.dev + at[N - 2]);
         b->work.n_image_items = (int)b->attn.image_items.size();
         b->work.n_images = b->attn.images;
         return FLLM_OK;
@@ -243,11 +243,19 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
 extern "C" int32_t fllm_batch_destroy(fllm_batch* b) {
     if (!b) return FLLM_OK;
     fllm_pages* p = b->p;
-    hipSetDevice(p->ctx->device);
-    hipStreamSynchronize(p->ctx->stream);
-    if (b->dev) hipFree(b->dev);
-    if (b->pin) hipHostFree(b->pin);
-    if (b->sent) hipEventDestroy(b->sent);
+    SpareBlocks& spare = p->ctx->spare;
+    bool kept = false;
+    {
+        std::lock_guard<std::mutex> lock(spare.mu);
+        if (spare.n < SpareBlocks::kMost) spare.blocks[spare.n++] = b->mem, kept = true;
+    }
+    if (!kept) {
+        hipSetDevice(p->ctx->device);
+        hipStreamSynchronize(p->ctx->stream);
+        if (b->mem.dev) hipFree(b->mem.dev);
+        if (b->mem.pin) hipHostFree(b->mem.pin);
+        hipEventDestroy(b->mem.sent);
+    }
     delete b;
     p->n_batches--;
     if (p->disposed && p->n_batches == 0) pages_free(p);
@@ -304,10 +312,26 @@ static int32_t check_rows(fllm_ctx* ctx, const fllm_rows* r, const char* name, i
     return FLLM_OK;
 }
 
+// Whether n rows of each share memory: exact for rows of one stride (columns of one matrix), else by their ranges.
 static bool overlap(const RowsView& a, const RowsView& b, int64_t n, int64_t width) {
     if (n <= 0) return false;
-    const auto end = [&](const RowsView& r) { return r.p + ((n - 1) * r.ld + width) * (r.type == FLLM_TYPE_F32 ? 4 : 2); };
-    return a.p < end(b) && b.p < end(a);
+    const auto size = [](const RowsView& r) { return (int64_t)(r.type == FLLM_TYPE_F32 ? 4 : 2); };
+    const auto end = [&](const RowsView& r) { return r.p + ((n - 1) * r.ld + width) * size(r); };
+    if (!(a.p < end(b) && b.p < end(a))) return false;
+    const int64_t stride = a.ld * size(a);
+    if (stride != b.ld * size(b)) return true;
+    const int64_t d = b.p - a.p, first = -d / stride;
+    for (int64_t k = first - 1; k <= first + 1; k++)  // row i of a and row i + k of b
+        if (k > -n && k < n && d + k * stride < width * size(a) && d + k * stride > -width * size(b)) return true;
+    return false;
+}
+
+// Rows of a call on pages must not lie in the pages themselves.
+static int32_t check_apart(const fllm_pages* p, const RowsView& r, const char* name, int64_t n, int64_t width) {
+    if (n <= 0) return FLLM_OK;
+    const uint8_t* end = r.p + ((n - 1) * r.ld + width) * (r.type == FLLM_TYPE_F32 ? 4 : 2);
+    const uint64_t bytes = 2 * p->cell * (uint64_t)p->d.n_kv_heads * (uint64_t)p->d.n_pages * (uint64_t)p->d.n_layers;
+    return r.p < p->ptr + bytes && p->ptr < end ? fail(FLLM_E_ARG, "%s overlaps the pages", name) : FLLM_OK;
 }
 
 static int32_t check_call(fllm_batch* b, int32_t layer) {
@@ -340,6 +364,7 @@ extern "C" int32_t fllm_pages_append(fllm_batch* b, int32_t layer, const fllm_ro
     RowsView rk{}, rv{};
     if ((rc = check_rows(p->ctx, k, "k", b->view.n_rows, width, &rk))) return rc;
     if ((rc = check_rows(p->ctx, v, "v", b->view.n_rows, width, &rv))) return rc;
+    if ((rc = check_apart(p, rk, "k", b->view.n_rows, width)) || (rc = check_apart(p, rv, "v", b->view.n_rows, width))) return rc;
     if (b->view.n_rows == 0) return FLLM_OK;
     HIP_TRY(hipSetDevice(p->ctx->device));
     HIP_TRY(launch_pages_append(pages_view(p, layer), b->view, rk, rv, p->ctx->stream));
@@ -357,6 +382,7 @@ extern "C" int32_t fllm_pages_read(fllm_batch* b, int32_t layer, int32_t new_onl
     if (!k && !v) return fail(FLLM_E_NULL, "k and v must not both be null");
     if (k && (rc = check_rows(p->ctx, k, "k", n, width, &rk))) return rc;
     if (v && (rc = check_rows(p->ctx, v, "v", n, width, &rv))) return rc;
+    if ((k && (rc = check_apart(p, rk, "k", n, width))) || (v && (rc = check_apart(p, rv, "v", n, width)))) return rc;
     if (k && v && overlap(rk, rv, n, width)) return fail(FLLM_E_ARG, "k and v overlap");
     if (!new_only && b->view.n_seqs && b->plan.holes) return fail(FLLM_E_INVALID_OP, "pages before the window were given back");
     if (n == 0) return FLLM_OK;
@@ -374,6 +400,7 @@ extern "C" int32_t fllm_pages_attention(fllm_batch* b, int32_t layer, const fllm
     RowsView rq{}, ro{};
     if ((rc = check_rows(p->ctx, q, "q", b->view.n_rows, width, &rq))) return rc;
     if ((rc = check_rows(p->ctx, out, "out", b->view.n_rows, width, &ro))) return rc;
+    if ((rc = check_apart(p, rq, "q", b->view.n_rows, width)) || (rc = check_apart(p, ro, "out", b->view.n_rows, width))) return rc;
     if (overlap(rq, ro, b->view.n_rows, width)) return fail(FLLM_E_ARG, "q and out overlap");
     if (!isfinite(scale)) return fail(FLLM_E_ARG_RANGE, "scale must be finite");
     if (!isfinite(softcap) || softcap < 0.0f) return fail(FLLM_E_ARG_RANGE, "softcap must be finite and not negative");
@@ -429,6 +456,18 @@ extern "C" int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d) {
     if ((rc = check_values(ctx, d->out_tokens, "out_tokens", nt))) return rc;
     if ((rc = check_values(ctx, d->out_counts, "out_counts", n))) return rc;
     if (n == 0) return FLLM_OK;
+    // the outputs are written while other sequences' inputs are still read
+    const uint8_t* outs[2] = {d->out_tokens->ptr, d->out_counts->ptr};
+    const uint64_t out_bytes[2] = {4 * (uint64_t)nt, 4 * (uint64_t)n};
+    const auto meet = [&](const uint8_t* p, uint64_t bytes, int o) { return p && bytes && p < outs[o] + out_bytes[o] && outs[o] < p + bytes; };
+    const auto rows_bytes = [&](const RowsView& r, int64_t m) { return m ? (uint64_t)((m - 1) * r.ld + d->vocab) * 4 : 0; };
+    for (int o = 0; o < 2; o++) {
+        const bool bad = meet(target.p, rows_bytes(target, nt), o) || meet(draft.p, rows_bytes(draft, nd), o) ||
+                         (d->n_draft && (meet(d->tokens->ptr, 4 * (uint64_t)nd, o) || meet(d->u_accept->ptr, 4 * (uint64_t)nd, o))) ||
+                         (d->counts && meet(d->counts->ptr, 4 * (uint64_t)n, o)) || meet(d->u_sample->ptr, 4 * (uint64_t)n, o) ||
+                         (o == 0 && meet(outs[1], out_bytes[1], 0));
+        if (bad) return fail(FLLM_E_ARG, "%s overlaps another argument", o ? "out_counts" : "out_tokens");
+    }
     HIP_TRY(hipSetDevice(ctx->device));
     DraftView v{};
     v.n_seqs = d->n_seqs;

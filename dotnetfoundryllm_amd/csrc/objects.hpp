@@ -34,6 +34,22 @@ struct Workspace {
     uint64_t n_cnt = 0;
 };
 
+// A batch's arrays on the device and the pinned block that they are copied from; `sent` says when the last copy has
+// read it. Those of destroyed batches serve the next ones: calls still under way read `dev` before the stream's
+// next copy into it.
+struct BatchBlock {
+    uint8_t *dev = nullptr, *pin = nullptr;
+    uint64_t cap = 0;
+    hipEvent_t sent = nullptr;
+    bool in_flight = false;
+};
+struct SpareBlocks {
+    static constexpr size_t kMost = 8;
+    std::mutex mu;
+    BatchBlock blocks[kMost];
+    size_t n = 0;
+};
+
 }  // namespace fllm
 
 struct fllm_ctx {
@@ -45,6 +61,7 @@ struct fllm_ctx {
     uint8_t* scratch = nullptr;  // this device's address of the no-allocation scratch array
     hipError_t scratch_err = hipSuccess;  // why it could not be resolved, if so
     fllm::Workspace ws;          // partial results of the paged attention and of the draft check
+    fllm::SpareBlocks spare;
 };
 
 struct fllm_buf {

@@ -432,8 +432,9 @@ FLLM_API int32_t fllm_batch_destroy(fllm_batch* b);
 
 /* The calls below are enqueued on the context's stream. Their rows lie in buffers of the same context;
  * rows behind the batch's last one are neither read nor written. layer outside [0, n_layers) ->
- * FLLM_E_ARG_RANGE; rows that do not fit their buffer, misaligned offsets or strides -> FLLM_E_ARG; other
- * element types -> FLLM_E_NOT_SUPPORTED. */
+ * FLLM_E_ARG_RANGE; rows that do not fit their buffer or reach into the pages, misaligned offsets or strides ->
+ * FLLM_E_ARG; other element types -> FLLM_E_NOT_SUPPORTED. Two operands that must not overlap may be columns of one
+ * matrix (equal strides) or lie apart. */
 
 /* Writes the new tokens' keys and values (rows of n_kv_heads * head_dim) into their pages. */
 FLLM_API int32_t fllm_pages_append(fllm_batch* b, int32_t layer, const fllm_rows* k, const fllm_rows* v);
@@ -471,8 +472,8 @@ typedef struct fllm_draft_desc {
     fllm_buf* out_tokens;    /* int32 [n_seqs][n_draft + 1]: the kept tokens, the drawn one, then -1 */
     fllm_buf* out_counts;    /* int32 [n_seqs]: kept tokens */
 } fllm_draft_desc;
-/* Enqueued on the context's stream. Negative sizes, vocab < 1 -> FLLM_E_ARG_RANGE; buffers too small,
- * misaligned rows -> FLLM_E_ARG; other types than F32, vocabularies above 1048576 -> FLLM_E_NOT_SUPPORTED. */
+/* Enqueued on the context's stream. Negative sizes, vocab < 1 -> FLLM_E_ARG_RANGE; buffers too small, misaligned
+ * rows, outputs that overlap another argument -> FLLM_E_ARG; other types than F32, vocabularies above 1048576 -> FLLM_E_NOT_SUPPORTED. */
 FLLM_API int32_t fllm_draft_verify(fllm_ctx* ctx, const fllm_draft_desc* d);
 
 /* ---- per-kernel timing of the decode step ----------------------------------- */

@@ -505,8 +505,76 @@ def test_draft_verify_refuses(ctx):
     with pytest.raises(F.ArgumentException):
         F.draft_verify(ctx, 1, 1, 8, **{**ok, "out_tokens": tiny})
     F.draft_verify(ctx, 0, 1, 8, **ok)
-    for x in (b, tiny):
+    ids, kept = F.DeviceBuffer(ctx, 64), F.DeviceBuffer(ctx, 64)
+    b.write(np.zeros(64, np.float32))
+    for same in ({"out_tokens": b}, {"out_counts": b}, {"out_counts": ids}):  # outputs that are read or written elsewhere too
+        with pytest.raises(F.ArgumentException):
+            F.draft_verify(ctx, 1, 1, 8, **{**ok, "out_tokens": ids, "out_counts": kept, **same})
+    F.draft_verify(ctx, 1, 1, 8, **{**ok, "out_tokens": ids, "out_counts": kept})
+    ctx.sync()
+    assert list(ids.read(8, np.int32)) == [7, -1] and list(kept.read(4, np.int32)) == [0]
+    for x in (b, tiny, ids, kept):
         x.close()
+
+
+@pytest.mark.parametrize("cache", TYPES)
+def test_operands_that_are_columns_of_one_matrix(make, cache):
+    """q, k and v, the rows read back and the outputs as columns of one matrix; what shares memory is refused."""
+    kv, heads, hd = 2, 4, 64
+    s = make(cache, kv, hd, 32, [3, 50], [40, 50], seed=11)
+    k, v = s.fill()
+    b, w, wq, n = s.batch(heads), kv * hd, heads * hd, 53
+    ld = 2 * (w + wq)
+    x = s.rng.standard_normal((n, ld)).astype(np.float32)
+    buf = F.DeviceBuffer(s.ctx, x.nbytes)
+    s.bufs.append(buf)
+    buf.write(x)
+    part = lambda at: F.Rows(buf, ld, F.F32, 4 * at)  # noqa: E731
+    b.append(1, part(wq), part(wq + w))
+    b.attention(1, part(0), part(wq + 2 * w), 0.125)
+    b.read(1, part(wq), part(wq + w), new_only=True)
+    s.ctx.sync()
+    got = buf.read(x.nbytes).reshape(n, ld)
+    assert np.array_equal(got[:, :wq], x[:, :wq])
+    fresh = [stored(x[:, a:a + w].reshape(n, kv, hd), cache) for a in (wq, wq + w)]
+    for a, f in zip((wq, wq + w), fresh):
+        assert np.array_equal(got[:, a:a + w], f.reshape(n, w).astype(np.float32))
+    for lo, hi, i, pos0 in ((0, 3, 0, 37), (3, 53, 1, 0)):
+        ki, vi = (np.concatenate([old[i][:pos0], f[lo:hi]]) for old, f in zip((k, v), fresh))
+        want = attend(x[lo:hi, :wq].reshape(-1, heads, hd).astype(np.float64), ki, vi, 2, pos0, F.NO_WINDOW, 0.125, 0.0)
+        check(got[lo:hi, wq + 2 * w:].astype(np.float64), want, "f32")
+    for at in (0, 4, wq - 4, ld - 4):
+        if at + wq <= ld or at == ld - 4:
+            with pytest.raises(F.ArgumentException):
+                b.attention(1, part(0), part(at), 0.125)
+    with pytest.raises(F.ArgumentException):
+        b.read(1, part(0), part(w - 4), new_only=True)
+    inside = F.Rows(s.mem, wq)
+    for call in (lambda: b.append(1, inside, part(0)), lambda: b.append(1, part(0), inside), lambda: b.read(1, inside, None, new_only=True),
+                 lambda: b.attention(1, inside, part(0), 1.0), lambda: b.attention(1, part(0), inside, 1.0)):
+        with pytest.raises(F.ArgumentException):
+            call()
+
+
+def test_batches_reuse_memory_of_destroyed_ones(make):
+    """Batches that come and go while calls on them are under way."""
+    s = make("f16", 1, 64, 16, [1, 20], [500, 60], seed=12)
+    k, v = s.fill()
+    q = s.put(s.rng.standard_normal((21, 256)), "f32")
+    host = from_bits(q.host[0][:21, :256], "f32")
+    outs = [s.put(np.zeros((21, 256)), "f32") for _ in range(30)]
+    for i, o in enumerate(outs):
+        length = [500 - i, 60 - i]
+        b = s.pages.batch(4)
+        b.set(s.new, length, s.tables)
+        b.attention(1, q, o, 0.125)
+        b.close()
+    s.ctx.sync()
+    for i in (0, 1, 14, 29):
+        got = s.get(outs[i], "f32")
+        for lo, hi, j in ((0, 1, 0), (1, 21, 1)):
+            ln = (500 - i, 60 - i)[j]
+            check(got[lo:hi], attend(host[lo:hi].reshape(-1, 4, 64), k[j][:ln], v[j][:ln], 4, ln - (hi - lo), F.NO_WINDOW, 0.125, 0.0), "f32")
 
 
 def test_wrapped_buffers(ctx):
