@@ -356,6 +356,14 @@ extern "C" int32_t fllm_buf_wrap(fllm_ctx* ctx, void* device_ptr, uint64_t nbyte
     *out = nullptr;
     NOT_NULL(device_ptr);
     if ((uintptr_t)device_ptr % 16 != 0) return fail(FLLM_E_ARG, "device_ptr must be 16-byte aligned");
+    hipPointerAttribute_t at{};
+    if (hipPointerGetAttributes(&at, device_ptr) != hipSuccess) {
+        (void)hipGetLastError();
+        return fail(FLLM_E_ARG, "device_ptr is no memory that this HIP runtime knows");
+    }
+    if (at.type != hipMemoryTypeDevice && at.type != hipMemoryTypeManaged) return fail(FLLM_E_ARG, "device_ptr is not device memory");
+    if (at.type == hipMemoryTypeDevice && at.device != ctx->device)
+        return fail(FLLM_E_ARG, "device_ptr lies on device %d, the context on %d", at.device, ctx->device);
     fllm_buf* b = new (std::nothrow) fllm_buf();
     if (!b) return fail(FLLM_E_OOM, "out of host memory");
     b->ctx = ctx;

@@ -3,6 +3,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
 #include <mutex>
 #include <new>
 #include <vector>
@@ -275,8 +276,9 @@ static hipError_t workspace_room(fllm_ctx* ctx, uint64_t part_bytes, uint64_t n_
         if (w.part) hipFree(w.part);
         w.part = nullptr;
         w.part_bytes = 0;
-        e = hipMalloc(&w.part, part_bytes + part_bytes / 2);
-        if (e == hipSuccess) w.part_bytes = part_bytes + part_bytes / 2;
+        const uint64_t want = part_bytes + std::min<uint64_t>(part_bytes / 2, (uint64_t)64 << 20);
+        e = hipMalloc(&w.part, want);
+        if (e == hipSuccess) w.part_bytes = want;
     }
     if (e == hipSuccess && n_cnt > w.n_cnt) {
         if (w.cnt) hipFree(w.cnt);

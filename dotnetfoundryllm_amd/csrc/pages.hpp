@@ -51,10 +51,6 @@ struct AttnWork {
     void* images;
     float* image_units;
 };
-// bytes of the images of one kv head's 64 keys; wide: F32 rows of q or out
-inline uint64_t attend_image_bytes(int hd, bool wide) {
-    return (uint64_t)(hd <= 64 ? 64 : hd <= 128 ? 128 : 256) * kKeyStep * 2 * 2 * (wide ? 2 : 1);
-}
 hipError_t launch_pages_attention(const PagesView& pg, const BatchView& b, const AttnWork& w, const RowsView& q,
                                   const RowsView& out, float scale, float softcap, hipStream_t st);
 
@@ -83,21 +79,11 @@ int draft_segments(int n_seqs, int vocab, int n_cu, int* seg, int* runs);
 hipError_t launch_draft_verify(const DraftView& d, int seg, int n_seg, int runs, double* part, unsigned* cnt, hipStream_t st);
 
 // ---- elements ---------------------------------------------------------------------------
-__device__ __forceinline__ float row_elem(const RowsView& r, int64_t i) {
-    if (r.type == FLLM_TYPE_F32) return ((const float*)r.p)[i];
-    if (r.type == FLLM_TYPE_F16) return (float)((const _Float16*)r.p)[i];
-    return bf16_exact(((const uint16_t*)r.p)[i]);
-}
 // round to nearest even; a NaN stays one
 __device__ __forceinline__ uint16_t bf16_round(float f) {
     const uint32_t u = __float_as_uint(f);
     if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)((u >> 16) | 0x40u);
     return (uint16_t)((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
-}
-__device__ __forceinline__ void row_store(const RowsView& r, int64_t i, float f) {
-    if (r.type == FLLM_TYPE_F32) ((float*)r.p)[i] = f;
-    else if (r.type == FLLM_TYPE_F16) ((_Float16*)r.p)[i] = (_Float16)f;
-    else ((uint16_t*)r.p)[i] = bf16_round(f);
 }
 
 }  // namespace fllm

@@ -42,7 +42,7 @@ typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 enum { DPP_ROR4 = 0x124, DPP_ROR8 = 0x128 };  // rotation within 16 lanes
-constexpr float kNoScore = -1e30f;  // the running maximum before any key
+constexpr float kNoScore = -3e38f;  // the running maximum before any key: below finite scores of any size that q k may have
 
 union H8 {
     h8 v;
@@ -129,7 +129,6 @@ __device__ __forceinline__ H8 codes8(uint32_t a, uint32_t b, int half) {
     return r;
 }
 
-// x as fp16 halves: one rounded to nearest, or a high and a low one (both cut, together 21 to 22 bits)
 // Mixed-precision multiply-adds on half SEL of a word: a b of two halves, a b of a half and a float, x - a.
 template <int SEL>
 __device__ __forceinline__ float mix_mul(uint32_t a, uint32_t b) {
@@ -162,6 +161,7 @@ __device__ __forceinline__ void split2(float x, float y, h2* hi, h2* lo) {
     *lo = b.h;
 }
 
+// x as fp16 halves: one rounded to nearest, or a high and a low one (both cut, together 21 to 22 bits)
 template <int NP>
 __device__ __forceinline__ void split4(const f4 x, h2 out[NP][2]) {
     for (int i = 0; i < 2; i++) {
@@ -215,10 +215,9 @@ __device__ __forceinline__ void softcap_n(V& s, float us, float cap) {
         s[i] = cap * __uint_as_float((__float_as_uint(q) & big) | (__float_as_uint(p) & ~big));
     }
 }
-template <typename V>
-__device__ __forceinline__ void softcap16(V& s, float us, float cap) {
-    softcap_n<16, true>(s, us, cap);
-}
+// Weights are exp2(us s - m) in one rounding. Where a maximum m is so large that its own rounding shows (2^-24 of
+// 2^20 and more), the products are rounded first, so that the largest score's weight is 1; m is that rounded product.
+__device__ __forceinline__ bool is_far(float m) { return __any(m > kNoScore && fabsf(m) >= 0x1p20f); }
 
 __device__ __forceinline__ f4 load_row4(const RowsView& r, int64_t i) {
     if (r.type == FLLM_TYPE_F32) return *(const f4*)(r.p + 4 * i);
@@ -581,6 +580,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ?
             const float down = __builtin_amdgcn_exp2f(mx[m] - nm);
             mx[m] = nm;
             float l = 0.0f;
+            if (is_far(nm)) {
+                for (int i = 0; i < RUN; i++) s[m][i] *= us;
+                us = 1.0f;
+            }
             for (int i = 0; i < RUN; i++) {
                 s[m][i] = __builtin_amdgcn_exp2f(fmaf(s[m][i], us, -nm));
                 l += s[m][i];
@@ -1129,7 +1132,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         if (QUANT) us *= ik;
         if (a.softcap > 0.0f) {
 #pragma unroll
-            for (int t = 0; t < T; t++) softcap16(s[t], us, a.softcap * kLog2e);
+            for (int t = 0; t < T; t++) softcap_n<16, true>(s[t], us, a.softcap * kLog2e);
             us = 1.0f;
         }
         const int hide_hi = pos - k0 - 8 * h, hide_lo = low - k0 - 8 * h;
@@ -1160,6 +1163,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
         float wunit = wbits;
         if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
+        if (is_far(mx)) {
+#pragma unroll
+            for (int t = 0; t < T; t++) s[t] *= us;
+            us = 1.0f;
+        }
 #pragma unroll
         for (int t = 0; t < T; t++)
             for (int i = 0; i < 16; i++) {
@@ -1420,6 +1428,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         float wunit = wbits;
         if (SRC == SRC_IMAGE) wunit *= ldexpf(1.0f, max(ev, -7) - max(vexp, -7));  // the step's own units to o's
         float w[8], l = 0.0f;
+        if (is_far(mx)) {
+            for (int i = 0; i < 8; i++) s[i] *= us;
+            us = 1.0f;
+        }
         for (int i = 0; i < 8; i++) {
             s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], us, -mx));
             l += s[i];

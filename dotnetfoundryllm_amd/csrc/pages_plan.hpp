@@ -189,6 +189,11 @@ constexpr int kAttnTile[kAttnClasses] = {4, 8, 16, 32, 128, 128};
 constexpr int kAttnSplit[kAttnClasses] = {128, 128, 128, 128, 32, 32};
 constexpr int kImageTiles = 4;  // tiles from which images pay
 constexpr int kImageRun = 4;    // key steps of an image item
+constexpr uint64_t kImageBytes = (uint64_t)4 << 30;  // a batch's images at most; beyond, every tile turns the codes itself
+// bytes of the images of one kv head's key step; wide: F32 rows of q or out
+inline uint64_t attend_image_bytes(int hd, bool wide) {
+    return (uint64_t)(hd <= 64 ? 64 : hd <= 128 ? 128 : 256) * kKeyStep * 2 * 2 * (wide ? 2 : 1);
+}
 
 struct AttnPlan {
     std::vector<AttnItem> items[kAttnClasses];  // tiles of up to kAttnTile[c] rows
@@ -254,13 +259,19 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, b
     const int group = n_heads / n_kv;
     p->part_rows = p->images = 0;
     p->image_items.clear();
+    const auto imaged = [&](const SeqPlan& s) { return quant && (int64_t)s.n_new * group > (kImageTiles - 1) * kAttnTile[kAttnMany]; };
+    const auto first_image = [&](const SeqPlan& s) { return std::max<int64_t>(0, (int64_t)s.len - s.n_new - window + 1) / kKeyStep; };
+    uint64_t steps_imaged = 0;
+    for (const SeqPlan& s : b.seqs)
+        if (imaged(s)) steps_imaged += (uint64_t)((s.len - 1) / kKeyStep + 1 - first_image(s));
+    const bool images = steps_imaged * (uint64_t)n_kv * attend_image_bytes(head_dim, true) <= kImageBytes;
     // the smallest tile that holds the sequence's rows; an F16 cache has no use for the two smallest (pages_attend.hpp)
     const auto class_of = [&](const SeqPlan& s) {
         const int64_t rows = (int64_t)s.n_new * group;
         int c = quant ? 0 : 2;
         while (c < kAttnMany && rows > kAttnTile[c]) c++;
         if (c == 3 && head_dim > 128) c = 2;  // wide heads leave no registers for two tiles of 16: one after the other
-        return quant && rows > (kImageTiles - 1) * kAttnTile[kAttnMany] ? kAttnImage : c;
+        return images && imaged(s) ? kAttnImage : c;
     };
     // two workgroups are resident on a CU, one of heads wider than 128
     const int64_t slots = (head_dim > 128 ? 1 : 2) * (int64_t)n_cu;
@@ -299,12 +310,11 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, b
         int64_t image = 0;
         if (s.n_new && c == kAttnImage) {
             const int64_t low = std::max<int64_t>(0, (int64_t)s.len - s.n_new - window + 1);
-            const int g0 = (int)(low / kKeyStep), g1 = (s.len - 1) / kKeyStep + 1;
+            const int g0 = (int)first_image(s), g1 = (s.len - 1) / kKeyStep + 1;
             image = p->images - g0;
             for (int g = g0; g < g1; g += kImageRun)
                 p->image_items.push_back({i * b.tab_w, s.len, (int)low, g * kKeyStep, std::min(kImageRun, g1 - g), (int)(image + g), {0, 0}});
             p->images += g1 - g0;
-            if (p->images > INT32_MAX / 4 / n_kv) return false;
         }
         if (s.n_new)
             attn_items(s, i, i * b.tab_w, (int)image, group, window, c, c >= kAttnMany ? many : std::max(few, join_steps(s, group, window, c, quant)),

@@ -319,7 +319,8 @@ FLLM_API int32_t fllm_buf_create(fllm_ctx* ctx, uint64_t nbytes, fllm_buf** out)
  * a larger allocation. device_ptr is a 16-byte aligned address on the context's device; the caller frees
  * the memory after fllm_buf_destroy and after the calls that use it have run (fllm_ctx_sync). Calls on
  * the buffer run on the context's stream and know no other: work on other streams is ordered by the
- * caller. No counterpart in the reference. */
+ * caller. Misaligned addresses, host memory and memory of another device -> FLLM_E_ARG. No counterpart in the
+ * reference. */
 FLLM_API int32_t fllm_buf_wrap(fllm_ctx* ctx, void* device_ptr, uint64_t nbytes, fllm_buf** out);
 FLLM_API int32_t fllm_buf_destroy(fllm_buf* b);
 FLLM_API int32_t fllm_buf_write(fllm_buf* b, uint64_t offset, const void* src, uint64_t n);

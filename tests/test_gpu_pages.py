@@ -590,6 +590,9 @@ def test_wrapped_buffers(ctx):
     assert list(whole.read(24, offset=76)) == [19, 9, 9, 9, 9, 24]
     with pytest.raises(F.ArgumentException):
         F.DeviceBuffer.wrap(ctx, base.value + 4, 16)
+    host = np.zeros(64, np.float32)
+    with pytest.raises(F.ArgumentException):
+        F.DeviceBuffer.wrap(ctx, (host.ctypes.data + 15) // 16 * 16, 16)
     x, y = F.DeviceBuffer(ctx, 128), F.DeviceBuffer(ctx, 128)
     with pytest.raises(F.ArgumentException):  # 8 x 32 floats fill it: nothing behind them
         F.gemv(ctx, F.F32, w, 8, 32, x, y)
@@ -652,7 +655,7 @@ def test_attention_of_other_magnitudes(make, cache, act, new, length):
     are relative to the outputs; scores stay of size 1."""
     for scale, of_k, of_v, of_q in ((-0.125, 1, 1, 1), (0.0, 1, 1, 1), (0.125, 1, 2.0 ** -18, 1), (0.125, 1, 10000, 1),
                                     (0.125 * 2.0 ** 12, 2.0 ** -12, 1, 1), (0.125 * 2.0 ** -90, 1, 1, 2.0 ** 90),
-                                    (0.125 * 2.0 ** 90, 1, 1, 2.0 ** -90)):
+                                    (0.125 * 2.0 ** 90, 1, 1, 2.0 ** -90), (1.0, 0, 1, 2.0 ** 120)):
         s = make(cache, 2, 64, 32, new, length, seed=5)
         k, v = s.fill(of_k, of_v)
         q = s.rng.standard_normal((sum(new), 6 * 64)) * of_q
@@ -687,6 +690,20 @@ def test_attention_over_a_shared_prefix(make, cache):
     part = [[np.concatenate([a[:64], a[lo:hi]]) for lo, hi in ((64, 70), (70, 81), (81, 151))] for a in x]
     k, v = ([stored(a, cache).reshape(-1, 2, 64) for a in p] for p in part)
     for got, want in attention_of(s, k, v, 4):
+        check(got, want, "f32")
+
+
+@pytest.mark.parametrize("cache,new,length", [("f16", 1, 50), ("q8_0", 1, 50), ("q8_0", 100, 100), ("q4_0", 500, 500)])
+def test_attention_of_far_scores(make, cache, new, length):
+    """Scores of -1e34 and less are scores: the largest of them has the weight."""
+    s = make(cache, 1, 32, 16, [new], [length], seed=9)
+    k, v = s.fill()
+    down = np.full((length, 32), -1.0, np.float32) * (1 + np.arange(length)[::-1, None] // 16).astype(np.float32)  # -n in page n from the end
+    b = s.batch(1, new=[length])
+    b.append(1, s.put(down, "f32"), s.put(v[0].reshape(length, 32), "f32"))
+    v = [stored(v[0].reshape(length, 32).astype(np.float32), cache).reshape(length, 1, 32)]
+    q = np.full((new, 32), 2.0 ** 114)
+    for got, want in attention_of(s, [stored(down, cache).reshape(length, 1, 32)], v, 1, scale=1.0, q=q):
         check(got, want, "f32")
 
 
