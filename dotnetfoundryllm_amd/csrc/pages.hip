@@ -314,8 +314,10 @@ int log2_up(int n) {
     return k;
 }
 
-// A tile of few rows has little work for 256 threads: one wave starts sooner and leaves the CU to others.
-int threads_for(const PagesView& pg, int rows) { return rows * (pg.hd >> 5) <= 16 ? 64 : 256; }
+// A tile of few rows has little work for 256 threads: one wave starts sooner and leaves the CU to others (64 sequences of 8
+// heads of 128, Q8_0, in and out, in us with 256 and 64 threads: 1 row 9.5 and 8.7, 4 rows 16.3 and 13.3, 8 rows 20.5
+// and 19.1).
+int threads_for(const PagesView& pg, int rows) { return rows * (pg.hd >> 5) <= 32 ? 64 : 256; }
 
 // The heads of a page follow each other, so that what lies side by side in the dense rows moves at the same time
 // (8 sequences of 3000 to 16000 positions, 8 heads of 256, Q8_0 to F16: 217 us, and 249 with the pages of a head in

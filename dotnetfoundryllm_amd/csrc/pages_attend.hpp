@@ -401,14 +401,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ?
             vf[d] = *(const uv*)(vp + (uint32_t)((d < (TYPE == FLLM_TYPE_Q4_0 ? nb : 2 * nb) ? d : 0) * 16 * P * VE));
     };
     const int first = it.k0 + wave * STEP;
-    constexpr bool AHEAD = !(QUANT && TM == 2 && HDP > 64);  // there the registers do not allow it
     if (first < it.k1) {
         pages_at(first);
-        if (AHEAD) {
-            load_k(first);
-            load_v(first);
-            pages_at(first + 4 * STEP < it.k1 ? first + 4 * STEP : first);
-        }
+        load_k(first);
+        load_v(first);
+        pages_at(first + 4 * STEP < it.k1 ? first + 4 * STEP : first);
     }
 
     // q as fp16 halves in LDS, 16 lanes a row: every row scaled by the power of two 2^e that brings its largest
@@ -489,11 +486,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ?
         const int kv = k0 + ksub * g;
         // unconditionally, or the waits for this step's loads would wait for the next one's too: the last step again
         const int next = k0 + 4 * STEP < it.k1 ? k0 + 4 * STEP : k0;
-        if (!AHEAD) {
-            load_k(k0);
-            load_v(k0);
-            pages_at(next);
-        }
         float s[TM][RUN];
 #pragma unroll
         for (int m = 0; m < TM; m++)
@@ -527,7 +519,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ?
                 }
                 for (int e = 0; e < 4; e++) s[m][4 * t + e] = acc[e];
             }
-        if (AHEAD) load_k(next);
+        load_k(next);
 
         const bool edge = k0 < all_lo || k0 + STEP > all_hi;
         if (edge) {
@@ -629,10 +621,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HDP > 128 ?
                 }
             }
         }
-        if (AHEAD) {
-            load_v(next);
-            pages_at(next + 4 * STEP < it.k1 ? next + 4 * STEP : next);
-        }
+        load_v(next);
+        pages_at(next + 4 * STEP < it.k1 ? next + 4 * STEP : next);
     }
 
     // the four waves' results, a row tile at a time
@@ -1521,7 +1511,7 @@ hipError_t launch_items(AttnArgsP a, const AttnWork& w, hipStream_t st) {
             else if (whole) go(std::integral_constant<int, SRC_PAGES>());
             else go(std::integral_constant<int, SRC_PARTS>());
         } else if (c == 3) {
-            if constexpr (HDP <= 128) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2, 16>), grid(c), dim3(256), 0, st, a);
+            if constexpr (!QUANT && HDP <= 128) hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 2, 16>), grid(c), dim3(256), 0, st, a);
         } else if (c == 2) {
             hipLaunchKernelGGL((k_attend_few<TYPE, HDP, NP, 1, 16>), grid(c), dim3(256), 0, st, a);
         } else {

@@ -187,7 +187,10 @@ constexpr int kKeyStep = 64;
 constexpr int kAttnClasses = 6, kAttnMany = 4, kAttnImage = 5;
 constexpr int kAttnTile[kAttnClasses] = {4, 8, 16, 32, 128, 128};
 constexpr int kAttnSplit[kAttnClasses] = {128, 128, 128, 128, 32, 32};
-constexpr int kImageTiles = 4;  // tiles from which images pay
+// Tiles from which images pay. One sequence of 4000, 8 kv heads, Q8_0, in us with images and without: heads of 128,
+// BF16 rows: 2 tiles 57.0 and 49.0, 4 tiles 64.7 and 58.7, 8 tiles 76.7 and 73.1; heads of 256, F32 rows: 4 tiles 106.5 and
+// 90.5, 8 tiles 200 and 216. Two of 2000, Q4_0, F32 rows: 8 tiles 103.6 and 103.2.
+constexpr int kImageTiles = 8;
 constexpr int kImageRun = 4;    // key steps of an image item
 constexpr uint64_t kImageBytes = (uint64_t)4 << 30;  // a batch's images at most; beyond, every tile turns the codes itself
 // bytes of the images of one kv head's key step; wide: F32 rows of q or out
@@ -270,7 +273,10 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, b
         const int64_t rows = (int64_t)s.n_new * group;
         int c = quant ? 0 : 2;
         while (c < kAttnMany && rows > kAttnTile[c]) c++;
-        if (c == 3 && head_dim > 128) c = 2;  // wide heads leave no registers for two tiles of 16: one after the other
+        // 17 to 32 rows: two tiles of 16, except where one pass over the keys is faster (8 sequences of 4000, 20 and 32
+        // rows, in us in one pass and in two: F16 38.3 and 41.5, 41.2 and 41.5; Q8_0 30.9 and 31.4, 33.8 and 31.9).
+        // Wide heads leave no registers for it.
+        if (c == 3 && (quant || head_dim > 128)) c = 2;
         return images && imaged(s) ? kAttnImage : c;
     };
     // two workgroups are resident on a CU, one of heads wider than 128

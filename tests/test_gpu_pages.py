@@ -638,6 +638,10 @@ def attention_of(s, k, v, heads, act="f32", window=F.NO_WINDOW, scale=None, soft
     (1, 2, 256, 128, [65], [6000], None, 0.0),
     (1, 1, 128, 64, [1], [70000], None, 0.0),             # one row over very many keys
     (1, 16, 32, 16, [1, 1], [20000, 31], 19990, 0.0),
+    (1, 8, 256, 64, [120], [361], 150, 50.0),             # 960 rows and more: a quantised cache's keys turned once
+    (1, 9, 192, 16, [101, 2], [130, 77], None, 0.0),
+    (2, 20, 128, 128, [100], [700], None, 0.0),
+    (1, 12, 96, 32, [80, 77], [80, 400], 99, 0.0),
     (1, 32, 128, 64, [2], [4000], None, 0.0),
 ])
 def test_attention_over_longer_ranges(make, cache, kv, heads, hd, page, new, length, window, softcap):
