@@ -694,11 +694,14 @@ enum { SRC_PAGES, SRC_PARTS, SRC_IMAGE, SRC_CODES };
 constexpr int kManyRows = kAttnTile[kAttnClasses - 1], kManySplit = kAttnSplit[kAttnClasses - 1];
 
 // LDS planes of a step: K [keys][HDP], V [HDP][keys], halves in chunks of 8. Chunk c of a row lies at
-// c ^ swizzle(row), so that the 16 rows that a quarter of a wave reads cover the banks once.
+// c ^ swizzle(row), so that the 16 lanes that read together (0 to 3, 12 to 15 and 20 to 27, the others of the first 32,
+// and so on) cover the banks once.
 template <int HDP> __device__ __forceinline__ int k_swizzle(int key) {
     return HDP == 64 ? key >> 1 & 7 : HDP == 128 ? key & 15 : (key & 3) | (key >> 1 & 12);  // 256: k_attend_wide's rows
 }
-template <int STEP> __device__ __forceinline__ int v_swizzle(int d) { return STEP == 64 ? d >> 1 & 7 : d >> 2 & 3; }
+template <int STEP> __device__ __forceinline__ int v_swizzle(int d) {
+    return STEP == 64 ? d >> 1 & 7 : ((d >> 3 ^ d >> 2) & 1) << 1 | (d >> 3 & 1);
+}
 template <int HDP>
 __device__ __forceinline__ int k_chunk(int key, int c) {
     return key * (HDP / 8) + (c ^ k_swizzle<HDP>(key));
