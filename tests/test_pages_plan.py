@@ -163,3 +163,34 @@ def test_long_sequences(lib):
     check(lib, [1], [n], 32, 8, NO_WINDOW)
     # rows and positions past 2^31 in all are refused
     assert plan(lib, [1] * 20, [n] * 20, np.repeat(table, 20, 0), 32, 8, 128, 128, n // 128) == N.E_ARG
+
+
+def test_images(lib):
+    """A quantised cache's keys are turned once for sequences of many rows, unless the images would be too large."""
+    def images(new, length, kind=N.Q8_0, hd=128, kv=8, window=NO_WINDOW):
+        n = -(-length // 128)
+        assert plan(lib, [new], [length], np.arange(n, dtype=np.int32)[None], 4 * kv, kv, hd, 128, n, window, kind=kind) == 0
+        check(lib, [new], [length], 4 * kv, kv, window)
+        total = C.c_int64()
+        lib.plan_images(None, C.byref(total))
+        return total.value
+
+    assert images(224, 4000) == 0 and images(225, 4000) == 63  # 7 tiles of 128 rows and one more
+    assert images(400, 4000, N.F16) == 0
+    assert images(300, 4000, window=500) == 63 - (4000 - 300 - 499) // STEP
+    per = 128 * STEP * 2 * 2 * 2 * 8  # bytes of a key step
+    most = (4 << 30) // per * STEP
+    assert images(225, most) == most // STEP and images(225, most + 1) == 0
+
+
+def test_a_join_is_worth_its_steps(lib):
+    """Few rows over a middling length: items of at least sqrt(steps rows / 16) steps once that is 4."""
+    def steps(length, heads, kv):
+        n = -(-length // 64)
+        assert plan(lib, [1], [length], np.arange(n, dtype=np.int32)[None], heads, kv, 128, 64, n) == 0
+        check(lib, [1], [length], heads, kv, NO_WINDOW)
+        a = np.concatenate(items(lib))
+        return max(-(-k1 // STEP) - k0 // STEP for k0, k1 in a[:, 3:5].tolist())
+
+    assert [steps(n, 32, 8) for n in (518, 2048, 4096, 8192)] == [2, 2, 4, 6]
+    assert steps(131071, 32, 8) > 8
