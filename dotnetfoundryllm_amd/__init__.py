@@ -209,7 +209,16 @@ class Rows:
     def __init__(self, buf, ld, tensor_type=F32, offset=0):
         self.buf = buf  # kept alive
         self.d = N.RowsDesc(buf.h, offset, ld, tensor_type, 0)
-        self.ref = C.byref(self.d)
+        self._ref = C.byref(self.d)
+
+    def desc(self):
+        self.d.buf = self.buf.h  # None once the buffer is closed
+        return self.d
+
+    @property
+    def ref(self):
+        self.desc()
+        return self._ref
 
 
 class PagedKvCache:
@@ -257,6 +266,8 @@ class PagedBatch:
     def _handle(self):
         if not self.h:
             raise ObjectDisposedException("PagedBatch")
+        if self.pages.memory is not None and not self.pages.memory.h:
+            raise ObjectDisposedException("the pages' memory")
         return self.h
 
     def set(self, new_tokens, lengths, tables):
@@ -297,7 +308,8 @@ def draft_verify(ctx, n_seqs, n_draft, vocab, target, tokens, u_accept, u_sample
     """Drafted tokens against the target's probabilities (fllm_draft_verify): kept tokens, then the drawn
     one, then -1 in out_tokens, their number in out_counts. target, draft: Rows; the others DeviceBuffers."""
     hd = lambda b: b.h if b is not None else None  # noqa: E731
-    d = N.DraftDesc(n_seqs, n_draft, vocab, 0, target.d, draft.d if draft is not None else N.RowsDesc(), hd(tokens),
+    rows = lambda r: r.desc() if r is not None else N.RowsDesc()  # noqa: E731
+    d = N.DraftDesc(n_seqs, n_draft, vocab, 0, rows(target), rows(draft), hd(tokens),
                     hd(counts), hd(u_accept), hd(u_sample), hd(out_tokens), hd(out_counts))
     _check(N.dev.fllm_draft_verify(ctx.h, C.byref(d)))
 

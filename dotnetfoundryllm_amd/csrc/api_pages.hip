@@ -84,6 +84,7 @@ extern "C" int32_t fllm_pages_create(fllm_ctx* ctx, const fllm_pages_desc* desc,
         hipError_t e = hipSetDevice(ctx->device);
         if (e == hipSuccess) e = hipMalloc(&p->ptr, bytes);
         if (e != hipSuccess) {
+            (void)hipGetLastError();
             delete p;
             return fail(e == hipErrorOutOfMemory ? FLLM_E_OOM : FLLM_E_DEVICE, "hipMalloc(%llu): %s", (unsigned long long)bytes,
                         hipGetErrorString(e));
@@ -164,6 +165,7 @@ static hipError_t batch_room(fllm_ctx* ctx, BatchBlock* b, uint64_t n) {
     e = hipMalloc(&b->dev, want);
     if (e == hipSuccess) e = hipHostMalloc((void**)&b->pin, want, hipHostMallocDefault);
     if (e == hipSuccess) b->cap = want;
+    else (void)hipGetLastError();  // reported here: not to be found by the next launch
     return e;
 }
 
@@ -197,18 +199,16 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
             return fail(FLLM_E_ARG, "the batch is too large");
         }
         b->plan.n_seqs = 0;  // empty until everything is on its way
-        // sequences, items, images, tables: parts of 16, 64, 32 and 4 bytes
-        constexpr int N = kAttnClasses + 3;
+        // sequences, items, images, tiles, starts, tables: parts of 16, 64, 32, 16 and 4 bytes
+        constexpr int N = kAttnClasses + 5;
         const void* from[N] = {pl.seqs.data()};
         uint64_t size[N] = {(pl.seqs.size() * sizeof(SeqPlan) + 63) / 64 * 64}, at[N + 1] = {0};
-        for (int i = 0; i < kAttnClasses; i++) {
-            from[1 + i] = b->attn.items[i].data();
-            size[1 + i] = b->attn.items[i].size() * sizeof(AttnItem);
-        }
-        from[N - 2] = b->attn.image_items.data();
-        size[N - 2] = b->attn.image_items.size() * sizeof(ImageItem);
-        from[N - 1] = pl.tables.data();
-        size[N - 1] = pl.tables.size() * sizeof(int32_t);
+        const auto part = [&](int i, const auto& v) { from[i] = v.data(), size[i] = v.size() * sizeof(v[0]); };
+        for (int i = 0; i < kAttnClasses; i++) part(1 + i, b->attn.items[i]);
+        part(N - 4, b->attn.image_items);
+        part(N - 3, pl.new_tiles);
+        part(N - 2, pl.first);
+        part(N - 1, pl.tables);
         for (int i = 0; i < N; i++) at[i + 1] = at[i] + size[i];
         hipError_t e = batch_room(p->ctx, &b->mem, at[N]);
         if (e != hipSuccess)
@@ -221,10 +221,11 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
         b->plan.n_seqs = n_plan_seqs;
         b->view.seqs = (const int4*)b->mem.dev;
         b->view.tables = (const int*)(b->mem.dev + at[N - 1]);
-        b->view.tab_w = pl.tab_w;
+        b->view.first = (const int*)(b->mem.dev + at[N - 2]);
+        b->view.new_tiles = (const int4*)(b->mem.dev + at[N - 3]);
         b->view.n_seqs = n_plan_seqs;
-        b->view.new_blocks = pl.new_blocks;
-        b->view.all_blocks = pl.all_blocks;
+        b->view.n_new_tiles = (int)pl.new_tiles.size();
+        b->view.n_blocks = (int)pl.tables.size();
         b->view.n_rows = pl.n_rows;
         b->view.max_new = pl.max_new;
         b->view.n_heads = b->n_heads;
@@ -234,7 +235,7 @@ extern "C" int32_t fllm_batch_set(fllm_batch* b, int32_t n_seqs, const int32_t* 
             b->work.n[i] = (int)b->attn.items[i].size();
         }
         b->work.part_rows = b->attn.part_rows;
-        b->work.image_items = (const ImageItem*)(b->mem.dev + at[N - 2]);
+        b->work.image_items = (const ImageItem*)(b->mem.dev + at[N - 4]);
         b->work.n_image_items = (int)b->attn.image_items.size();
         b->work.n_images = b->attn.images;
         return FLLM_OK;
@@ -289,6 +290,7 @@ static hipError_t workspace_room(fllm_ctx* ctx, uint64_t part_bytes, uint64_t n_
         if (e == hipSuccess) e = hipMemsetAsync(w.cnt, 0, n * sizeof(unsigned), ctx->stream);
         if (e == hipSuccess) w.n_cnt = n;
     }
+    if (e != hipSuccess) (void)hipGetLastError();
     return e;
 }
 

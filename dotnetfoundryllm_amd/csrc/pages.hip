@@ -24,19 +24,34 @@ struct Tile {
     uint64_t cell;  // the cell's offset
 };
 
-// The tile of sequence s that workgroup column bx covers; false where it covers none.
-__device__ __forceinline__ bool tile_of(const PagesView& pg, const BatchView& b, bool new_only, int s, int bx, int head,
-                                        Tile* t) {
-    const int4 q = b.seqs[s];
-    const int first = new_only ? q.z - q.y : 0;
-    const int pb = (first >> pg.page_log2) + bx;
-    const int lo = max(first, pb << pg.page_log2), hi = min(q.z, (pb + 1) << pg.page_log2);
-    if (lo >= hi) return false;
-    t->off = lo - (pb << pg.page_log2);
-    t->n = hi - lo;
-    t->row = (int64_t)(new_only ? q.x : q.w) + (lo - first);
-    t->cell = ((uint64_t)(uint32_t)b.tables[(int64_t)s * b.tab_w + pb] * pg.nkv + head) * pg.cell;
-    return true;
+// Tile `at` of the new tokens, one load away, or of all positions: page `at` of the sequences' pages, whose sequence a wave
+// finds with one load for up to 64 of them (203 us of the case at grid_of; 212 by halving).
+__device__ __forceinline__ Tile tile_of(const PagesView& pg, const BatchView& b, bool new_only, int at, int head) {
+    Tile t;
+    int page;
+    if (new_only) {
+        const int4 q = b.new_tiles[at];
+        t.off = q.x;
+        t.n = q.y;
+        t.row = q.z;
+        page = q.w;
+    } else {
+        int s = 0;  // the last sequence whose pages start at `at` or before
+        for (int n = b.n_seqs; n > 1;) {
+            const int step = (n + 63) >> 6, i = (int)(threadIdx.x & 63) * step;
+            const int k = __builtin_popcountll(__ballot(i < n && b.first[s + (i < n ? i : 0)] <= at)) - 1;
+            s += k * step;
+            n = min(step, n - k * step);
+        }
+        const int4 q = b.seqs[s];
+        const int pos = (at - (b.n_seqs > 1 ? b.first[s] : 0)) << pg.page_log2;
+        t.off = 0;
+        t.n = min(q.z - pos, 1 << pg.page_log2);
+        t.row = (int64_t)q.w + pos;
+        page = b.tables[at];
+    }
+    t.cell = ((uint64_t)(uint32_t)page * pg.nkv + head) * pg.cell;
+    return t;
 }
 
 __device__ __forceinline__ uint32_t half_bits(float f) {
@@ -131,10 +146,8 @@ __global__ __launch_bounds__(256) void k_pages_append(PagesView pg, BatchView b,
     const int P = 1 << pg.page_log2, nb = pg.hd >> 5;
     const RowsView& src = kind ? rv : rk;
     const int pitch = lds_pitch<TYPE>(pg.hd);
-    for (int s = blockIdx.z; s < b.n_seqs; s += gridDim.z)
-    for (int at = blockIdx.y; at < b.new_blocks; at += gridDim.y) {
-        Tile t;
-        if (!tile_of(pg, b, true, s, at, head, &t)) continue;
+    for (int at = blockIdx.y; at < b.n_new_tiles; at += gridDim.y) {
+        const Tile t = tile_of(pg, b, true, at, head);
         uint8_t* cell = (kind ? pg.v : pg.k) + t.cell;
         const int e = threadIdx.x & 3;
         for (int u = threadIdx.x >> 2; u < t.n << nb_log2; u += blockDim.x >> 2) {
@@ -222,11 +235,9 @@ __global__ __launch_bounds__(256) void k_pages_read(PagesView pg, BatchView b, b
     const int pitch = lds_pitch<TYPE>(pg.hd);
     constexpr int VB = v_bytes<TYPE>(), RUN = 16 / VB;
     constexpr int PER = TYPE == FLLM_TYPE_F16 ? 64 : TYPE == FLLM_TYPE_Q8_0 ? 32 : 16;
-    const int blocks = new_only ? b.new_blocks : b.all_blocks;
-    for (int s = blockIdx.z; s < b.n_seqs; s += gridDim.z)
-    for (int at = blockIdx.y; at < blocks; at += gridDim.y) {
-        Tile t;
-        if (!tile_of(pg, b, new_only, s, at, head, &t)) continue;
+    const int tiles = new_only ? b.n_new_tiles : b.n_blocks;
+    for (int at = blockIdx.y; at < tiles; at += gridDim.y) {
+        const Tile t = tile_of(pg, b, new_only, at, head);
         const uint8_t* cell = (kind ? pg.v : pg.k) + t.cell;
         if (kind) {
             const int lo0 = t.off / RUN, held = (t.off + t.n - 1) / RUN - lo0 + 1;
@@ -323,14 +334,12 @@ int threads_for(const PagesView& pg, int rows) { return rows * (pg.hd >> 5) <= 3
 
 // The heads of a page follow each other, so that what lies side by side in the dense rows moves at the same time
 // (8 sequences of 3000 to 16000 positions, 8 heads of 256, Q8_0 to F16: 217 us, and 249 with the pages of a head in
-// a row). The second and third dimension end at 65535: the kernels go on from there.
-dim3 grid_of(const PagesView& pg, const BatchView& b, int blocks) {
-    return dim3(2 * pg.nkv, blocks < 65535 ? blocks : 65535, b.n_seqs < 65535 ? b.n_seqs : 65535);
-}
+// a row). The second dimension ends at 65535: the kernels go on from there.
+dim3 grid_of(const PagesView& pg, int tiles) { return dim3(2 * pg.nkv, tiles < 65535 ? tiles : 65535); }
 
 template <int TYPE>
 hipError_t append(const PagesView& pg, const BatchView& b, const RowsView& k, const RowsView& v, hipStream_t st) {
-    const dim3 grid = grid_of(pg, b, b.new_blocks);
+    const dim3 grid = grid_of(pg, b.n_new_tiles);
     const size_t lds = (size_t)lds_pitch<TYPE>(pg.hd) << pg.page_log2;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)k_pages_append<TYPE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -342,7 +351,7 @@ hipError_t append(const PagesView& pg, const BatchView& b, const RowsView& k, co
 
 template <int TYPE, int EL>
 hipError_t read(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v, hipStream_t st) {
-    const dim3 grid = grid_of(pg, b, new_only ? b.new_blocks : b.all_blocks);
+    const dim3 grid = grid_of(pg, new_only ? b.n_new_tiles : b.n_blocks);
     const size_t lds = (size_t)lds_pitch<TYPE>(pg.hd) << pg.page_log2;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute((const void*)k_pages_read<TYPE, EL>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -379,7 +388,7 @@ hipError_t launch_pages_append(const PagesView& pg, const BatchView& b, const Ro
 
 hipError_t launch_pages_read(const PagesView& pg, const BatchView& b, bool new_only, const RowsView& k, const RowsView& v,
                              hipStream_t st) {
-    if ((new_only ? b.new_blocks : b.all_blocks) == 0) return hipSuccess;
+    if ((new_only ? b.n_new_tiles : b.n_blocks) == 0) return hipSuccess;
     switch (pg.type) {
         case FLLM_TYPE_F16: return read_both<FLLM_TYPE_F16>(pg, b, new_only, k, v, st);
         case FLLM_TYPE_Q8_0: return read_both<FLLM_TYPE_Q8_0>(pg, b, new_only, k, v, st);

@@ -15,14 +15,15 @@ struct PagesView {
     uint64_t cell;
     uint32_t scale_off;
 };
-// A batch on the device: the pages of sequence s at tables + s * tab_w, and per sequence
-// {first row of its new tokens, their number, its length, first row of its positions}.
+// A batch on the device: per sequence {first row of its new tokens, their number, its length, first row of its
+// positions} and where its pages start in `tables`; the pages with new tokens (PageTile).
 struct BatchView {
-    const int* tables;
     const int4* seqs;
-    int tab_w, n_seqs;
-    int new_blocks, all_blocks;  // most pages of a sequence that hold new tokens, that hold any
-    int n_rows, max_new;         // new tokens of all sequences, most of one
+    const int* first;
+    const int* tables;
+    const int4* new_tiles;
+    int n_seqs, n_new_tiles, n_blocks;  // n_blocks: pages of all sequences
+    int n_rows, max_new;                // new tokens of all sequences, most of one
     int n_heads, window;
 };
 struct RowsView {

@@ -70,27 +70,33 @@ struct SeqPlan {
     int row0, n_new, len, pos0;  // first new row, new tokens, positions, first row of the positions
 };
 
+// The new tokens of a sequence in one page: n positions from `off` on, whose rows start at `row`.
+struct PageTile {
+    int off, n, row, page;
+};
+
 struct BatchPlan {
     int n_seqs = 0, n_rows = 0, n_pos = 0;
-    int tab_w = 0;                       // pages of the longest sequence
-    int new_blocks = 0, all_blocks = 0;  // most pages of a sequence that hold new tokens, that hold any
     int max_new = 0;                     // most new tokens of a sequence
     bool holes = false;                  // some page before the windows was given back
     std::vector<SeqPlan> seqs;
-    std::vector<int32_t> tables;         // [n_seqs][tab_w], 0 where there is no page
+    std::vector<int32_t> first;          // where each sequence's pages start in `tables`; their number
+    std::vector<int32_t> tables;         // the sequences' pages one after the other, 0 where there is none
+    std::vector<PageTile> new_tiles;
     std::vector<uint8_t> uses;           // scratch: places that name a page (up to 2)
 };
 
 // Fills `p` from the arrays of fllm_batch_set, or says what is wrong with them.
 inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, const int32_t* n_new, const int32_t* lengths,
                           const int32_t* tables, int64_t ld, BatchPlan* p, BatchError* e) {
-    p->n_seqs = p->n_rows = p->n_pos = p->tab_w = p->new_blocks = p->all_blocks = p->max_new = 0;
+    p->n_seqs = p->n_rows = p->n_pos = p->max_new = 0;
     p->holes = false;
     p->seqs.clear();
-    p->tables.clear();
+    p->first.clear();
+    p->new_tiles.clear();
     e->code = FLLM_E_ARG_RANGE;
     const int P = d.page_size;
-    int64_t rows = 0, pos = 0;
+    int64_t rows = 0, pos = 0, all = 0;
     int wide = 0;
     for (int i = 0; i < n_seqs; i++) {
         const int n = n_new[i], len = lengths[i];
@@ -98,9 +104,9 @@ inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, 
             snprintf(e->text, sizeof(e->text), "sequence %d: %d new tokens, length %d (at most %d)", i, n, len, kPagesMaxLength);
             return e->code;
         }
-        const int blocks = (len + P - 1) / P, held = n ? blocks - (len - n) / P : 0;
+        const int blocks = (len + P - 1) / P;
         wide = blocks > wide ? blocks : wide;
-        p->new_blocks = held > p->new_blocks ? held : p->new_blocks;
+        all += blocks;
         p->max_new = n > p->max_new ? n : p->max_new;
         rows += n;
         pos += len;
@@ -115,15 +121,11 @@ inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, 
         snprintf(e->text, sizeof(e->text), "tables of %lld pages a sequence, %d are needed", (long long)ld, wide);
         return e->code;
     }
-    if ((int64_t)n_seqs * wide > INT32_MAX) {
-        e->code = FLLM_E_ARG;
-        snprintf(e->text, sizeof(e->text), "tables of %d sequences and %d pages", n_seqs, wide);
-        return e->code;
-    }
     p->uses.assign((size_t)d.n_pages, 0);
-    p->tables.assign((size_t)n_seqs * (size_t)wide, 0);
+    p->tables.assign((size_t)all, 0);  // at most n_pos
     p->seqs.reserve((size_t)n_seqs);
-    int r = 0, q = 0;
+    p->first.reserve((size_t)n_seqs + 1);
+    int r = 0, q = 0, f = 0;
     for (int i = 0; i < n_seqs; i++) {
         const int n = n_new[i], len = lengths[i], blocks = (len + P - 1) / P;
         // the first position that any new token sees; without new tokens nothing is read
@@ -140,28 +142,33 @@ inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, 
                 snprintf(e->text, sizeof(e->text), "sequence %d, block %d: page %d outside [0, %d)", i, k, page, d.n_pages);
                 return e->code;
             }
-            p->tables[(size_t)i * (size_t)wide + (size_t)k] = page;
+            p->tables[(size_t)(f + k)] = page;
             if (p->uses[(size_t)page] < 2) p->uses[(size_t)page]++;
         }
         p->seqs.push_back({r, n, len, q});
+        p->first.push_back(f);
         r += n;
         q += len;
+        f += blocks;
     }
+    p->first.push_back(f);
     for (int i = 0; i < n_seqs; i++) {
         const SeqPlan& s = p->seqs[(size_t)i];
-        for (int k = s.n_new ? (s.len - s.n_new) / P : 0; s.n_new && k < (s.len + P - 1) / P; k++) {
-            const int32_t page = p->tables[(size_t)i * (size_t)wide + (size_t)k];
+        const int old = s.len - s.n_new;
+        for (int k = old / P; s.n_new && k < (s.len + P - 1) / P; k++) {
+            const int32_t page = p->tables[(size_t)(p->first[(size_t)i] + k)];
             if (p->uses[(size_t)page] > 1) {
                 e->code = FLLM_E_ARG;
                 snprintf(e->text, sizeof(e->text), "sequence %d writes page %d, which the tables name twice", i, page);
                 return e->code;
             }
+            const int lo = std::max(old, k * P), hi = std::min(s.len, k * P + P);
+            p->new_tiles.push_back({lo - k * P, hi - lo, s.row0 + lo - old, page});
         }
     }
     p->n_seqs = n_seqs;
     p->n_rows = r;
     p->n_pos = q;
-    p->tab_w = p->all_blocks = wide;
     return e->code = FLLM_OK;
 }
 
@@ -319,16 +326,17 @@ inline bool attn_plan(const BatchPlan& b, int n_heads, int n_kv, int head_dim, b
             const int g0 = (int)first_image(s), g1 = (s.len - 1) / kKeyStep + 1;
             image = p->images - g0;
             for (int g = g0; g < g1; g += kImageRun)
-                p->image_items.push_back({i * b.tab_w, s.len, (int)low, g * kKeyStep, std::min(kImageRun, g1 - g), (int)(image + g), {0, 0}});
+                p->image_items.push_back({b.first[(size_t)i], s.len, (int)low, g * kKeyStep, std::min(kImageRun, g1 - g), (int)(image + g), {0, 0}});
             p->images += g1 - g0;
         }
         if (s.n_new)
-            attn_items(s, i, i * b.tab_w, (int)image, group, window, c, c >= kAttnMany ? many : std::max(few, join_steps(s, group, window, c, quant)),
+            attn_items(s, i, b.first[(size_t)i], (int)image, group, window, c, c >= kAttnMany ? many : std::max(few, join_steps(s, group, window, c, quant)),
                        &p->items[c], &p->part_rows);
         if (p->part_rows > INT32_MAX / n_kv) return false;
     }
+    if ((int64_t)p->image_items.size() * n_kv >= 1 << 23) return false;
     for (auto& v : p->items) {
-        if ((int64_t)v.size() * n_kv > INT32_MAX) return false;
+        if ((int64_t)v.size() * n_kv >= 1 << 23) return false;  // a grid ends at 2^32 threads
         // the long ones first: the short ones fill the end
         std::stable_sort(v.begin(), v.end(), [](const AttnItem& x, const AttnItem& y) { return x.k1 - x.k0 > y.k1 - y.k0; });
     }

@@ -407,7 +407,7 @@ typedef struct fllm_batch fllm_batch;  /* which positions of which sequences a c
 /* Bytes of the page array. FLLM_E_NOT_SUPPORTED for other types, FLLM_E_ARG for other sizes. */
 FLLM_API int32_t fllm_pages_bytes(const fllm_pages_desc* desc, uint64_t* out);
 /* The page array in mem at `offset` (a multiple of 16), or with mem NULL in memory of its own, which
- * starts as zeros. mem's contents are taken as they are. */
+ * starts as zeros. mem's contents are taken as they are, and it outlives the pages and their batches. */
 FLLM_API int32_t fllm_pages_create(fllm_ctx* ctx, const fllm_pages_desc* desc, fllm_buf* mem, uint64_t offset,
                                    fllm_pages** out);
 /* Calls on the batches of destroyed pages return FLLM_E_DISPOSED; the memory is released when the last
@@ -417,7 +417,7 @@ FLLM_API int32_t fllm_pages_destroy(fllm_pages* p);
 /* A batch for n_heads query heads (a multiple of n_kv_heads; query head h reads kv head
  * h / (n_heads / n_kv_heads)) and a sliding window: a query at position p attends to the positions
  * in (p - window, p] (INT32_MAX: all). One batch serves every layer of a step; models with two kinds of
- * layers keep one for each. */
+ * layers keep one for each. Batches of one context may be used by several threads, each batch by one at a time. */
 FLLM_API int32_t fllm_batch_create(fllm_pages* p, int32_t n_heads, int32_t window, fllm_batch** out);
 /* The sequences of the following calls, replacing earlier ones: sequence i has lengths[i] positions,
  * the last new_tokens[i] of them new (0 is allowed), in the pages tables[i * ld + 0 .. ceil(lengths[i] /

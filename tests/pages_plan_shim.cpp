@@ -27,11 +27,15 @@ extern "C" int64_t plan_images(ImageItem* out, int64_t* total) {
 }
 extern "C" int64_t plan_part_rows() { return g_attn.part_rows; }
 extern "C" void plan_sizes(int32_t* out) {
-    const int32_t v[] = {g_plan.n_seqs, g_plan.n_rows, g_plan.n_pos, g_plan.tab_w, g_plan.new_blocks, g_plan.all_blocks,
-                         g_plan.max_new, g_plan.holes};
+    const int32_t v[] = {g_plan.n_seqs, g_plan.n_rows, g_plan.n_pos, (int32_t)g_plan.tables.size(),
+                         (int32_t)g_plan.new_tiles.size(), (int32_t)g_plan.first.size(), g_plan.max_new, g_plan.holes};
     memcpy(out, v, sizeof(v));
 }
 extern "C" void plan_tables(int32_t* out) {
     if (!g_plan.tables.empty()) memcpy(out, g_plan.tables.data(), g_plan.tables.size() * 4);
+}
+extern "C" void plan_first(int32_t* out) { memcpy(out, g_plan.first.data(), g_plan.first.size() * 4); }
+extern "C" void plan_tiles(PageTile* out) {
+    if (!g_plan.new_tiles.empty()) memcpy(out, g_plan.new_tiles.data(), g_plan.new_tiles.size() * sizeof(PageTile));
 }
 extern "C" int32_t plan_desc(const fllm_pages_desc* d, uint64_t* bytes) { return pages_desc_check(*d, bytes, &g_err); }

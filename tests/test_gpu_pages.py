@@ -556,6 +556,53 @@ def test_operands_that_are_columns_of_one_matrix(make, cache):
             call()
 
 
+def test_one_long_prompt_among_many_decoding_sequences(make):
+    """Sequences of very different lengths in one batch, empty ones among them: rows in, rows out, attention."""
+    new = [1, 0, 700, 1, 1, 0, 0, 1] + [1, 0] * 40
+    length = [3, 0, 5000, 40, 16, 0, 17, 900] + [5, 0] * 40
+    s = make("q8_0", 2, 64, 16, new, length, seed=13)
+    k, v = s.fill()
+    out = [s.put(np.zeros((sum(length), 128)), "f32") for _ in (0, 1)]
+    b = s.batch(4)
+    b.read(1, *out)
+    fresh = [s.put(np.zeros((sum(new), 128)), "f32") for _ in (0, 1)]
+    b.read(1, *fresh, new_only=True)
+    s.ctx.sync()
+    for x, r, f in zip((k, v), out, fresh):
+        assert np.array_equal(s.get(r, "f32"), np.concatenate(x).reshape(-1, 128))
+        assert np.array_equal(s.get(f, "f32"), np.concatenate([a[len(a) - n:] for a, n in zip(x, new)]).reshape(-1, 128))
+    for got, want in attention_of(s, k, v, 4, batch=b):
+        check(got, want, "f32")
+
+
+def test_a_failed_allocation_is_forgotten(ctx):
+    """Memory that cannot be had is refused, and the next calls are not blamed for it."""
+    with pytest.raises(F.OutOfMemoryException):
+        F.PagedKvCache(ctx, F.F16, 1024, 1024, 256, 128, 1 << 20)  # 2^57 bytes
+    with F.PagedKvCache(ctx, F.F16, 1, 1, 32, 16, 2) as p, p.batch(1) as b:
+        b.set([1], [1], [[1]])
+        x = F.DeviceBuffer(ctx, 128)
+        x.write(np.ones(32, np.float32))
+        b.append(0, F.Rows(x, 32), F.Rows(x, 32))
+        ctx.sync()
+        x.close()
+
+
+def test_closed_buffers_are_refused(ctx):
+    mem = F.DeviceBuffer(ctx, F.PagedKvCache.bytes_for(F.F16, 1, 1, 32, 16, 2))
+    p, x = F.PagedKvCache(ctx, F.F16, 1, 1, 32, 16, 2, memory=mem), F.DeviceBuffer(ctx, 128)
+    b, r = p.batch(1), F.Rows(x, 32)
+    b.set([1], [1], [[1]])
+    x.close()
+    with pytest.raises(F.ArgumentNullException):
+        b.append(0, r, r)
+    mem.close()
+    with pytest.raises(F.ObjectDisposedException):
+        b.set([1], [1], [[1]])
+    b.close()
+    p.close()
+
+
 def test_batches_reuse_memory_of_destroyed_ones(make):
     """Batches that come and go while calls on them are under way."""
     s = make("f16", 1, 64, 16, [1, 20], [500, 60], seed=12)

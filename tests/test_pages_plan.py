@@ -49,7 +49,7 @@ def items(so):
 def sizes(so):
     a = np.zeros(8, np.int32)
     so.plan_sizes(a.ctypes.data_as(C.c_void_p))
-    return dict(zip(("seqs", "rows", "pos", "tab_w", "new_blocks", "all_blocks", "max_new", "holes"), a.tolist()))
+    return dict(zip(("seqs", "rows", "pos", "pages", "tiles", "first", "max_new", "holes"), a.tolist()))
 
 
 def test_refusals(lib):
@@ -88,13 +88,14 @@ def check(so, new, length, heads, kv, window):
     group = heads // kv
     seen = {}      # (sequence, row) -> ranges
     parts = set()  # partial rows in use
-    limit, tab_w = so.plan_part_rows(), sizes(so)["tab_w"]
+    limit, first = so.plan_part_rows(), np.zeros(len(new) + 1, np.int32)
+    so.plan_first(first.ctypes.data_as(C.c_void_p))
     for c, list_ in enumerate(items(so)):
         for seq, row0, nrows, k0, k1, part, split, nsplit, tok0, pos0, ln, table in list_[:, :12].tolist():  # noqa: E741
             assert 0 <= seq < len(new) and 0 <= row0 and 1 <= nrows <= TILE[c] and row0 + nrows <= new[seq] * group
             assert 0 <= k0 < k1 <= length[seq] and k0 % STEP == 0 and 0 <= split < nsplit <= SPLIT[c]
             assert k1 % STEP == 0 or split == nsplit - 1
-            assert (tok0, pos0, ln, table) == (sum(new[:seq]), length[seq] - new[seq], length[seq], seq * tab_w)
+            assert (tok0, pos0, ln, table) == (sum(new[:seq]), length[seq] - new[seq], length[seq], first[seq])
             for r in range(row0, row0 + nrows):
                 seen.setdefault((seq, r), []).append((k0, k1))
             if nsplit > 1:
@@ -118,7 +119,7 @@ def check(so, new, length, heads, kv, window):
         seq, row0, k0, k1, image = row[0], row[1], row[3], row[4], row[12]
         for k in range(k0 // STEP, -(-k1 // STEP)):
             tab, at, lo = made[image + k]
-            assert (tab, at) == (seq * tab_w, k * STEP)
+            assert (tab, at) == (first[seq], k * STEP)
             assert lo <= max(0, length[seq] - new[seq] + row0 // group - window + 1)
     for i, (n, ln) in enumerate(zip(new, length)):
         for r in range(n * group):
@@ -149,8 +150,21 @@ def test_items_cover_every_row_and_key_once(lib):
         assert plan(lib, new, length, table, heads, kv, rng.choice([64, 256]), page, max(1, sum(need)), window, rng.choice([1, 64, 256]),
                     rng.choice([N.F16, N.Q8_0, N.Q4_0])) == 0
         s = sizes(lib)
-        assert (s["rows"], s["pos"], s["all_blocks"], s["max_new"]) == (sum(new), sum(length), max(need), max(new))
-        assert s["new_blocks"] == max([0] + [-(-ln // page) - (ln - x) // page for x, ln in zip(new, length) if x])
+        assert (s["rows"], s["pos"], s["pages"], s["max_new"]) == (sum(new), sum(length), sum(need), max(new))
+        pages, first, tiles = np.zeros(sum(need), np.int32), np.zeros(n + 1, np.int32), np.zeros((s["tiles"], 4), np.int32)
+        for name, a in (("tables", pages), ("first", first), ("tiles", tiles)):
+            getattr(lib, "plan_" + name)(a.ctypes.data_as(C.c_void_p))
+        assert s["first"] == n + 1 and first.tolist() == np.cumsum([0] + need).tolist()
+        assert pages.tolist() == [x for row, k in zip(table, need) for x in row[:k]]
+        rows = 0  # the tiles are the new tokens in order, a page each
+        tiles = tiles.tolist()
+        for i, (x, ln) in enumerate(zip(new, length)):
+            at = ln - x
+            while at < ln:
+                off, m, row, pg = tiles.pop(0)
+                assert (off, row, pg) == (at % page, rows, table[i, at // page]) and m == min(page - off, ln - at)
+                at, rows = at + m, rows + m
+        assert not tiles
         check(lib, new, length, heads, kv, window)
 
 
