@@ -57,7 +57,7 @@ union H8 {
 // -inf, times zero it would be a NaN): a scale of zero makes q zero.
 __device__ __forceinline__ float scale_sign(float s) { return s < 0.0f ? -1.0f : s > 0.0f ? 1.0f : 0.0f; }
 __device__ __forceinline__ float scale_size(float s, int e, float softcap) {
-    return fmaxf(ldexpf(s == 0.0f ? 1.0f : fabsf(s), -e) * (softcap > 0.0f ? 1.0f / softcap : kLog2e), 1e-37f);
+    return fminf(fmaxf(ldexpf(s == 0.0f ? 1.0f : fabsf(s), -e) * (softcap > 0.0f ? 1.0f / softcap : kLog2e), 1e-37f), 3e38f);
 }
 
 // 4 bytes, each code + 128 or nibble, as fp16 integers: 0x6400 | byte is 1024 + byte exactly
@@ -821,6 +821,8 @@ struct Codes {
                 x.u &= keep;
                 y.u &= keep;
             }
+            const us2 nan = (us2)(x.h >= us2{0x7C00, 0x7C00});  // no unit: only its own key's scores are lost
+            x.h &= ~nan;
             tk = __builtin_elementwise_max(tk, x.h);
             tv = __builtin_elementwise_max(tv, y.h);
         }

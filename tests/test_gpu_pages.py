@@ -758,6 +758,24 @@ def test_attention_of_far_scores(make, cache, new, length):
         check(got, want, "f32")
 
 
+@pytest.mark.parametrize("cache", TYPES)
+@pytest.mark.parametrize("kv,heads,hd,new", [(2, 8, 64, 5), (1, 2, 128, 100), (1, 12, 128, 100), (1, 10, 256, 100)])
+def test_a_key_that_is_no_number_is_its_own_querys_matter(make, cache, kv, heads, hd, new):
+    """The last token's key is NaN: the tokens before it do not see it; itself and nobody else gets NaN."""
+    s = make(cache, kv, hd, 32, [new], [new + 20], seed=14)
+    k, v = s.fill()
+    b, n = s.batch(kv), new
+    x = [np.concatenate([a[0][20:]]).reshape(n, kv * hd).astype(np.float32) for a in (k, v)]
+    x[0][-1, 7] = np.nan
+    b.append(1, s.put(x[0], "f32"), s.put(x[1], "f32"))
+    k, v = ([np.concatenate([a[0][:20], stored(y, cache).reshape(n, kv, hd)])] for a, y in zip((k, v), x))
+    for scale, softcap in ((0.1, 0.0), (0.1, 30.0), (1e10, 1e-30)):
+        for got, want in attention_of(s, k, v, heads, scale=scale, softcap=softcap):
+            check(got[:-1], want[:-1], "f32")
+            group = heads // kv
+            assert np.isnan(got[-1].reshape(heads, hd)[:group]).all()
+
+
 @pytest.mark.parametrize("cache,act", [("f16", "f32"), ("q8_0", "bf16"), ("q4_0", "f32")])
 def test_the_same_call_gives_the_same_bits(make, cache, act):
     s = make(cache, 2, 128, 64, [1, 5, 100], [3000, 700, 400], seed=6)
