@@ -8,7 +8,7 @@
 // and a thread turns 4 rows by 16 positions in registers (byte permutes), so that the pages are read and written 16
 // bytes at a time too. Measured: 8 sequences of 3000 to 16000 positions, 8 heads of 256, Q8_0 to F16 rows: 825 MB in
 // 203 us (4.1 TB/s; a 1 GiB copy reaches 5.1); four prompts of 900 to 4000 rows, 4 heads of 128, F32 to Q4_0 and back:
-// 73 MB in 22.9 us, two launches; one row of 64 sequences in and out: 8.7 us, of which two empty launches are 7.4.
+// 73 MB in 21.8 us, two launches; one row of 64 sequences in and out: 8.7 us, of which two empty launches are 7.4.
 #include "pages.hpp"
 
 namespace fllm {

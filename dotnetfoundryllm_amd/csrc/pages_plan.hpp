@@ -83,7 +83,7 @@ struct BatchPlan {
     std::vector<int32_t> first;          // where each sequence's pages start in `tables`; their number
     std::vector<int32_t> tables;         // the sequences' pages one after the other, 0 where there is none
     std::vector<PageTile> new_tiles;
-    std::vector<uint8_t> uses;           // scratch: places that name a page (up to 2)
+    std::vector<uint8_t> uses;           // places that name a page (up to 2); zeros between calls
 };
 
 // Fills `p` from the arrays of fllm_batch_set, or says what is wrong with them.
@@ -121,8 +121,14 @@ inline int32_t batch_plan(const fllm_pages_desc& d, int window, int32_t n_seqs, 
         snprintf(e->text, sizeof(e->text), "tables of %lld pages a sequence, %d are needed", (long long)ld, wide);
         return e->code;
     }
-    p->uses.assign((size_t)d.n_pages, 0);
+    p->uses.resize((size_t)d.n_pages);
     p->tables.assign((size_t)all, 0);  // at most n_pos
+    struct Clear {  // what the tables name, not all pages: there may be millions
+        BatchPlan* p;
+        ~Clear() {
+            for (const int32_t page : p->tables) p->uses[(size_t)page] = 0;
+        }
+    } clear{p};
     p->seqs.reserve((size_t)n_seqs);
     p->first.reserve((size_t)n_seqs + 1);
     int r = 0, q = 0, f = 0;
