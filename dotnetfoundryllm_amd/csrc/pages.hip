@@ -36,15 +36,16 @@ __device__ __forceinline__ Tile tile_of(const PagesView& pg, const BatchView& b,
         t.row = q.z;
         page = q.w;
     } else {
-        int s = 0;  // the last sequence whose pages start at `at` or before
+        int s = 0, start = 0;  // the last sequence whose pages start at `at` or before, and where they do
         for (int n = b.n_seqs; n > 1;) {
             const int step = (n + 63) >> 6, i = (int)(threadIdx.x & 63) * step;
-            const int k = __builtin_popcountll(__ballot(i < n && b.first[s + (i < n ? i : 0)] <= at)) - 1;
+            const int f = b.first[s + (i < n ? i : 0)], k = __builtin_popcountll(__ballot(i < n && f <= at)) - 1;
+            start = __builtin_amdgcn_readlane(f, k);
             s += k * step;
             n = min(step, n - k * step);
         }
         const int4 q = b.seqs[s];
-        const int pos = (at - (b.n_seqs > 1 ? b.first[s] : 0)) << pg.page_log2;
+        const int pos = (at - start) << pg.page_log2;
         t.off = 0;
         t.n = min(q.z - pos, 1 << pg.page_log2);
         t.row = (int64_t)q.w + pos;
