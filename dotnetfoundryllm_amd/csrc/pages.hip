@@ -7,8 +7,8 @@
 // positions along the row (what the attention's second product reads): its codes pass through LDS as [position][row],
 // and a thread turns 4 rows by 16 positions in registers (byte permutes), so that the pages are read and written 16
 // bytes at a time too. Measured: 8 sequences of 3000 to 16000 positions, 8 heads of 256, Q8_0 to F16 rows: 825 MB in
-// 203 us (4.1 TB/s; a 1 GiB copy reaches 5.1); four prompts of 900 to 4000 rows, 4 heads of 128, F32 to Q4_0 and back:
-// 73 MB in 21.8 us, two launches; one row of 64 sequences in and out: 8.7 us, of which two empty launches are 7.4.
+// 202 us (4.1 TB/s; a 1 GiB copy reaches 5.1); four prompts of 900 to 4000 rows, 4 heads of 128, F32 to Q4_0 and back:
+// 73 MB in 21.8 us, two launches; one row of 64 sequences in and out: 8.9 us, of which two empty launches are 7.4.
 #include "pages.hpp"
 
 namespace fllm {
@@ -25,7 +25,7 @@ struct Tile {
 };
 
 // Tile `at` of the new tokens, one load away, or of all positions: page `at` of the sequences' pages, whose sequence a wave
-// finds with one load for up to 64 of them (203 us of the case at grid_of; 212 by halving).
+// finds with one load for up to 64 of them (202 us of the case at grid_of; 212 by halving).
 __device__ __forceinline__ Tile tile_of(const PagesView& pg, const BatchView& b, bool new_only, int at, int head) {
     Tile t;
     int page;
@@ -334,8 +334,8 @@ int log2_up(int n) {
 int threads_for(const PagesView& pg, int rows) { return rows * (pg.hd >> 5) <= 32 ? 64 : 256; }
 
 // The heads of a page follow each other, so that what lies side by side in the dense rows moves at the same time
-// (8 sequences of 3000 to 16000 positions, 8 heads of 256, Q8_0 to F16: 217 us, and 249 with the pages of a head in
-// a row). The second dimension ends at 65535: the kernels go on from there.
+// (8 sequences of 3000 to 16000 positions, 8 heads of 256, Q8_0 to F16: 249 us with the pages of a head in a row, then
+// 217). The second dimension ends at 65535: the kernels go on from there.
 dim3 grid_of(const PagesView& pg, int tiles) { return dim3(2 * pg.nkv, tiles < 65535 ? tiles : 65535); }
 
 template <int TYPE>

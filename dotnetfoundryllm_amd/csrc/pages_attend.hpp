@@ -1241,7 +1241,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // k_attend_wide: the same for heads wider than 128, whose q and o would take all of a 32-row wave's registers: eight
 // waves of 16 rows on the 16x16x32 products, two to a SIMD, so that one multiplies while the other reads. S^T tiles and
 // operands are k_attend_few's: a lane holds the keys 8 g .. + 8 of a step of 32. Every wave reads all of K and V from
-// LDS, which bounds it (4096 cycles a step of 64 KB for 3072 of products). Measured: 2047 rows over a window of 4096, 16 over
+// LDS, which bounds it (4096 cycles a step of 64 KB, a third more than its products). Measured: 2047 rows over a window of 4096, 16 over
 // 8 heads of 256, Q8_0, F32 rows (three products of halves for one): 137 GFLOP in 417 us, 35 of them the images; 537 us with
 // four waves of 32 rows, whose registers spill.
 template <int TYPE, int NP, int SRC>
